@@ -390,6 +390,91 @@ int spr_repair_apply(const void* base, const float* x_mean, const float* x_scale
                      float alpha, const int32_t* rows, const void* dense, int m, void* out,
                      void* stream);
 
+/* ---------------------------------------------------------------- adaLN */
+
+/*
+ * Operands of the modulated layer norm with an optional gated residual in front
+ * of it.  For every row (b, t) of [batch][tokens][channels]:
+ *   z = x + gate*y       (only when y != NULL; gate == NULL counts as 1; the product
+ *                         and the sum are each rounded to fp32, z to the element type)
+ *   n = (z - mean z) * rstd,  rstd = 1/sqrt(var z + eps)      (z = x when y == NULL)
+ *   h = n*(scale_offset + scale) + shift                      (one rounding)
+ * scale == NULL counts as 1 - scale_offset, shift == NULL as 0.  x, y, z, h and their
+ * gradients have element type `dtype`; shift, scale, gate and their gradients
+ * have `mod_dtype` (`dtype` or SPR_F32).  Channels are contiguous; *_sb and
+ * *_st are the element strides of the batch and token axes.  The strides of
+ * shift, scale and gate may be 0 (broadcast along that axis), the same axes for
+ * all three.  z and h are dense.  mean and rstd [batch*tokens] fp32 (nullable)
+ * are what the backward pass needs.  1 <= channels <= 16384.
+ */
+typedef struct SprAdaln {
+  int dtype, mod_dtype;
+  int64_t batch, tokens;
+  int channels;
+  float eps, scale_offset;
+  const void *x, *y;
+  const void *shift, *scale, *gate;
+  int64_t x_sb, x_st, y_sb, y_st;
+  int64_t shift_sb, shift_st, scale_sb, scale_st, gate_sb, gate_st;
+  void *z, *h;
+  float *mean, *rstd;
+} SprAdaln;
+
+/* The forward pass.  No counterpart in the reference (its adapters leave the
+ * norms and residuals to the model library). */
+int spr_adaln_forward(const SprAdaln* op, void* stream);
+
+/*
+ * The backward pass: op->x holds the stored z of the forward pass when
+ * op->y != NULL (op->z, op->h are not read), op->mean and op->rstd its
+ * statistics.  dh and dz (nullable: no gradient) with their strides; outputs
+ * dx and dy dense [batch][tokens][channels] (dy only with y), and the gradients
+ * of the vectors summed over the rows that share one, dense
+ * [groups][channels] in mod_dtype, where groups = the product of the axes that
+ * shift/scale/gate are not broadcast along; mod_batch and mod_tokens say which
+ * axes those are (1: kept, 0: summed).  dshift, dscale and dgate are nullable
+ * (not formed).  The sums run in a fixed order.  workspace:
+ * spr_adaln_backward_workspace_bytes(op's sizes).
+ */
+typedef struct SprAdalnGrad {
+  const void *dh, *dz;
+  int64_t dh_sb, dh_st, dz_sb, dz_st;
+  void *dx, *dy;
+  void *dshift, *dscale, *dgate;
+  int mod_batch, mod_tokens;
+} SprAdalnGrad;
+size_t spr_adaln_backward_workspace_bytes(int64_t batch, int64_t tokens, int channels, int mod_batch, int mod_tokens);
+int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* ---------------------------------------------------------------- 4-bit weights */
+
+/*
+ * y[r][n] = sum_k x[r][k] * (code[n][k] - zero[n][k/group]) * scale[n][k/group] + bias[n]
+ * for a few rows r (a conditioning vector per sample).  packed [n][groups*group/2]
+ * u8: two codes (0..15) per byte, the even column in the low half; scales
+ * [n][groups] (scale_dtype); zeros [n][groups] u8 (nullable: 8); bias [n]
+ * (dtype, nullable).  groups = ceil(k/group), group a multiple of 32; codes of
+ * columns >= k are ignored.  x [rows][k] (row stride x_stride elements), y
+ * [rows][n] dense, both `dtype`; sums in fp32, one rounding.  packed must be
+ * 16-byte aligned.  workspace: spr_int4_linear_workspace_bytes (0 is possible).
+ * No counterpart in the reference.
+ */
+size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype);
+int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64_t rows, int64_t n, int64_t k, int group,
+                    const uint8_t* packed, const void* scales, int scale_dtype, const uint8_t* zeros,
+                    const void* bias, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The gradient with respect to x: dx[r][k] = sum_n dy[r][n] * scale * (code - zero)
+ * (dy [rows][n], row stride dy_stride; dx [rows][k] dense).  Same weights,
+ * same types; the sums run in a fixed order.
+ */
+size_t spr_int4_linear_grad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype);
+int spr_int4_linear_grad(const void* dy, int64_t dy_stride, int dtype, int64_t rows, int64_t n, int64_t k, int group,
+                         const uint8_t* packed, const void* scales, int scale_dtype, const uint8_t* zeros, void* dx,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,10 @@ Public API:
 * :func:`sparse_attention` — the adapter-facing attention call.
 * :class:`RouteCache` — route reuse across steps and CFG branches.
 * :func:`batch_kmeans_Euclid`, :class:`FlashKMeans` — standalone batched k-means.
+* :func:`layer_norm`, :func:`modulated_layer_norm`, :func:`gated_residual_layer_norm` —
+  the adaptive layer norms of a DiT block, with gradients.
+* :func:`int4_linear`, :func:`quantize_int4`, :func:`dequantize_int4` — products of a
+  few rows with 4-bit weights.
 * :func:`check_status` — raise if a device-side bounded wait of the last layer gave up.
 * :mod:`sparsepr_b200.kernels` — tensor wrappers over the C ABI.
 """
@@ -23,6 +27,8 @@ from .attention import (  # noqa: F401
 )
 from .route_cache import RouteCache, RouteReuseConfig, route_action  # noqa: F401
 from .kmeans import FlashKMeans, batch_kmeans_Euclid  # noqa: F401
+from .adaln import gated_residual_layer_norm, layer_norm, modulated_layer_norm  # noqa: F401
+from .int4 import Int4Weight, dequantize_int4, int4_linear, quantize_int4  # noqa: F401
 from .kernels import wan_qkv_norm_rope_layout  # noqa: F401
 
 

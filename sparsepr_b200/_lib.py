@@ -63,6 +63,13 @@ PROTOTYPES = {
     "spr_sym_eig": (_I, [_P, _I64, _I, _I, _P, _P, _P]),
     "spr_sym_eig_top": (_I, [_P, _I64, _I, _I, _I, _P, _P, _P]),
     "spr_chol_solve": (_I, [_P, _P, _I64, _I, _I, _P, _P]),
+    "spr_adaln_forward": (_I, [_P, _P]),
+    "spr_adaln_backward_workspace_bytes": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "spr_adaln_backward": (_I, [_P, _P, _P, _SZ, _P]),
+    "spr_int4_linear_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I]),
+    "spr_int4_linear": (_I, [_P, _I64, _I, _I64, _I64, _I64, _I, _P, _P, _I, _P, _P, _P, _P, _SZ, _P]),
+    "spr_int4_linear_grad_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I]),
+    "spr_int4_linear_grad": (_I, [_P, _I64, _I, _I64, _I64, _I64, _I, _P, _P, _I, _P, _P, _P, _SZ, _P]),
     "spr_repair_apply": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I, _I, _F, _P, _P, _I, _P, _P]),
 }
 
@@ -71,6 +78,24 @@ class SprRepairState(C.Structure):
 
     _fields_ = [("x_mean", _P), ("x_scale", _P), ("y_mean", _P), ("left", _P), ("basis", _P), ("rank", _I),
                 ("alpha", _F), ("probe_rows", _P), ("probe_dense", _P), ("m", _I)]
+
+
+class SprAdaln(C.Structure):
+    """``SprAdaln`` of include/sparsepr_b200.h."""
+
+    _fields_ = [("dtype", _I), ("mod_dtype", _I), ("batch", _I64), ("tokens", _I64), ("channels", _I), ("eps", _F),
+                ("scale_offset", _F), ("x", _P), ("y", _P), ("shift", _P), ("scale", _P), ("gate", _P),
+                ("x_sb", _I64), ("x_st", _I64), ("y_sb", _I64), ("y_st", _I64), ("shift_sb", _I64),
+                ("shift_st", _I64), ("scale_sb", _I64), ("scale_st", _I64), ("gate_sb", _I64), ("gate_st", _I64),
+                ("z", _P), ("h", _P), ("mean", _P), ("rstd", _P)]
+
+
+class SprAdalnGrad(C.Structure):
+    """``SprAdalnGrad`` of include/sparsepr_b200.h."""
+
+    _fields_ = [("dh", _P), ("dz", _P), ("dh_sb", _I64), ("dh_st", _I64), ("dz_sb", _I64), ("dz_st", _I64),
+                ("dx", _P), ("dy", _P), ("dshift", _P), ("dscale", _P), ("dgate", _P), ("mod_batch", _I),
+                ("mod_tokens", _I)]
 
 
 _lock = threading.Lock()

@@ -1,0 +1,106 @@
+"""Linear layers with 4-bit weights under group scales, for a few rows.
+
+A diffusion transformer makes every block's modulation from one conditioning
+vector per sample: a product that reads its whole weight for one or two rows, so
+its time is the weight's bytes.  :func:`quantize_int4` stores a weight in 4 bits,
+:func:`int4_linear` multiplies rows by it (its gradient goes to the rows and the
+bias; the codes are frozen), :func:`dequantize_int4` gives the weight back.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels as K
+
+__all__ = ["Int4Weight", "quantize_int4", "dequantize_int4", "int4_linear"]
+
+
+class Int4Weight(NamedTuple):
+    """``packed`` uint8 [N, groups*group/2] (two codes a byte, the even column in the low
+    half), ``scales`` [N, groups], ``zeros`` uint8 [N, groups] or None (8)."""
+
+    packed: torch.Tensor
+    scales: torch.Tensor
+    zeros: torch.Tensor | None
+
+
+def quantize_int4(weight: torch.Tensor, group_size: int = 64, symmetric: bool = False,
+                  scale_dtype: torch.dtype | None = None) -> Int4Weight:
+    """4-bit codes of a [N, K] weight by round to nearest, on the weight's device.
+
+    Each run of ``group_size`` columns (a multiple of 32; the last may be partly
+    used) has a scale in ``scale_dtype`` (default: the weight's type) and, unless
+    ``symmetric``, a zero code; the codes are those nearest under the stored scale."""
+    if weight.dim() != 2 or weight.dtype not in K._DT or weight.numel() == 0:
+        raise RuntimeError(f"quantize_int4 expects a non-empty fp32/bf16/fp16 [N, K] weight, got "
+                           f"{tuple(weight.shape)} {weight.dtype}")
+    if group_size < 32 or group_size % 32:
+        raise ValueError(f"group_size must be a positive multiple of 32, got {group_size}")
+    sdt = weight.dtype if scale_dtype is None else scale_dtype
+    if sdt not in K._DT:
+        raise ValueError(f"scale_dtype must be fp32/bf16/fp16, got {sdt}")
+    n, k = weight.shape
+    groups = -(-k // group_size)
+    w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group_size - k)).view(n, groups, group_size)
+    lo, hi = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
+    step = torch.maximum(-lo, hi) / 7.0 if symmetric else (hi - lo) / 15.0
+    scales = step.clamp(min=torch.finfo(sdt).tiny).to(sdt)  # normal numbers, groups of zeros among them
+    s = scales.float()
+    zeros = None if symmetric else (-lo / s).round().clamp(0, 15).to(torch.uint8)
+    codes = ((w / s[..., None]).round() + (8.0 if symmetric else zeros.float()[..., None])).clamp(0, 15)
+    codes = codes.to(torch.uint8).view(n, groups * group_size)
+    return Int4Weight(codes[:, 0::2] | (codes[:, 1::2] << 4), scales, zeros)
+
+
+def dequantize_int4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, in_features: int,
+                    dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The [N, in_features] weight that the codes stand for."""
+    n, groups = scales.shape
+    codes = torch.stack((packed & 15, packed >> 4), dim=-1).view(n, groups, -1).float()
+    w = (codes - (8.0 if zeros is None else zeros.float()[..., None])) * scales.float()[..., None]
+    return w.view(n, -1)[:, :in_features].to(dtype)
+
+
+class _Int4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, packed, scales, zeros, bias):
+        ctx.save_for_backward(packed, scales, zeros)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.in_features = x.shape[1]
+        return K.int4_linear(x, packed, scales, zeros, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        packed, scales, zeros = ctx.saved_tensors
+        dx = dbias = None
+        if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
+            dy = dy.contiguous()
+        if ctx.needs_input_grad[0]:
+            dx = K.int4_linear_grad(dy, packed, scales, zeros, ctx.in_features)
+        if ctx.needs_input_grad[4]:
+            dbias = dy.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+        return dx, None, None, None, dbias
+
+
+def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+                bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ W.T + bias`` with the 4-bit weight ``W`` [N, K] of :func:`quantize_int4`.
+
+    ``x`` [..., K] in fp32, bf16 or fp16 and ``bias`` [N] in x's type; the result [..., N]
+    is rounded once from fp32 sums.  Any number of rows is computed, but the
+    weights are read once for each block of rows: the call is for a few rows."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"int4_linear: x must be [..., K], got {tuple(x.shape)}")
+    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
+        rows = rows.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        y = _Int4Linear.apply(rows, packed, scales, zeros, bias)
+    else:
+        y = K.int4_linear(rows, packed, scales, zeros, bias)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], packed.shape[0])

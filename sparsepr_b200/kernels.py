@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import contextlib
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -562,3 +564,141 @@ def ridge_cholesky(a: torch.Tensor, scale: torch.Tensor, relative_ridge: float, 
     _lib.call("spr_ridge_cholesky", _p(ac), _p(sc), b, m, float(relative_ridge), float(fallback_ridge), _p(l),
               _p(failed), _stream(dev))
     return l, failed.bool()
+
+
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """``_lib.call`` on ``dev``'s current stream, also where another device is current."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(dev))
+
+
+def _bt(t: torch.Tensor | None) -> tuple[int, int]:
+    """Element strides of the batch and token axes of a [B or 1, N or 1, C] view (0: broadcast)."""
+    if t is None:
+        return 0, 0
+    (b, n, _c), (sb, st, _sc) = t.shape, t.stride()
+    return (sb if b > 1 else 0), (st if n > 1 else 0)
+
+
+def _adaln_op(x, y, gate, shift, scale, eps, scale_offset, z, h, mean, rstd) -> _lib.SprAdaln:
+    mod = next((m for m in (shift, scale, gate) if m is not None), None)
+    b, n, c = x.shape
+    return _lib.SprAdaln(_DT[x.dtype], _DT[x.dtype if mod is None else mod.dtype], b, n, c, eps, scale_offset, _p(x),
+                         _p(y), _p(shift), _p(scale), _p(gate), *_bt(x), *_bt(y), *_bt(shift), *_bt(scale),
+                         *_bt(gate), _p(z), _p(h), _p(mean), _p(rstd))
+
+
+def adaln_forward(x, y, gate, shift, scale, eps: float, scale_offset: float, stats: bool):
+    """Modulated layer norm of [B,N,C] rows with an optional gated residual (``y``):
+    ``z = x + gate*y``, ``h = LN(z)*(scale_offset + scale) + shift``.
+
+    ``shift``, ``scale`` and ``gate`` are [B or 1, N or 1, C] views of one type (the
+    rows' or fp32) or None.  Returns ``(z, h, mean, rstd)``, ``z`` None without ``y``
+    and the row statistics fp32 [B*N] or None without ``stats``.  The shapes are
+    checked by :mod:`sparsepr_b200.adaln`."""
+    dev = _cuda(x, y, gate, shift, scale)
+    b, n, c = x.shape
+    h = torch.empty((b, n, c), dtype=x.dtype, device=dev)
+    z = None if y is None else torch.empty_like(h)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty((2, b * n), dtype=torch.float32, device=dev).unbind(0)
+    op = _adaln_op(x, y, gate, shift, scale, eps, scale_offset, z, h, mean, rstd)
+    _count(1)
+    _launch(dev, "spr_adaln_forward", ctypes.addressof(op))
+    return z, h, mean, rstd
+
+
+def adaln_backward(x, y, gate, scale, mean, rstd, dh, dz, scale_offset: float, needs=(True, True, True),
+                   mod_shape=(1, 1), mod_dtype: torch.dtype | None = None):
+    """Backward pass of :func:`adaln_forward` from its ``z`` (``x`` without a branch) and
+    row statistics: ``(dx, dy, dgate, dshift, dscale)``.
+
+    ``needs`` says which of (dgate, dshift, dscale) are formed; they are
+    ``mod_shape + (C,)`` with ``mod_shape`` (B or 1, N or 1) and summed over the
+    axes of extent 1, in a fixed order.  The workspace belongs to this call alone,
+    so that calls on several streams and captured graphs share none."""
+    dev = _cuda(x, y, gate, scale, mean, rstd, dh, dz)
+    b, n, c = x.shape
+    mdt = x.dtype if mod_dtype is None else mod_dtype
+    dx = torch.empty((b, n, c), dtype=x.dtype, device=dev)
+    dy = None if y is None else torch.empty_like(dx)
+    keep = (int(mod_shape[0] > 1), int(mod_shape[1] > 1))
+    dgate, dshift, dscale = (torch.empty((*mod_shape, c), dtype=mdt, device=dev) if need else None for need in needs)
+    if b * n == 0:
+        for t in (dgate, dshift, dscale):
+            if t is not None:
+                t.zero_()
+        return dx, dy, dgate, dshift, dscale
+    op = _adaln_op(x, y, gate, None, scale, 0.0, scale_offset, None, None, mean, rstd)
+    op.mod_dtype = _DT[mdt]
+    gr = _lib.SprAdalnGrad(_p(dh), _p(dz), *_bt(dh), *_bt(dz), _p(dx), _p(dy), _p(dshift), _p(dscale), _p(dgate),
+                           *keep)
+    nbytes = _lib.query("spr_adaln_backward_workspace_bytes", b, n, c, *keep)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _count(2)
+    _launch(dev, "spr_adaln_backward", ctypes.addressof(op), ctypes.addressof(gr), _p(ws), nbytes)
+    return dx, dy, dgate, dshift, dscale
+
+
+def _int4_checks(what, rows2d, length, packed, scales, zeros):
+    """(n, k rounded up to whole groups, group) of the weights; raises on what the kernels do not take."""
+    if rows2d.dtype not in _DT or scales.dtype not in _DT:
+        raise RuntimeError(f"{what}: rows and scales must be fp32/bf16/fp16, got {rows2d.dtype} and {scales.dtype}")
+    if packed.dtype != torch.uint8 or packed.dim() != 2 or scales.dim() != 2 or scales.shape[0] != packed.shape[0]:
+        raise RuntimeError(f"{what}: packed codes must be uint8 [N, K/2] and scales [N, groups], got {packed.dtype} "
+                           f"{tuple(packed.shape)} and {tuple(scales.shape)}")
+    n, kp, groups = packed.shape[0], 2 * packed.shape[1], scales.shape[1]
+    if groups == 0 or kp % (32 * groups):
+        raise RuntimeError(f"{what}: {kp} codes a row in {groups} groups; a group must be a multiple of 32 codes")
+    group = kp // groups
+    if not kp - group < length <= kp:
+        raise RuntimeError(f"{what}: {length} input features do not end in the last of {groups} groups of {group}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise RuntimeError(f"{what}: zeros must be uint8 {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
+    for name, t in (("packed", packed), ("scales", scales), ("zeros", zeros)):
+        if t is not None:
+            _contig(f"{what}: {name}", t)
+    if rows2d.shape[1] > 1 and rows2d.stride(1) != 1:
+        raise RuntimeError(f"{what}: the last dimension must be contiguous, got strides {rows2d.stride()}")
+    return n, group
+
+
+def int4_linear(x, packed, scales, zeros=None, bias=None) -> torch.Tensor:
+    """``y[r,n] = sum_k x[r,k]*(code[n,k] - zero[n,k//group])*scale[n,k//group] + bias[n]``
+    for a few rows ``x`` [R,K] (row stride free) -> [R,N] in x's type.
+
+    ``packed`` uint8 [N, groups*group/2]: two 4-bit codes a byte, the even column in
+    the low half; ``scales`` [N, groups]; ``zeros`` uint8 [N, groups] (None: 8).  The
+    group size is a multiple of 32; codes of columns >= K are ignored."""
+    dev = _cuda(x, packed, scales, zeros, bias)
+    r, k = x.shape
+    n, group = _int4_checks("int4_linear", x, k, packed, scales, zeros)
+    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or (n > 1 and bias.stride(0) != 1)):
+        raise RuntimeError(f"int4_linear: bias must be contiguous {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
+    y = torch.empty((r, n), dtype=x.dtype, device=dev)
+    nbytes = _lib.query("spr_int4_linear_workspace_bytes", r, n, k, group, _DT[x.dtype])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _count(1)
+    _launch(dev, "spr_int4_linear", _p(x), x.stride(0), _DT[x.dtype], r, n, k, group, _p(packed), _p(scales),
+            _DT[scales.dtype], _p(zeros), _p(bias), _p(y), _p(ws), nbytes)
+    return y
+
+
+def int4_linear_grad(dy, packed, scales, zeros, in_features: int) -> torch.Tensor:
+    """Gradient of :func:`int4_linear` with respect to its rows: ``dy`` [R,N] -> [R, in_features]."""
+    dev = _cuda(dy, packed, scales, zeros)
+    n, group = _int4_checks("int4_linear_grad", dy, in_features, packed, scales, zeros)
+    r = dy.shape[0]
+    if dy.shape[1] != n:
+        raise RuntimeError(f"int4_linear_grad: dy {tuple(dy.shape)} does not match {n} weight rows")
+    dx = torch.empty((r, in_features), dtype=dy.dtype, device=dev)
+    nbytes = _lib.query("spr_int4_linear_grad_workspace_bytes", r, n, in_features, group, _DT[dy.dtype])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _count(1)
+    _launch(dev, "spr_int4_linear_grad", _p(dy), dy.stride(0), _DT[dy.dtype], r, n, in_features, group, _p(packed),
+            _p(scales), _DT[scales.dtype], _p(zeros), _p(dx), _p(ws), nbytes)
+    return dx
