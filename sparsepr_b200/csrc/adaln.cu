@@ -4,6 +4,8 @@
 //   u = dh*w,  g = dz + rstd*(u - mean u - n*mean(u*n)),  dx = g,  dy = g*gate
 //   dshift = sum dh,  dscale = sum dh*n,  dgate = sum g*y   over the rows of a group
 // Statistics and sums are fp32.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace spr {
@@ -150,25 +152,22 @@ __device__ __forceinline__ void store_row(T* p, const Vals<V>& f) {
 // A row belongs to a team of threads: a power of two of lanes up to 32 (several
 // teams to a warp, no barrier), or a whole CTA of several warps.
 __device__ __forceinline__ float team_sum(float v, int team) {
-  for (int o = min(team, 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < team) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 __device__ __forceinline__ uint64_t team_sum2(uint64_t v, int team) {
-  for (int o = min(team, 32) / 2; o > 0; o >>= 1) v = add2(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ uint64_t warp_sum2(uint64_t v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = add2(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < team) v = add2(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
 // Two sums over a CTA's warps with one barrier.  Two buffers in turn: a warp that
 // writes the next row's pair does not meet readers of this row's.  `red` starts
 // as zeros, so an odd number of warps reads a zero pair.
-__device__ __forceinline__ uint64_t warps_sum2(uint64_t v, ulonglong2* red, int warps) {
-  if ((threadIdx.x & 31) == 0) reinterpret_cast<uint64_t*>(red)[threadIdx.x >> 5] = v;
-  __syncthreads();
+__device__ __forceinline__ uint64_t join_warps(const ulonglong2* red, int warps) {
   uint64_t a = 0, b = 0;
 #pragma unroll 4
   for (int w = 0; w < (warps + 1) / 2; ++w) {
@@ -177,6 +176,11 @@ __device__ __forceinline__ uint64_t warps_sum2(uint64_t v, ulonglong2* red, int 
     b = add2(b, e.y);
   }
   return add2(a, b);
+}
+__device__ __forceinline__ uint64_t warps_sum2(uint64_t v, ulonglong2* red, int warps) {
+  if ((threadIdx.x & 31) == 0) reinterpret_cast<uint64_t*>(red)[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return join_warps(red, warps);
 }
 
 // The residual stream: product and sum rounded to fp32 one after the other, so
@@ -218,10 +222,64 @@ __device__ __forceinline__ void load_gate(const SprAdaln& op, const RowId& id, i
   else w.fill(1.f);
 }
 
-// One row per team.  The row stays in registers; the variance is taken about the
-// warp's own mean and the warps' values are joined by
+// The rows that share one vector: row r of group g is g*group_step + r*row_step.
+// A group's rows are cut into `chunks` runs; run s of group g writes its column
+// sums to partial[g][s] (or, with one run, the gradients themselves).
+struct Groups {
+  int64_t count, rows, group_step, row_step;
+  int chunks;
+  int64_t chunk_rows;
+};
+
+__device__ __forceinline__ void copy16_async(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+
+// Mean and 1/sqrt(var + eps) of a row that a team holds.  The variance is taken about
+// the warp's own mean and the warps' values are joined by
 //   M2 = sum_w M2_w + n_w (mean_w - mean)^2,
 // so that a row costs one barrier and loses nothing to an offset.
+template <int V, int P>
+__device__ __forceinline__ float2 row_stats(const Vals<V> (&z)[P], int lane, int team, int nvec, float inv_c, float eps,
+                                            float4* red) {
+  const int first = lane & ~31, width = min(team, 32);  // the warp's vectors in its team
+  int n = 0;
+  uint64_t acc[2] = {0, 0};
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    n += min(max(nvec - first - p * team, 0), width) * V;
+#pragma unroll
+    for (int i = 0; i < Vals<V>::kPairs; ++i) acc[i & 1] = add2(acc[i & 1], z[p].q[i]);
+  }
+  float2 h = halves(add2(acc[0], acc[1]));
+  const float sum = team_sum(h.x + h.y, team);
+  float mean = sum * __frcp_rn((float)n);
+  const uint64_t minus = both<V>(-mean);
+  acc[0] = acc[1] = 0;
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (lane + p * team < nvec)
+#pragma unroll
+      for (int i = 0; i < Vals<V>::kPairs; ++i) {
+        const uint64_t d = add2(z[p].q[i], minus);
+        acc[i & 1] = fma2(d, d, acc[i & 1]);
+      }
+  h = halves(add2(acc[0], acc[1]));
+  float m2 = team_sum(h.x + h.y, team);
+  if (team > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float4(sum, mean, m2, (float)n);
+    __syncthreads();
+    const int w = threadIdx.x & 31;
+    const float4 part = w < team / 32 ? red[w] : make_float4(0.f, 0.f, 0.f, 0.f);
+    mean = team_sum(part.x, 32) * inv_c;
+    const float d = part.y - mean;
+    m2 = team_sum(fmaf(d * d, part.w, part.z), 32);
+  }
+  return make_float2(mean, rsqrtf(m2 * inv_c + eps));
+}
+
+// One row per team, kept in registers: any width, and a vector for every row.
 template <typename T, typename MT, int V, int P, bool kRes>
 __global__ void __launch_bounds__(1024) adaln_forward_kernel(const SprAdaln op, int team) {
   __shared__ float4 red[32];
@@ -254,51 +312,10 @@ __global__ void __launch_bounds__(1024) adaln_forward_kernel(const SprAdaln op, 
       }
     }
   }
-  // Mean and centred squares of the warp's (or the smaller team's) elements.
-  const int first = lane & ~31;  // the warp's first vector in its team
-  uint64_t acc = 0;
-  int n = 0;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    n += min(max(nvec - first - p * team, 0), min(team, 32)) * V;
-#pragma unroll
-    for (int i = 0; i < Vals<V>::kPairs; ++i) acc = add2(acc, z[p].q[i]);
-  }
-  float2 h = halves(acc);
-  const float sum = team_sum(h.x + h.y, team);
-  float mean = sum * __frcp_rn((float)n);
-  uint64_t minus = both<V>(-mean);
-  acc = 0;
-#pragma unroll
-  for (int p = 0; p < P; ++p)
-    if (lane + p * team < nvec)
-#pragma unroll
-      for (int i = 0; i < Vals<V>::kPairs; ++i) {
-        const uint64_t d = add2(z[p].q[i], minus);
-        acc = fma2(d, d, acc);
-      }
-  h = halves(acc);
-  float m2 = team_sum(h.x + h.y, team);
-  const float inv_c = __frcp_rn((float)c);
-  if (team > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float4(sum, mean, m2, (float)n);
-    __syncthreads();
-    const int warps = team / 32;
-    float total = 0.f;
-    m2 = 0.f;
-#pragma unroll 4
-    for (int w = 0; w < warps; ++w) total += red[w].x;
-    mean = total * inv_c;
-#pragma unroll 4
-    for (int w = 0; w < warps; ++w) {
-      const float4 e = red[w];
-      const float d = e.y - mean;
-      m2 += fmaf(d * d, e.w, e.z);
-    }
-  }
-  const float rstd = rsqrtf(m2 * inv_c + op.eps);
+  const float2 ms = row_stats<V, P>(z, lane, team, nvec, __frcp_rn((float)c), op.eps, red);
+  const float mean = ms.x, rstd = ms.y;
   if (!valid) return;
-  minus = both<V>(-mean);
+  const uint64_t minus = both<V>(-mean);
   const uint64_t r2 = both<V>(rstd);
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -318,20 +335,162 @@ __global__ void __launch_bounds__(1024) adaln_forward_kernel(const SprAdaln op, 
   }
 }
 
-// The rows that share one vector: row r of group g is g*group_step + r*row_step.
-// A group's rows are cut into `chunks` runs; run s of group g writes its column
-// sums to partial[g][s] (or, with one run, the gradients themselves).
-struct Groups {
-  int64_t count, rows, group_step, row_step;
-  int chunks;
-  int64_t chunk_rows;
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The sum over lanes 0..15 (a CTA's warps, one a lane) in all of them.
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, 16);
+  return v;
+}
+
+// Where a run's rows lie: the first row and the step to the next, for rows that are
+// equally spaced in every operand.
+struct Run {
+  int64_t row0, step;
+  int rows;
+  RowId first, group;
+  __device__ __forceinline__ Run(const SprAdaln& op, const Groups& gp, int64_t unit) {
+    const int64_t g = unit / gp.chunks, r0 = unit % gp.chunks * gp.chunk_rows;
+    row0 = g * gp.group_step + r0 * gp.row_step;
+    step = gp.row_step;
+    rows = (int)(min(gp.rows, r0 + gp.chunk_rows) - r0);
+    first = row_id(op, row0);
+    group = row_id(op, g * gp.group_step);
+  }
+  __device__ __forceinline__ const char* at(const void* base, int64_t sb, int64_t st, int e) const {
+    return (const char*)base + (first.b * sb + first.t * st) * e + threadIdx.x * 16;
+  }
 };
 
-// The row arithmetic that both backward kernels share: n, u and the sums before
-// the reduction, the gradients after it.
+// Long groups of wide rows that share their vectors: CTAs that stay on their SM walk
+// runs of rows with the vectors in registers, P 16-byte vectors a thread.  Each
+// thread copies its own vectors of the next kStages - 1 rows into shared memory:
+// the copies need no barrier and stay in flight across the one that joins a row's
+// statistics.  kFull: every thread has all of its P vectors.
+template <typename T, typename MT, int P, bool kRes, bool kFull, int kThreads, int kMin, int kStages>
+__global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(const SprAdaln op, const Groups gp) {
+  constexpr int V = kVec<T>, kIn = kRes ? 2 : 1, e = sizeof(T);
+  __shared__ float2 red[2][16];
+  extern __shared__ uint4 ring[];  // [stage][operand][P][thread]
+  const int c = op.channels, nvec = c / V, team = blockDim.x, lane = threadIdx.x, warps = team / 32;
+  const Run run(op, gp, blockIdx.x);
+  auto mine = [&](int p) { return kFull || lane + p * team < nvec; };
+  // This warp's elements, and those of warp `lane` for the join.
+  auto elements = [&](int w) {
+    int n = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) n += min(max(nvec - 32 * w - p * team, 0), 32) * V;
+    return (float)n;
+  };
+  const int who = lane & 15;
+  const float n_who = who < warps ? elements(who) : 0.f;
+  const float inv_who = n_who > 0.f ? __frcp_rn(n_who) : 0.f;
+  const float inv_n = __frcp_rn(elements(lane >> 5)), inv_c = __frcp_rn((float)c);
+  if (lane < 32) red[lane >> 4][lane & 15] = make_float2(0.f, 0.f);
+  __syncthreads();
+  const char* x = run.at(op.x, op.x_sb, op.x_st, e);
+  const char* y = kRes ? run.at(op.y, op.y_sb, op.y_st, e) : nullptr;
+  const int64_t x_step = (run.step == 1 ? op.x_st : op.x_sb) * e, y_step = (run.step == 1 ? op.y_st : op.y_sb) * e;
+  int fetched = 0;
+  auto fetch = [&](int stage) {
+    if (fetched++ < run.rows) {
+      uint4* to = ring + stage * (kIn * P) * team + lane;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (mine(p)) {
+          copy16_async(to + p * team, x + p * team * 16);
+          if constexpr (kRes) copy16_async(to + (P + p) * team, y + p * team * 16);
+        }
+      x += x_step;
+      if constexpr (kRes) y += y_step;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  Vals<V> w[P], b[P], gate[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int v = lane + p * team;
+    if (!mine(p)) continue;
+    load_factor<MT, V>(op, run.group, v, w[p]);
+    if (op.shift)
+      load_vector<MT, V>((const MT*)op.shift + run.group.b * op.shift_sb + run.group.t * op.shift_st + v * V, b[p]);
+    else b[p].fill(0.f);
+    if constexpr (kRes) load_gate<MT, V>(op, run.group, v, gate[p]);
+  }
+  int stage = 0;
+  char* z_out = (char*)op.z + (run.row0 * c * e + lane * 16);
+  char* h_out = (char*)op.h + (run.row0 * c * e + lane * 16);
+  const int64_t out_step = run.step * c * e;
+  for (int r = 0; r < run.rows; ++r) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    const uint4* slot = ring + stage * (kIn * P) * team + lane;
+    Vals<V> z[P];
+    uint64_t acc[2] = {0, 0};
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (!mine(p)) continue;
+      unpack16<T>(slot[p * team], z[p].q);
+      if constexpr (kRes) {
+        Vals<V> yv;
+        unpack16<T>(slot[(P + p) * team], yv.q);
+        residual<T, V>(z[p], yv, gate[p]);
+        *reinterpret_cast<uint4*>(z_out + p * team * 16) = pack16<T>(z[p].q);
+      }
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) acc[i & 1] = add2(acc[i & 1], z[p].q[i]);
+    }
+    // The slot that this fetch fills was read in the round before.
+    fetch(stage == 0 ? kStages - 1 : stage - 1);
+    float2 h = halves(add2(acc[0], acc[1]));
+    const float sum = warp_sum(h.x + h.y);
+    const float near = -sum * inv_n;
+    acc[0] = acc[1] = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (mine(p))
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          const uint64_t d = add2(z[p].q[i], pair(near, near));
+          acc[i & 1] = fma2(d, d, acc[i & 1]);
+        }
+    h = halves(add2(acc[0], acc[1]));
+    float m2 = warp_sum(h.x + h.y);
+    if ((lane & 31) == 0) red[r & 1][lane >> 5] = make_float2(sum, m2);
+    __syncthreads();
+    // M2 = sum_w M2_w + n_w (mean_w - mean)^2, a warp's values in each of 16 lanes.
+    const float2 part = red[r & 1][who];
+    const float mean = sum16(part.x) * inv_c;
+    const float off = fmaf(part.x, inv_who, -mean);
+    const float rstd = rsqrtf(sum16(fmaf(off * off, n_who, part.y)) * inv_c + op.eps);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (!mine(p)) continue;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+        z[p].q[i] = fma2(mul2(add2(z[p].q[i], pair(-mean, -mean)), pair(rstd, rstd)), w[p].q[i], b[p].q[i]);
+      *reinterpret_cast<uint4*>(h_out + p * team * 16) = pack16<T>(z[p].q);
+    }
+    if (lane == 0 && op.mean) {
+      op.mean[run.row0 + r * run.step] = mean;
+      op.rstd[run.row0 + r * run.step] = rstd;
+    }
+    if constexpr (kRes) z_out += out_step;
+    h_out += out_step;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// The row arithmetic that both backward kernels share: n = (z - mean)*rstd, u = dh*w
+// and a lane's sums before the reduction, the gradients after it.
 template <int V, int P>
-struct Backward {
-  Vals<V> n[P], u[P];
+struct Sums {
   Vals<V> shift[P], scale[P], gate[P];  // column sums
 
   __device__ __forceinline__ void clear() {
@@ -340,28 +499,19 @@ struct Backward {
       shift[p].fill(0.f);
       scale[p].fill(0.f);
       gate[p].fill(0.f);
-      n[p].fill(0.f);
-      u[p].fill(0.f);
     }
   }
   __device__ __forceinline__ void first(int p, const Vals<V>& z, const Vals<V>& dh, const Vals<V>& w, uint64_t minus,
-                                        uint64_t rstd, uint64_t& s0, uint64_t& s1) {
+                                        uint64_t rstd, Vals<V>& n, Vals<V>& u, uint64_t& s0, uint64_t& s1) {
 #pragma unroll
     for (int i = 0; i < Vals<V>::kPairs; ++i) {
-      n[p].q[i] = mul2(add2(z.q[i], minus), rstd);
-      u[p].q[i] = mul2(dh.q[i], w.q[i]);
-      s0 = add2(s0, u[p].q[i]);
-      s1 = fma2(u[p].q[i], n[p].q[i], s1);
+      n.q[i] = mul2(add2(z.q[i], minus), rstd);
+      u.q[i] = mul2(dh.q[i], w.q[i]);
+      s0 = add2(s0, u.q[i]);
+      s1 = fma2(u.q[i], n.q[i], s1);
       shift[p].q[i] = add2(shift[p].q[i], dh.q[i]);
-      scale[p].q[i] = fma2(dh.q[i], n[p].q[i], scale[p].q[i]);
+      scale[p].q[i] = fma2(dh.q[i], n.q[i], scale[p].q[i]);
     }
-  }
-  // rstd*(u - m0 - n*m1) + dz
-  __device__ __forceinline__ void second(int p, uint64_t minus_m0, uint64_t minus_m1, uint64_t rstd, const Vals<V>& dz,
-                                         Vals<V>& g) const {
-#pragma unroll
-    for (int i = 0; i < Vals<V>::kPairs; ++i)
-      g.q[i] = fma2(fma2(n[p].q[i], minus_m1, add2(u[p].q[i], minus_m0)), rstd, dz.q[i]);
   }
   // dgate += g*y, dy = g*gate
   __device__ __forceinline__ void branch(int p, const Vals<V>& g, const Vals<V>& y, Vals<V>& dy) {
@@ -372,6 +522,14 @@ struct Backward {
     }
   }
 };
+// rstd*(u - m0 - n*m1) + dz
+template <int V>
+__device__ __forceinline__ void second(const Vals<V>& n, const Vals<V>& u, uint64_t minus_m0, uint64_t minus_m1,
+                                       uint64_t rstd, const Vals<V>& dz, Vals<V>& g) {
+#pragma unroll
+  for (int i = 0; i < Vals<V>::kPairs; ++i)
+    g.q[i] = fma2(fma2(n.q[i], minus_m1, add2(u.q[i], minus_m0)), rstd, dz.q[i]);
+}
 
 template <typename MT, int V>
 __device__ __forceinline__ void store_sums(const SprAdalnGrad& gr, const Groups& gp, int64_t unit, int c, int v,
@@ -412,7 +570,8 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
   const RowId gid = row_id(op, g * gp.group_step);
   if (threadIdx.x < 64) (&red[0][0].x)[threadIdx.x] = 0;
   if (team > 32) __syncthreads();
-  Backward<V, P> st;
+  Vals<V> n[P], u[P];
+  Sums<V, P> st;
   st.clear();
   for (int64_t i = 0; i < rounds; ++i) {
     const int64_t r = base + i * step;
@@ -430,7 +589,7 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
         load_row<T, V>((const T*)op.x + id.b * op.x_sb + id.t * op.x_st + v * V, z);
         load_row<T, V>((const T*)gr.dh + id.b * gr.dh_sb + id.t * gr.dh_st + v * V, dh);
         load_factor<MT, V>(op, gid, v, w);
-        st.first(p, z, dh, w, minus, rstd, s0, s1);
+        st.first(p, z, dh, w, minus, rstd, n[p], u[p], s0, s1);
       }
     const float2 a = halves(s0), b = halves(s1);
     uint64_t sums = team_sum2(pair(a.x + a.y, b.x + b.y), team);
@@ -445,7 +604,7 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
         Vals<V> dz, gx;
         if (kRes && gr.dz) load_row<T, V>((const T*)gr.dz + id.b * gr.dz_sb + id.t * gr.dz_st + v * V, dz);
         else dz.fill(0.f);
-        st.second(p, m0, m1, rstd, dz, gx);
+        second<V>(n[p], u[p], m0, m1, rstd, dz, gx);
         if constexpr (kRes) {
           Vals<V> y, dy;
           load_row<T, V>((const T*)op.y + id.b * op.y_sb + id.t * op.y_st + v * V, y);
@@ -492,142 +651,153 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
     }
 }
 
-__device__ __forceinline__ void copy16_async(uint4* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-
-// A thread's place in one operand, moved row by row along a group.
-struct Cursor {
-  const char* p;
-  int64_t step, wrap;  // bytes to the group's next row, and further where the batch ends
-  __device__ __forceinline__ Cursor(const void* base, int64_t sb, int64_t st, int e, const RowId& id, int64_t tokens,
-                                    bool along_tokens, int first)
-      : p((const char*)base + (id.b * sb + id.t * st) * e + first * 16),
-        step((along_tokens ? st : sb) * e),
-        wrap((sb - tokens * st) * e) {}
-  __device__ __forceinline__ void next(bool ends) { p += ends ? step + wrap : step; }
-};
-
-// Long groups of wide rows: a few CTAs per SM walk runs of rows with their column
-// sums in registers.  Each thread copies its own 16-byte vectors of the next
-// kStages - 1 rows into shared memory, so the copies need no barrier and stay in
-// flight across the one that joins a row's two sums.
-template <typename T, typename MT, int P, bool kRes, int kThreads, int kStages>
+// Long groups of wide rows: CTAs that stay on their SM walk runs of rows with the
+// vectors and their column sums in registers, P 16-byte vectors a thread.  Each
+// thread copies its own vectors of the next kStages - 1 rounds into shared memory,
+// so the copies need no barrier and stay in flight across the one that joins a
+// round's sums.  A round is R rows, which share the latency of shuffles and barrier.
+// kAgain: n and u are formed again after the barrier instead of held across it
+// (512 threads have 128 registers each; held, they spill).
+constexpr int kStatRows = 256;  // rows whose statistics are in shared memory at a time
+template <typename T, typename MT, int P, bool kRes, bool kFull, bool kAgain, int R, int kThreads, int kStages>
 __global__ void __launch_bounds__(kThreads)
 adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups gp, float* partial) {
   constexpr int V = kVec<T>, kIn = kRes ? 4 : 2, e = sizeof(T);
-  __shared__ ulonglong2 red[2][16];
-  extern __shared__ uint4 ring[];  // [stage][operand][P][thread]
+  __shared__ uint64_t red[2][R][16];
+  __shared__ float stats[2][kStatRows];
+  extern __shared__ uint4 ring[];  // [stage][row][operand][P][thread]
   const int c = op.channels, nvec = c / V, team = blockDim.x, lane = threadIdx.x;
-  const int64_t g = blockIdx.x / gp.chunks, s = blockIdx.x % gp.chunks;
-  const int64_t r0 = s * gp.chunk_rows;
-  const int rows = (int)(min(gp.rows, r0 + gp.chunk_rows) - r0);
+  const Run run(op, gp, blockIdx.x);
+  auto mine = [&](int p) { return kFull || lane + p * team < nvec; };
   const float inv_c = 1.f / c;
-  const int64_t row0 = g * gp.group_step + r0 * gp.row_step;
-  const RowId gid = row_id(op, g * gp.group_step), id0 = row_id(op, row0);
-  const bool along = gp.row_step == 1;
-  if (lane < 64) (&red[0][0].x)[lane] = 0;
-  __syncthreads();
-  Backward<V, P> st;
+  for (int i = lane; i < 32 * R; i += team) (&red[0][0][0])[i] = 0;
+  Sums<V, P> st;
   st.clear();
-  Vals<V> w[P], gate[P];
+  constexpr int kHeld = kAgain ? 1 : P;
+  Vals<V> n[R][kHeld], u[R][kHeld], w[P], gate[P];
 #pragma unroll
   for (int p = 0; p < P; ++p)
-    if (lane + p * team < nvec) {
-      load_factor<MT, V>(op, gid, lane + p * team, w[p]);
-      if constexpr (kRes) load_gate<MT, V>(op, gid, lane + p * team, gate[p]);
+    if (mine(p)) {
+      load_factor<MT, V>(op, run.group, lane + p * team, w[p]);
+      if constexpr (kRes) load_gate<MT, V>(op, run.group, lane + p * team, gate[p]);
     }
-  Cursor cx(op.x, op.x_sb, op.x_st, e, id0, op.tokens, along, lane);
-  Cursor cd(gr.dh, gr.dh_sb, gr.dh_st, e, id0, op.tokens, along, lane);
-  Cursor cy(kRes ? op.y : op.x, op.y_sb, op.y_st, e, id0, op.tokens, along, lane);
-  Cursor cz(kRes && gr.dz ? gr.dz : op.x, gr.dz_sb, gr.dz_st, e, id0, op.tokens, along, lane);
-  int left = along ? (int)(op.tokens - id0.t) : 0x7fffffff;  // rows before the batch ends
+  const bool has_dz = kRes && gr.dz != nullptr;
+  const char* in[4] = {run.at(op.x, op.x_sb, op.x_st, e), run.at(gr.dh, gr.dh_sb, gr.dh_st, e),
+                       kRes ? run.at(op.y, op.y_sb, op.y_st, e) : nullptr,
+                       has_dz ? run.at(gr.dz, gr.dz_sb, gr.dz_st, e) : nullptr};
+  const bool along = run.step == 1;
+  const int64_t step[4] = {(along ? op.x_st : op.x_sb) * e, (along ? gr.dh_st : gr.dh_sb) * e,
+                           (along ? op.y_st : op.y_sb) * e, (along ? gr.dz_st : gr.dz_sb) * e};
   int fetched = 0;
   auto fetch = [&](int stage) {
-    if (fetched < rows) {
-      uint4* to = ring + stage * (kIn * P) * team + lane;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-        if (lane + p * team < nvec) {
-          copy16_async(to + (0 * P + p) * team, cx.p + p * team * 16);
-          copy16_async(to + (1 * P + p) * team, cd.p + p * team * 16);
-          if constexpr (kRes) {
-            copy16_async(to + (2 * P + p) * team, cy.p + p * team * 16);
-            if (gr.dz) copy16_async(to + (3 * P + p) * team, cz.p + p * team * 16);
-          }
+    for (int q = 0; q < R; ++q)
+      if (fetched++ < run.rows) {
+        uint4* to = ring + (stage * R + q) * (kIn * P) * team + lane;
+#pragma unroll
+        for (int k = 0; k < kIn; ++k) {
+          if (k == 3 && !has_dz) continue;
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+            if (mine(p)) copy16_async(to + (k * P + p) * team, in[k] + p * team * 16);
+          in[k] += step[k];
         }
-      const bool ends = --left == 0;
-      if (ends) left = (int)op.tokens;
-      cx.next(ends);
-      cd.next(ends);
-      if constexpr (kRes) {
-        cy.next(ends);
-        cz.next(ends);
       }
-      ++fetched;
-    }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
   int stage = 0;
-  const float *mean_at = op.mean + row0, *rstd_at = op.rstd + row0;
-  float mean = *mean_at, rstd = *rstd_at;
-  char* dx = (char*)gr.dx + ((row0 * c) * e + lane * 16);
-  char* dy = (char*)gr.dy + ((row0 * c) * e + lane * 16);
-  const int64_t out_step = gp.row_step * c * e;
-  for (int r = 0; r < rows; ++r) {
-    if (r + 1 < rows) {
-      mean_at += gp.row_step;
-      rstd_at += gp.row_step;
-    }
-    const float next_mean = *mean_at, next_rstd = *rstd_at;
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    const uint4* slot = ring + stage * (kIn * P) * team + lane;
-    uint64_t s0 = 0, s1 = 0;
-    const uint64_t rs = pair(rstd, rstd);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      if (lane + p * team >= nvec) continue;
-      Vals<V> z, dh;
-      unpack16<T>(slot[(0 * P + p) * team], z.q);
-      unpack16<T>(slot[(1 * P + p) * team], dh.q);
-      st.first(p, z, dh, w[p], pair(-mean, -mean), rs, s0, s1);
-    }
-    const float2 a = halves(s0), b = halves(s1);
-    uint64_t sums = warp_sum2(pair(a.x + a.y, b.x + b.y));
-    // The slot that this fetch fills was read in the round before.
-    fetch(stage == 0 ? kStages - 1 : stage - 1);
-    sums = warps_sum2(sums, red[r & 1], team / 32);
-    const float2 m = halves(sums);
-    const uint64_t m0 = both<V>(-m.x * inv_c), m1 = both<V>(-m.y * inv_c);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      if (lane + p * team >= nvec) continue;
-      Vals<V> gx, dz;
-      if (kRes && gr.dz) unpack16<T>(slot[(3 * P + p) * team], dz.q);
-      else dz.fill(0.f);
-      st.second(p, m0, m1, rs, dz, gx);
-      if constexpr (kRes) {
-        Vals<V> y, gy = gate[p];
-        unpack16<T>(slot[(2 * P + p) * team], y.q);
-        st.branch(p, gx, y, gy);
-        *reinterpret_cast<uint4*>(dy + p * team * 16) = pack16<T>(gy.q);
+  char* dx = (char*)gr.dx + (run.row0 * c * e + lane * 16);
+  char* dy = (char*)gr.dy + (run.row0 * c * e + lane * 16);
+  const int64_t out_step = run.step * c * e;
+  for (int r = 0, odd = 0; r < run.rows; r += R, odd ^= 1) {
+    const int at = r % kStatRows;
+    if (at == 0) {
+      __syncthreads();  // the last readers of the statistics are done
+      for (int i = lane; i < min(kStatRows, run.rows - r); i += team) {
+        stats[0][i] = -op.mean[run.row0 + (r + i) * run.step];
+        stats[1][i] = op.rstd[run.row0 + (r + i) * run.step];
       }
-      *reinterpret_cast<uint4*>(dx + p * team * 16) = pack16<T>(gx.q);
+      __syncthreads();
     }
-    dx += out_step;
-    if constexpr (kRes) dy += out_step;
-    mean = next_mean;
-    rstd = next_rstd;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    const uint4* slot = ring + stage * R * (kIn * P) * team + lane;
+    uint64_t sums[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      uint64_t s0 = 0, s1 = 0;
+      if (R == 1 || r + q < run.rows) {
+        const uint64_t minus = both<V>(stats[0][at + q]), rs = both<V>(stats[1][at + q]);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          if (!mine(p)) continue;
+          Vals<V> z, dh;
+          unpack16<T>(slot[((q * kIn + 0) * P + p) * team], z.q);
+          unpack16<T>(slot[((q * kIn + 1) * P + p) * team], dh.q);
+          st.first(p, z, dh, w[p], minus, rs, n[q][kAgain ? 0 : p], u[q][kAgain ? 0 : p], s0, s1);
+        }
+      }
+      const float2 a = halves(s0), b = halves(s1);
+      sums[q] = pair(a.x + a.y, b.x + b.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int q = 0; q < R; ++q) sums[q] = add2(sums[q], __shfl_xor_sync(0xffffffffu, sums[q], o));
+    // The slots that this fetch fills were read in the round before.
+    fetch(stage == 0 ? kStages - 1 : stage - 1);
+    if ((lane & 31) == 0)
+#pragma unroll
+      for (int q = 0; q < R; ++q) red[odd][q][lane >> 5] = sums[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < R; ++q) sums[q] = red[odd][q][lane & 15];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+      for (int q = 0; q < R; ++q) sums[q] = add2(sums[q], __shfl_xor_sync(0xffffffffu, sums[q], o, 16));
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (R > 1 && r + q >= run.rows) continue;
+      const float2 m = halves(sums[q]);
+      const uint64_t m0 = both<V>(-m.x * inv_c), m1 = both<V>(-m.y * inv_c), rs = both<V>(stats[1][at + q]);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        if (!mine(p)) continue;
+        Vals<V> gx, dz;
+        if (has_dz) unpack16<T>(slot[((q * kIn + 3) * P + p) * team], dz.q);
+        else dz.fill(0.f);
+        if constexpr (kAgain) {
+          Vals<V> z, dh;
+          unpack16<T>(slot[((q * kIn + 0) * P + p) * team], z.q);
+          unpack16<T>(slot[((q * kIn + 1) * P + p) * team], dh.q);
+          const uint64_t minus = both<V>(stats[0][at + q]);
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            n[q][0].q[i] = mul2(add2(z.q[i], minus), rs);
+            u[q][0].q[i] = mul2(dh.q[i], w[p].q[i]);
+          }
+        }
+        second<V>(n[q][kAgain ? 0 : p], u[q][kAgain ? 0 : p], m0, m1, rs, dz, gx);
+        if constexpr (kRes) {
+          Vals<V> y, gy = gate[p];
+          unpack16<T>(slot[((q * kIn + 2) * P + p) * team], y.q);
+          st.branch(p, gx, y, gy);
+          *reinterpret_cast<uint4*>(dy + p * team * 16) = pack16<T>(gy.q);
+        }
+        *reinterpret_cast<uint4*>(dx + p * team * 16) = pack16<T>(gx.q);
+      }
+      dx += out_step;
+      if constexpr (kRes) dy += out_step;
+    }
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int v = lane + p * team;
-    if (v < nvec) store_sums<MT, V>(gr, gp, blockIdx.x, c, v, partial, st.shift[p], st.scale[p], st.gate[p]);
+    if (mine(p)) store_sums<MT, V>(gr, gp, blockIdx.x, c, v, partial, st.shift[p], st.scale[p], st.gate[p]);
   }
 }
 
@@ -713,6 +883,18 @@ int by_type(const SprAdaln* op, F f) {
   return op->mod_dtype == SPR_F32 ? f(__half{}, float{}) : f(__half{}, __half{});
 }
 
+// Rows without gaps between the samples are one sample of batch*tokens rows.
+bool dense_batch(int64_t sb, int64_t st, int64_t tokens) { return sb == tokens * st; }
+void merge_batch(SprAdaln& op, SprAdalnGrad* g) {
+  if (op.batch == 1 || op.shift_sb || op.scale_sb || op.gate_sb || op.shift_st || op.scale_st || op.gate_st) return;
+  if (!dense_batch(op.x_sb, op.x_st, op.tokens) || (op.y && !dense_batch(op.y_sb, op.y_st, op.tokens))) return;
+  if (g && (g->mod_batch || g->mod_tokens || !dense_batch(g->dh_sb, g->dh_st, op.tokens) ||
+            (g->dz && !dense_batch(g->dz_sb, g->dz_st, op.tokens))))
+    return;
+  op.tokens *= op.batch;
+  op.batch = 1;
+}
+
 template <int N>
 struct Int {
   static constexpr int value = N;
@@ -733,26 +915,9 @@ int by_shape(bool vec, int per, F f) {
 
 constexpr int kCtaThreads = 256;  // of a CTA whose teams are at most a warp
 
-template <typename T>
-int forward_per_thread(bool vec, int nvec) {
-  if (nvec <= 32) return 1;
-  if (vec) return nvec <= 64 ? 1 : nvec <= 128 ? 2 : 4;
-  return nvec <= 4096 ? 4 : 16;
-}
-
-template <typename T, typename MT, bool kRes>
-int launch_forward(const SprAdaln* op, cudaStream_t st) {
-  const bool vec = vectors_fit(op);
-  const int nvec = op->channels / (vec ? kVec<T> : 1);
-  return by_shape<T>(vec, forward_per_thread<T>(vec, nvec), [&](auto v, auto p) {
-    constexpr int V = decltype(v)::value, P = decltype(p)::value;
-    const int team = team_for((nvec + P - 1) / P);
-    const int threads = team > 32 ? team : kCtaThreads;
-    const int64_t rows = op->batch * op->tokens, teams = threads / team;
-    adaln_forward_kernel<T, MT, V, P, kRes><<<(unsigned)((rows + teams - 1) / teams), threads, 0, st>>>(*op, team);
-    return check_launch("adaln forward");
-  });
-}
+// Whether a run's rows are equally spaced in every operand: within one sample, or
+// the same token of every sample, or all rows of operands without gaps.
+bool even_rows(const Groups& g, int64_t batch) { return batch == 1 || g.row_step != 1 || g.count % batch == 0; }
 
 Groups make_groups(int64_t batch, int64_t tokens, int mod_batch, int mod_tokens) {
   Groups g{};
@@ -770,7 +935,94 @@ void cut_groups(Groups& g, int64_t ctas, int64_t least) {
   g.chunks = (int)((g.rows + g.chunk_rows - 1) / g.chunk_rows);
 }
 
-constexpr int kMaxCtasPerSm = 4;
+template <typename T>
+int forward_per_thread(bool vec, int nvec) {
+  if (nvec <= 32) return 1;
+  if (vec) return nvec <= 64 ? 1 : nvec <= 128 ? 2 : 4;
+  return nvec <= 4096 ? 4 : 16;
+}
+
+// CTAs of a kernel that an SM holds, asked once for each number of warps.
+template <typename K>
+int resident(K kern, int threads, int smem) {
+  static std::atomic<int> known[33] = {};
+  std::atomic<int>& n = known[threads / 32];
+  if (n.load(std::memory_order_relaxed) == 0) {
+    int got = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kern, threads, smem) != cudaSuccess) got = 1;
+    n.store(std::max(1, got), std::memory_order_relaxed);
+  }
+  return n.load(std::memory_order_relaxed);
+}
+
+// How a streaming launch cuts its groups: as many runs as fit on the GPU at once, and
+// up to `most_waves` times that while a run still reads `least` bytes.  More waves
+// leave uneven SMs less to wait for at the end, each run costs its start (and in
+// the backward pass a set of column sums).  Of measured bandwidth, 1 / 6 waves:
+// 75,600 x 5120 bf16 forward 92% / 98%, 60,000 x 1024 fp16 forward 86% / 80%,
+// 75,600 x 5120 bf16 gated backward 89% / 98%, ungated 101% / 88%.
+void cut_stream(Groups& g, int64_t at_once, int64_t row_bytes, int64_t most_waves, int64_t least, int64_t most) {
+  const int64_t waves = g.count * g.rows * row_bytes / (at_once * least);
+  cut_groups(g, std::min(most, at_once * std::max<int64_t>(1, std::min(most_waves, waves))), 4);
+}
+
+// Stages of a ring whose stage takes `bytes` at the kernel's most threads; 0: none fits.
+constexpr int ring_stages(int bytes) {
+  return 4 * bytes <= 200 * 1024 ? 4 : 3 * bytes <= 200 * 1024 ? 3 : 2 * bytes <= 200 * 1024 ? 2 : 0;
+}
+
+template <typename T, typename MT, bool kRes, int P, bool kFull, int kThreads, int kMin>
+int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
+  constexpr int kIn = kRes ? 2 : 1, kStages = ring_stages(kIn * P * kThreads * 16);
+  auto kern = adaln_forward_stream_kernel<T, MT, P, kRes, kFull, kThreads, kMin, kStages>;
+  const int team = team_for((op->channels / kVec<T> + P - 1) / P);
+  const int smem = kStages * kIn * P * team * 16;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * kIn * P * kThreads * 16) !=
+      cudaSuccess)
+    return check_launch("adaln forward");
+  cut_stream(g, (int64_t)sm_count() * resident(kern, team, smem), (int64_t)kIn * op->channels * sizeof(T), 6, 65536,
+             INT64_MAX);
+  kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, g);
+  return check_launch("adaln forward");
+}
+
+// Whether P/2 vectors a thread leave fewer idle places in a CTA of at most 512.
+bool half_fits_better(int nvec, int P) {
+  const int half = team_for((nvec + P / 2 - 1) / (P / 2));
+  return half <= 512 && half * (P / 2) < team_for((nvec + P - 1) / P) * P;
+}
+
+template <typename T, typename MT, bool kRes>
+int launch_forward(const SprAdaln* op, cudaStream_t st) {
+  const bool vec = vectors_fit(op);
+  const int nvec = op->channels / (vec ? kVec<T> : 1);
+  auto kept = [&](int64_t scale, int64_t shift, int64_t gate) { return scale || shift || gate; };
+  const Groups g = make_groups(op->batch, op->tokens, kept(op->scale_sb, op->shift_sb, op->gate_sb),
+                               kept(op->scale_st, op->shift_st, op->gate_st));
+  constexpr int P = 16 / kVec<T>;  // 16 values a thread, or 8 where that leaves fewer threads idle
+  if (vec && nvec > 32 && nvec <= 512 * P && g.rows >= 8 && even_rows(g, op->batch)) {
+    if (nvec % (32 * P) == 0)
+      return nvec <= 320 * P ? launch_forward_stream<T, MT, kRes, P, true, 320, 2>(op, g, st)
+                             : launch_forward_stream<T, MT, kRes, P, true, 512, 1>(op, g, st);
+    if (half_fits_better(nvec, P)) return launch_forward_stream<T, MT, kRes, P / 2, false, 512, 1>(op, g, st);
+    return launch_forward_stream<T, MT, kRes, P, false, 512, 1>(op, g, st);
+  }
+  return by_shape<T>(vec, forward_per_thread<T>(vec, nvec), [&](auto v, auto p) {
+    constexpr int V = decltype(v)::value, P = decltype(p)::value;
+    const int team = team_for((nvec + P - 1) / P);
+    const int threads = team > 32 ? team : kCtaThreads;
+    const int64_t rows = op->batch * op->tokens, teams = threads / team;
+    adaln_forward_kernel<T, MT, V, P, kRes><<<(unsigned)((rows + teams - 1) / teams), threads, 0, st>>>(*op, team);
+    return check_launch("adaln forward");
+  });
+}
+
+// Runs of a backward launch, all groups together: sixteen an SM, and no more than
+// 48 MB of column sums.  The workspace is sized for that many.
+int64_t most_runs(int channels) {
+  const int64_t sms = sm_count();
+  return std::min(16 * sms, std::max(sms, (int64_t)(1 << 22) / channels));
+}
 
 template <typename MT>
 int join(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, const float* partial, cudaStream_t st) {
@@ -780,13 +1032,17 @@ int join(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, const floa
   return check_launch("adaln backward");
 }
 
-template <typename T, typename MT, bool kRes, int P, int kThreads, int kStages>
-int launch_stream(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, int team, float* partial, cudaStream_t st) {
-  auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kThreads, kStages>;
-  const int smem = kStages * (kRes ? 4 : 2) * P * team * 16;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+template <typename T, typename MT, bool kRes, int P, bool kFull, bool kAgain, int R, int kThreads>
+int launch_backward_stream(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, float* partial, cudaStream_t st) {
+  constexpr int kIn = kRes ? 4 : 2, kStages = std::min(kRes ? 4 : 3, ring_stages(R * kIn * P * kThreads * 16));
+  auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kFull, kAgain, R, kThreads, kStages>;
+  const int team = team_for((op->channels / kVec<T> + P - 1) / P);
+  const int smem = kStages * R * kIn * P * team * 16;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * R * kIn * P * kThreads * 16) !=
+      cudaSuccess)
     return check_launch("adaln backward");
-  cut_groups(g, (int64_t)sm_count() * std::min(kMaxCtasPerSm, std::max(1, 320 / team)), 4);
+  cut_stream(g, (int64_t)sm_count() * resident(kern, team, smem), (int64_t)kIn * op->channels * sizeof(T),
+             kRes ? 6 : 1, 3 << 19, most_runs(op->channels));
   kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, *gr, g, partial);
   return join<MT>(op, gr, g, partial, st);
 }
@@ -796,11 +1052,17 @@ int launch_backward(const SprAdaln* op, const SprAdalnGrad* gr, float* partial, 
   const bool vec = vectors_fit(op, gr);
   const int nvec = op->channels / (vec ? kVec<T> : 1);
   Groups g = make_groups(op->batch, op->tokens, gr->mod_batch, gr->mod_tokens);
-  if (vec && nvec > 32 && nvec <= 1024 && g.rows >= 8) {
-    if (nvec <= 128) return launch_stream<T, MT, kRes, 1, 128, 4>(op, gr, g, team_for(nvec), partial, st);
-    const int team = team_for((nvec + 1) / 2);
-    if (team <= 384) return launch_stream<T, MT, kRes, 2, 384, 4>(op, gr, g, team, partial, st);
-    return launch_stream<T, MT, kRes, 2, 512, 3>(op, gr, g, team, partial, st);
+  constexpr int kPer = 16 / kVec<T>;  // 16 values a thread, or 8 where that leaves fewer threads idle
+  constexpr int kWide = kRes && sizeof(T) == 4 ? 320 : 512;  // threads whose ring fits
+  if (vec && nvec > 32 && nvec <= kWide * kPer && g.rows >= 8 && even_rows(g, op->batch)) {
+    if (nvec % (32 * kPer) == 0) {
+      if (nvec <= 320 * kPer)
+        return launch_backward_stream<T, MT, kRes, kPer, true, false, kRes ? 1 : 2, 320>(op, gr, g, partial, st);
+      return launch_backward_stream<T, MT, kRes, kPer, true, kRes, 1, kWide>(op, gr, g, partial, st);
+    }
+    if (half_fits_better(nvec, kPer))
+      return launch_backward_stream<T, MT, kRes, kPer / 2, false, false, 1, 512>(op, gr, g, partial, st);
+    return launch_backward_stream<T, MT, kRes, kPer, false, kRes, 1, kWide>(op, gr, g, partial, st);
   }
   const int per = nvec <= 32 ? 1 : vec ? (nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : 4) : nvec <= 4096 ? 4 : 16;
   return by_shape<T>(vec, per, [&](auto v, auto p) {
@@ -812,7 +1074,7 @@ int launch_backward(const SprAdaln* op, const SprAdalnGrad* gr, float* partial, 
       g.chunks = 1;
       g.chunk_rows = g.rows;
     } else {
-      cut_groups(g, (int64_t)sm_count() * kMaxCtasPerSm, 4 * teams);
+      cut_groups(g, std::min((int64_t)sm_count() * 4, most_runs(op->channels)), 4 * teams);
     }
     const int64_t units = g.count * g.chunks, ctas = own ? (units + teams - 1) / teams : units;
     const size_t smem = !own && teams > 1 ? (size_t)teams * 3 * op->channels * sizeof(float) : 0;
@@ -831,11 +1093,13 @@ extern "C" int spr_adaln_forward(const SprAdaln* op, void* stream) {
   if (int rc = check_adaln(op)) return rc;
   if (op->batch * op->tokens == 0) return SPR_OK;
   if (!op->x || !op->h || (op->y && !op->z)) return fail(SPR_ERR_ARG, "adaln forward: null operand");
+  SprAdaln o = *op;
+  merge_batch(o, nullptr);
   return by_type(op, [&](auto t, auto m) {
     using T = decltype(t);
     using MT = decltype(m);
-    return op->y ? launch_forward<T, MT, true>(op, (cudaStream_t)stream)
-                 : launch_forward<T, MT, false>(op, (cudaStream_t)stream);
+    return op->y ? launch_forward<T, MT, true>(&o, (cudaStream_t)stream)
+                 : launch_forward<T, MT, false>(&o, (cudaStream_t)stream);
   });
 }
 
@@ -843,7 +1107,7 @@ extern "C" size_t spr_adaln_backward_workspace_bytes(int64_t batch, int64_t toke
                                                      int mod_tokens) {
   if (batch <= 0 || tokens <= 0 || channels <= 0) return 0;
   Groups g = make_groups(batch, tokens, mod_batch, mod_tokens);
-  cut_groups(g, (int64_t)sm_count() * kMaxCtasPerSm, 4);  // as many runs as any launch takes
+  cut_groups(g, most_runs(channels), 4);  // as many runs as any launch takes
   return g.chunks == 1 ? 0 : (size_t)g.count * g.chunks * 3 * channels * sizeof(float);
 }
 
@@ -859,10 +1123,13 @@ extern "C" int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, 
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(SPR_ERR_WORKSPACE, "adaln backward: workspace %zu < %zu bytes or not 16-byte aligned", workspace_bytes,
                 need);
+  SprAdaln o = *op;
+  SprAdalnGrad gr = *grad;
+  merge_batch(o, &gr);
   return by_type(op, [&](auto t, auto m) {
     using T = decltype(t);
     using MT = decltype(m);
-    return op->y ? launch_backward<T, MT, true>(op, grad, (float*)workspace, (cudaStream_t)stream)
-                 : launch_backward<T, MT, false>(op, grad, (float*)workspace, (cudaStream_t)stream);
+    return op->y ? launch_backward<T, MT, true>(&o, &gr, (float*)workspace, (cudaStream_t)stream)
+                 : launch_backward<T, MT, false>(&o, &gr, (float*)workspace, (cudaStream_t)stream);
   });
 }
