@@ -2,15 +2,19 @@
 // with respect to the rows (layout and formula at spr_int4_linear in the header).
 //   y[r][n] = sum_g scale[n][g] * sum_{k in g} x[r][k]*(code[n][k] - zero[n][g]) + bias[n]
 //   dx[r][k] = sum_n (dy[r][n]*scale[n][g]) * (code[n][k] - zero[n][g])
-// What bounds both is the codes' bytes (an SM takes 23 bytes, 46 codes, a cycle from
-// HBM), so the arithmetic on a code has to stay within two or three instructions.
-// Tensor-core products (m16n8k16, bf16 with fp32 sums) take a code as the exact bf16
-// integer code - zero: three instructions make two of them.  The other operand is
-// split into as many bf16 parts as its significand needs (bf16 1, fp16 2, fp32 3, by
-// cutting off, which is exact), each part a row or column of its own in the same
-// product, so that nothing is rounded before the fp32 sums.  With at most 32 rows
-// the 5th-generation tensor instructions would idle on 128-row tiles, and their
-// operands would have to pass through shared memory once more after unpacking.
+// What bounds both is the codes' bytes: HBM gives an SM 23 bytes, 46 codes, a cycle,
+// so a 16 x 32 block of codes has 44 instruction slots of the SM's four schedulers
+// for everything.  Hence tensor-core products whose operand is a few instructions
+// from the packed codes, and no rounding of x:
+// * 16-bit x: integer products (m16n8k32).  The codes are the bytes w & 0x0f0f0f0f and
+//   (w >> 4) & 0x0f0f0f0f; x is a 23-bit integer relative to its row's largest
+//   magnitude, in three signed bytes, each a column of the product.  An inner sum is
+//   an exact integer.
+// * fp32 x, and more rows than the integer columns hold: bf16 products (m16n8k16).  A
+//   code is the exact integer code - zero, and x is cut into as many bf16 parts as
+//   its significand needs (bf16 1, fp16 2, fp32 3; exact), each a column.
+// The 5th-generation tensor instructions work on 128 rows: with so few, they would
+// idle, and their operands would pass through shared memory again once unpacked.
 #include <math.h>
 
 #include "common.cuh"
@@ -19,12 +23,12 @@ namespace spr {
 
 namespace {
 
-constexpr int kWarps = 8;        // of a CTA, at most
-constexpr int kTile = 16;        // weight rows of a product
-constexpr int kChunk = 256;      // codes of a row in one stage of a warp's ring: 128 bytes
-constexpr int kBlocks = kChunk / 32;
+constexpr int kWarps = 8;  // of a CTA, at most
+constexpr int kTile = 16;  // weight rows of a product
+constexpr int kBlocks = 8;  // blocks of 32 codes in one stage of a warp's ring: 128 bytes of a row
 constexpr int kStages = 4;
-constexpr int kStageBytes = kTile * kChunk / 2;
+constexpr int kStageBytes = kTile * kBlocks * 16;
+constexpr int kLimbs = 3;
 
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
   if (dtype == SPR_F32) return __ldg((const float*)p + i);
@@ -63,6 +67,14 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_int(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // Codes i and i + 4 of a word as bf16 integers 128 + code, less `zero` = 128 + zero
 // in both halves: exact.
 template <int I>
@@ -83,46 +95,56 @@ struct Weights {
   int64_t n;
   int k, groups, group_blocks, blocks;  // blocks of 32 codes a row, the unused ones of the last group too
 };
+struct Rows {
+  const void* x;
+  int64_t stride;
+  int dtype, parts, all, pass;  // columns a row, rows, rows a launch's pass takes
+};
 
 // A warp's ring holds the codes of 16 weight rows by 256 columns a stage.  16-byte
-// piece j of row r lies at j ^ (r & 7): what eight lanes groups read at once falls
-// into different banks.
-__device__ __forceinline__ int piece(int row, int j) { return row * 128 + ((j ^ (row & 7)) << 4); }
+// piece j of row r lies at j ^ (r's low bits reversed): lanes that read one, two or
+// four words of neighbouring rows at once meet different banks.
+__device__ __forceinline__ int turn(int row) { return (row & 1) << 2 | (row & 2) | (row >> 2 & 1); }
+__device__ __forceinline__ int piece(int row, int j) { return row * 128 + ((j ^ turn(row)) << 4); }
 
-__device__ __forceinline__ void fetch_codes(const Weights& w, int64_t tile, int chunk, char* stage, int lane) {
-  const int j = lane & 7;
-  if (chunk * kBlocks + j < w.blocks) {
-#pragma unroll
-    for (int i = 0; i < kTile / 4; ++i) {
-      const int row = i * 4 + (lane >> 3);
-      const int64_t n = min(tile * kTile + row, w.n - 1);
-      copy16_async(stage + piece(row, j), w.packed + (n * w.blocks + chunk * kBlocks + j) * 16);
-    }
+template <int U>
+__device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[U]) {
+  if constexpr (U == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (U == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
-// Scale and 128 + zero (bf16, in both halves) of a stage's rows and groups: loaded one
-// stage ahead into registers, then put where the warp's lanes find them.
-template <int kRegs>
+// Scale and zero of a stage's rows and segments (GB blocks, within one group), loaded
+// one stage ahead into registers, then put where the warp's lanes find them.
+template <int GB, bool kInt>
 struct Meta {
+  static constexpr int kRegs = kBlocks / GB * kTile / 32 > 0 ? kBlocks / GB * kTile / 32 : 1;
   float scale[kRegs];
   uint32_t zero[kRegs];
-  __device__ __forceinline__ void load(const Weights& w, int64_t tile, int chunk, int lane, float up) {
-    const int64_t n = min(tile * kTile + (lane & 15), w.n - 1);
-    const int g0 = chunk * kBlocks / w.group_blocks;
+  __device__ __forceinline__ void load(const Weights& w, int64_t row_at, int chunk, int lane, float up) {
+    // row_at: the lane's row's first group.
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) {
-      const int g = min(g0 + 2 * i + (lane >> 4), w.groups - 1);
-      scale[i] = load_as_f32(w.scales, w.scale_dtype, n * w.groups + g) * up;
-      zero[i] = 0x43004300u + 0x00010001u * (w.zeros ? (uint32_t)__ldg(w.zeros + n * w.groups + g) : 8u);
+      int g = chunk * (kBlocks / GB) + 2 * i + (lane >> 4);
+      if (w.group_blocks != GB) g = g * GB / w.group_blocks;
+      g = min(g, w.groups - 1);
+      scale[i] = load_as_f32(w.scales, w.scale_dtype, row_at + g) * up;
+      zero[i] = w.zeros ? (uint32_t)__ldg(w.zeros + row_at + g) : 8u;
     }
   }
   __device__ __forceinline__ void store(float2* meta, int lane) const {
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i) meta[i * 32 + lane] = make_float2(scale[i], __uint_as_float(zero[i]));
+    for (int i = 0; i < kRegs; ++i)
+      meta[i * 32 + lane] =
+          make_float2(scale[i], __uint_as_float(kInt ? zero[i] : 0x43004300u + 0x00010001u * zero[i]));
   }
 };
-constexpr int kMetaRegs(int gb) { return gb == 1 ? 4 : gb == 4 ? 1 : 2; }  // groups a stage touches, in pairs
 
 // Where a launch's warps work: `along` warps of a CTA share a tile, each with every
 // `along`-th chunk of the CTA's slice of the columns; `tiles` such teams to a CTA.
@@ -131,153 +153,280 @@ struct Shape {
   int slice_chunks, slices;
 };
 
-// y for up to NT*8 columns (a row's parts each one): warp products of 16 weight rows
-// by 32 columns of the weight a step, the x parts staged in shared memory in the order
-// in which a word's codes come apart (k, k+4), (k+1, k+5), ...
-template <int NT, int GB>
+// Eight values of x from column k, zeros past the end.
+__device__ __forceinline__ void load_x(const Rows& in, bool wide, int64_t at, int k, int k_end, float (&v)[8]) {
+  if (wide && k + 8 <= k_end) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>((const char*)in.x + at * 2));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t h = (&u.x)[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+      v[e] = in.dtype == SPR_BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k + e < k_end ? load_as_f32(in.x, in.dtype, at + e) : 0.f;
+  }
+}
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// The slice's x in shared memory in the order in which codes come apart.  A unit is
+// U blocks, whose 4*U words go to the four lanes of a weight row U at a time: word j
+// of lane t is word t*U + j of the unit.
+// bf16: [block][column][lane] the pairs (k, k+4), (k+1, k+5), (k+2, k+6), (k+3, k+7)
+// of the lane's word.  Integers: the bytes (k, k+2, k+4, k+6), (k+1, k+3, k+5, k+7).
+template <int U>
+__device__ __forceinline__ int x_place(int b, int word, int cols, int col) {
+  const int at = (b % U) * 4 + word;  // within the unit
+  return ((b / U * U + at % U) * cols + col) * 4 + at / U;
+}
+
+template <int U>
+__device__ __forceinline__ void stage_bf16(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, float down,
+                                           bool wide, uint4* xs) {
+  const int cols = rows * in.parts;
+  for (int i = threadIdx.x; i < nb * rows * 4; i += blockDim.x) {
+    const int word = i & 3, b = (i >> 2) % nb, r = (i >> 2) / nb, k = (b0 + b) * 32 + word * 8;
+    float v[8];
+    load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
+    for (int p = 0; p < in.parts; ++p) {
+      uint32_t h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = bf16_part(v[e] * down, p);
+      xs[x_place<U>(b, word, cols, r * in.parts + p)] =
+          make_uint4(bf16_pair(h[0], h[4]), bf16_pair(h[1], h[5]), bf16_pair(h[2], h[6]), bf16_pair(h[3], h[7]));
+    }
+  }
+}
+
+// Integers round(x * 2^power[r]) below 2^22 in magnitude, as bytes d0 + 256 d1 + 65536 d2;
+// sums[segment's first block][column]: the bytes of a segment added up.  What is not
+// finite counts as 0 and sets bad[r].
+template <int U, int GB>
+__device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, bool wide,
+                                          uint2* xs, int* sums, int sum_cols, uint32_t* largest, int* power, int* bad) {
+  const int cols = rows * kLimbs;
+  if (threadIdx.x < 32) {
+    largest[threadIdx.x] = 0;
+    bad[threadIdx.x] = 0;
+  }
+  for (int i = threadIdx.x; i < nb * sum_cols; i += blockDim.x) sums[i] = 0;
+  __syncthreads();
+  const int words = nb * 4;
+  for (int i = threadIdx.x; i < words * rows; i += blockDim.x) {
+    const int r = i / words, k = b0 * 32 + i % words * 8;
+    float v[8];
+    load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
+    uint32_t m = 0;
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t u = __float_as_uint(v[e]) & 0x7fffffffu;
+      any |= u >= 0x7f800000u;
+      m = max(m, u >= 0x7f800000u ? 0u : u);
+    }
+    if (any) bad[r] = 1;
+    if (m > largest[r]) atomicMax(&largest[r], m);
+  }
+  __syncthreads();
+  if (threadIdx.x < rows) power[threadIdx.x] = 21 - ((int)(largest[threadIdx.x] >> 23) - 127);
+  __syncthreads();
+  for (int i = threadIdx.x; i < words * rows; i += blockDim.x) {
+    const int r = i / words, b = i % words >> 2, word = i & 3, k = (b0 + b) * 32 + word * 8;
+    float v[8];
+    load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
+    uint32_t d[kLimbs][2] = {};
+    int total[kLimbs] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int q = finite(v[e]) ? __float2int_rn(scalbnf(v[e], power[r])) : 0;
+#pragma unroll
+      for (int l = 0; l < kLimbs; ++l) {
+        const int byte = l == kLimbs - 1 ? q : (int)(int8_t)(q & 255);
+        q = (q - byte) >> 8;
+        d[l][e & 1] |= (uint32_t)(byte & 255) << (8 * (e >> 1));
+        total[l] += byte;
+      }
+    }
+#pragma unroll
+    for (int l = 0; l < kLimbs; ++l) {
+      xs[x_place<U>(b, word, cols, r * kLimbs + l)] = make_uint2(d[l][0], d[l][1]);
+      atomicAdd(&sums[b / GB * GB * sum_cols + r * kLimbs + l], total[l]);  // whole numbers: any order
+    }
+  }
+}
+
+// y for up to NT*8 columns (a row's parts or bytes each one): warp products of 16 weight
+// rows by 32 columns of the weight a step.
+template <int NT, int GB, bool kInt>
 __global__ void __launch_bounds__(kWarps * 32, 2)
-int4_linear_kernel(const Weights w, const Shape sh, const void* x, int64_t x_stride, int dtype, int parts, int all_rows,
-                   int pass_rows, float down, float up, const void* bias, void* y, float* partial) {
-  constexpr int kRegs = kMetaRegs(GB);
+int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, float up, const void* bias, void* y,
+                   float* partial) {
+  using M = Meta<GB, kInt>;
+  constexpr int U = GB < 4 ? GB : 4, kMeta = M::kRegs * 32;
   extern __shared__ __align__(128) char smem[];
+  __shared__ uint32_t largest[32];
+  __shared__ int power[32], bad[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = sh.along * sh.tiles;
-  const int row0 = blockIdx.y * pass_rows, rows = min(pass_rows, all_rows - row0), cols = rows * parts;
+  const int row0 = blockIdx.y * in.pass, rows = min(in.pass, in.all - row0), cols = rows * in.parts;
   const int c0 = blockIdx.z * sh.slice_chunks;
   const int c1 = min((w.blocks + kBlocks - 1) / kBlocks, c0 + sh.slice_chunks);
   const int b0 = c0 * kBlocks, nb = min(w.blocks, c1 * kBlocks) - b0;  // the slice's blocks
   char* ring = smem + warp * kStages * kStageBytes;
-  float2* meta = reinterpret_cast<float2*>(smem + warps * kStages * kStageBytes) + warp * 2 * 32 * kRegs;
-  float* red = reinterpret_cast<float*>(smem + warps * (kStages * kStageBytes + 2 * 32 * kRegs * 8));
-  uint4* xs = reinterpret_cast<uint4*>(red + 2 * warps * kTile * NT * 8);  // [block][column][word of the block]
+  float2* meta = reinterpret_cast<float2*>(smem + warps * kStages * kStageBytes) + warp * 2 * kMeta;
+  float* red = reinterpret_cast<float*>(smem + warps * (kStages * kStageBytes + 2 * kMeta * 8));
+  char* xs = reinterpret_cast<char*>(red + 2 * warps * kTile * NT * 8);
+  int* sums = reinterpret_cast<int*>(xs + nb * cols * 32);  // integers only
 
   const int wt = warp / sh.along, wk = warp % sh.along;
-  const int64_t tiles = (w.n + kTile - 1) / kTile, tile_step = (int64_t)gridDim.x * sh.tiles;
+  const int tiles = (int)((w.n + kTile - 1) / kTile), tile_step = gridDim.x * sh.tiles;
+  const int64_t pitch = (int64_t)w.blocks * 16;
   // Three places in the warp's sequence of stages: being copied, its scales being
   // loaded, being computed.
   struct Place {
-    int64_t tile;
-    int chunk;
+    int tile, chunk;
   };
   auto next = [&](Place& p) {
     p.chunk += sh.along;
     if (p.chunk >= c1) {
       p.chunk = c0 + wk;
       p.tile += tile_step;
+      return true;
     }
+    return false;
   };
-  const Place start = {(int64_t)blockIdx.x * sh.tiles + wt, c0 + wk};
+  const Place start = {(int)(blockIdx.x * sh.tiles + wt), c0 + wk};
   Place copy = start, load = start, at = start;
+
+  const uint8_t* from[kTile / 4];  // the lane's 16 bytes in the first chunk of rows lane/8 + 4i
+  auto aim = [&]() {
+#pragma unroll
+    for (int i = 0; i < kTile / 4; ++i)
+      from[i] = w.packed + min((int64_t)copy.tile * kTile + i * 4 + (lane >> 3), w.n - 1) * pitch + (lane & 7) * 16;
+  };
+  uint32_t to[kTile / 4];
+#pragma unroll
+  for (int i = 0; i < kTile / 4; ++i)
+    to[i] = (uint32_t)__cvta_generic_to_shared(ring) + piece(i * 4 + (lane >> 3), lane & 7);
+  aim();
   auto fetch = [&](int stage) {
     if (copy.tile < tiles) {
-      fetch_codes(w, copy.tile, copy.chunk, ring + stage * kStageBytes, lane);
-      next(copy);
+      if (copy.chunk * kBlocks + (lane & 7) < w.blocks)
+#pragma unroll
+        for (int i = 0; i < kTile / 4; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kStageBytes),
+                       "l"(from[i] + copy.chunk * (kBlocks * 16))
+                       : "memory");
+      if (next(copy)) aim();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
-  Meta<kRegs> mt;
-  if (load.tile < tiles) mt.load(w, load.tile, load.chunk, lane, up);
+  M mt;
+  int64_t load_at = min((int64_t)load.tile * kTile + (lane & 15), w.n - 1) * w.groups;
+  if (load.tile < tiles) mt.load(w, load_at, load.chunk, lane, up);
 
-  const int esize = dtype == SPR_F32 ? 4 : 2;
-  const bool wide = esize == 2 && x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  for (int i = threadIdx.x; i < nb * rows * 4; i += blockDim.x) {
-    const int word = i & 3, r = (i >> 2) % rows, b = (i >> 2) / rows;
-    const int k = (b0 + b) * 32 + word * 8;
-    const int64_t at_x = (int64_t)(row0 + r) * x_stride + k;
-    float v[8];
-    if (wide && k + 8 <= w.k) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>((const char*)x + at_x * 2));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t h = (&u.x)[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-        v[e] = dtype == SPR_BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = k + e < w.k ? load_as_f32(x, dtype, at_x + e) : 0.f;
-    }
-    for (int p = 0; p < parts; ++p) {
-      uint32_t h[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = bf16_part(v[e] * down, p);
-      xs[(b * cols + r * parts + p) * 4 + word] =
-          make_uint4(bf16_pair(h[0], h[4]), bf16_pair(h[1], h[5]), bf16_pair(h[2], h[6]), bf16_pair(h[3], h[7]));
-    }
-  }
+  const bool wide = in.dtype != SPR_F32 && in.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in.x) % 16 == 0;
+  if constexpr (kInt)
+    stage_int<U, GB>(w, in, row0, rows, b0, nb, wide, reinterpret_cast<uint2*>(xs), sums, NT * 8, largest, power, bad);
+  else stage_bf16<U>(w, in, row0, rows, b0, nb, down, wide, reinterpret_cast<uint4*>(xs));
   mt.store(meta, lane);
   __syncthreads();
-  next(load);
+  auto advance_load = [&]() {
+    if (next(load)) load_at = min((int64_t)load.tile * kTile + (lane & 15), w.n - 1) * w.groups;
+  };
+  advance_load();
 
   float acc[NT][4] = {};
   int stage = 0, buffer = 0, odd = 0;
   const int t = lane & 3, r8 = lane >> 2;
-  const char* codes_at = ring + r8 * 128 + t * 4;
   while (at.tile < tiles) {
-    if (load.tile < tiles) mt.load(w, load.tile, load.chunk, lane, up);
-    next(load);
+    if (load.tile < tiles) mt.load(w, load_at, load.chunk, lane, up);
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();
     const int first = at.chunk * kBlocks, here = min(kBlocks, w.blocks - first);
-    const char* words = codes_at + stage * kStageBytes;
-    const float2* mp = meta + buffer * 32 * kRegs + r8;
-    float c[NT][4];
+    const char* words = ring + stage * kStageBytes + r8 * 128;
+    const float2* mp = meta + buffer * kMeta + r8;
+    const char* xb = xs + (((first - b0) * cols + r8) * 4 + t) * (kInt ? 8 : 16);
+    const int* sb = sums + (first - b0) * (NT * 8) + 2 * t;
+    constexpr int kUnits = GB / U;  // of a segment
     float2 m0, m1;
-    int left = 0, g = 0;  // of a group's blocks, without GB
-    if (GB == 0) left = w.group_blocks - first % w.group_blocks;
+    float c[NT][4];
+    int ci[NT][4];
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      if (b < here) {
-        const bool begins = GB ? b % (GB ? GB : 1) == 0 : b == 0 || left == w.group_blocks;
-        if (begins) {
-          const int gi = GB ? b / (GB ? GB : 1) : g;
-          m0 = mp[gi * 16];
-          m1 = mp[gi * 16 + 8];
-#pragma unroll
-          for (int q = 0; q < NT; ++q) c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.f;
-        }
-        const int at16 = (b ^ r8) << 4;
-        const uint32_t u0 = *reinterpret_cast<const uint32_t*>(words + at16);
-        const uint32_t u1 = *reinterpret_cast<const uint32_t*>(words + at16 + 1024);
-        const uint32_t z0 = __float_as_uint(m0.y), z1 = __float_as_uint(m1.y);
-        const uint32_t a0 = codes<0>(u0, z0), a1 = codes<0>(u1, z1), a2 = codes<1>(u0, z0), a3 = codes<1>(u1, z1);
-        const uint32_t d0 = codes<2>(u0, z0), d1 = codes<2>(u1, z1), d2 = codes<3>(u0, z0), d3 = codes<3>(u1, z1);
-        const uint4* xb = xs + ((first - b0 + b) * cols) * 4 + t;
+    for (int u = 0; u < kBlocks / U; ++u) {
+      if (u * U >= here) break;
+      if (u % kUnits == 0) {
+        m0 = mp[u / kUnits * 16];
+        m1 = mp[u / kUnits * 16 + 8];
 #pragma unroll
         for (int q = 0; q < NT; ++q) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (q * 8 + r8 < cols) v = xb[(q * 8 + r8) * 4];
-          mma_bf16(c[q], a0, a1, a2, a3, v.x, v.y);
-          mma_bf16(c[q], d0, d1, d2, d3, v.z, v.w);
-        }
-        const bool ends = b == here - 1 || (GB ? b % (GB ? GB : 1) == (GB ? GB : 1) - 1 : left == 1);
-        if (ends) {
-#pragma unroll
-          for (int q = 0; q < NT; ++q) {
-            acc[q][0] = fmaf(c[q][0], m0.x, acc[q][0]);
-            acc[q][1] = fmaf(c[q][1], m0.x, acc[q][1]);
-            acc[q][2] = fmaf(c[q][2], m1.x, acc[q][2]);
-            acc[q][3] = fmaf(c[q][3], m1.x, acc[q][3]);
+          if constexpr (kInt) {  // sums of x*(code - zero), as the low bits of 1.5*2^23
+            const int2 xsum = *reinterpret_cast<const int2*>(sb + u * U * NT * 8 + q * 8);
+            const int z0 = -__float_as_int(m0.y), z1 = -__float_as_int(m1.y);
+            ci[q][0] = 0x4b400000 + z0 * xsum.x;
+            ci[q][1] = 0x4b400000 + z0 * xsum.y;
+            ci[q][2] = 0x4b400000 + z1 * xsum.x;
+            ci[q][3] = 0x4b400000 + z1 * xsum.y;
+          } else {
+            c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.f;
           }
         }
-        if (GB == 0 && --left == 0) {
-          left = w.group_blocks;
-          ++g;
+      }
+      // U words of the lane's share of the unit, of rows r8 and r8 + 8.
+      uint32_t w0[U], w1[U];
+      const char* from0 = words + (((u * U + t * U / 4) ^ turn(r8)) << 4) + (t * U % 4) * 4;
+      load_words<U>(from0, w0);
+      load_words<U>(from0 + 1024, w1);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int b = u * U + j;
+        if constexpr (kInt) {
+          const uint32_t a0 = w0[j] & 0x0f0f0f0fu, a1 = w1[j] & 0x0f0f0f0fu;
+          const uint32_t a2 = w0[j] >> 4 & 0x0f0f0f0fu, a3 = w1[j] >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+          for (int q = 0; q < NT; ++q) {
+            uint2 v = make_uint2(0, 0);
+            if (q * 8 + r8 < cols) v = *reinterpret_cast<const uint2*>(xb + (b * cols + q * 8) * 32);
+            mma_int(ci[q], a0, a1, a2, a3, v.x, v.y);
+          }
+        } else {
+          const uint32_t z0 = __float_as_uint(m0.y), z1 = __float_as_uint(m1.y);
+          const uint32_t a0 = codes<0>(w0[j], z0), a1 = codes<0>(w1[j], z1);
+          const uint32_t a2 = codes<1>(w0[j], z0), a3 = codes<1>(w1[j], z1);
+          const uint32_t d0 = codes<2>(w0[j], z0), d1 = codes<2>(w1[j], z1);
+          const uint32_t d2 = codes<3>(w0[j], z0), d3 = codes<3>(w1[j], z1);
+#pragma unroll
+          for (int q = 0; q < NT; ++q) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (q * 8 + r8 < cols) v = *reinterpret_cast<const uint4*>(xb + (b * cols + q * 8) * 64);
+            mma_bf16(c[q], a0, a1, a2, a3, v.x, v.y);
+            mma_bf16(c[q], d0, d1, d2, d3, v.z, v.w);
+          }
         }
+      }
+      if (u % kUnits == kUnits - 1) {
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = kInt ? __int_as_float(ci[q][i]) - 12582912.f : c[q][i];
+            acc[q][i] = fmaf(v, i < 2 ? m0.x : m1.x, acc[q][i]);
+          }
       }
     }
     // The stage that this fetch fills was read in the round before.
     fetch(stage == 0 ? kStages - 1 : stage - 1);
     stage = stage + 1 == kStages ? 0 : stage + 1;
     buffer ^= 1;
-    mt.store(meta + buffer * 32 * kRegs, lane);
-    const int64_t tile = at.tile;
-    next(at);
-    if (at.tile == tile) {
+    mt.store(meta + buffer * kMeta, lane);
+    advance_load();
+    const int tile = at.tile;
+    if (!next(at)) {
       __syncwarp();
       continue;
     }
-    // The tile is done: join the warps' sums and the parts.
+    // The tile is done: join the warps' sums and a row's columns.
     float* mine = red + ((odd * sh.tiles + wt) * sh.along + wk) * kTile * NT * 8;
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
@@ -287,16 +436,31 @@ int4_linear_kernel(const Weights w, const Shape sh, const void* x, int64_t x_str
     }
     if (sh.along > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(sh.along * 32) : "memory");
     else __syncwarp();
-    const float* sums = red + (odd * sh.tiles + wt) * sh.along * kTile * NT * 8;
+    const float* part = red + (odd * sh.tiles + wt) * sh.along * kTile * NT * 8;
     for (int i = wk * 32 + lane; i < kTile * rows; i += sh.along * 32) {
       const int row = i % kTile, r = i / kTile;
-      const int64_t n = tile * kTile + row;
+      const int64_t n = (int64_t)tile * kTile + row;
       if (n >= w.n) continue;
-      float v = 0.f;
-      for (int q = 0; q < sh.along; ++q)
-        for (int p = 0; p < parts; ++p) v += sums[(q * kTile + row) * NT * 8 + r * parts + p];
-      if (partial) partial[((int64_t)blockIdx.z * all_rows + row0 + r) * w.n + n] = v;
-      else store_f32(y, dtype, (row0 + r) * w.n + n, bias ? v + load_as_f32(bias, dtype, n) : v);
+      float v = 0.f, unit = 1.f;
+      for (int p = 0; p < in.parts; ++p) {
+        float a = 0.f;
+        for (int q = 0; q < sh.along; ++q) a += part[(q * kTile + row) * NT * 8 + r * in.parts + p];
+        v = fmaf(a, unit, v);
+        if (kInt) unit *= 256.f;
+      }
+      if constexpr (kInt) {
+        v = scalbnf(v, -power[r]);
+        if (bad[r])  // infinities and NaN of the row, one by one
+          for (int k = b0 * 32; k < min(w.k, (b0 + nb) * 32); ++k) {
+            const float xv = load_as_f32(in.x, in.dtype, (int64_t)(row0 + r) * in.stride + k);
+            if (finite(xv)) continue;
+            const int64_t g = n * w.groups + k / (w.group_blocks * 32);
+            const int code = w.packed[n * pitch + k / 2] >> (k & 1) * 4 & 15;
+            v += xv * ((float)(code - (w.zeros ? w.zeros[g] : 8)) * load_as_f32(w.scales, w.scale_dtype, g));
+          }
+      }
+      if (partial) partial[((int64_t)blockIdx.z * in.all + row0 + r) * w.n + n] = v;
+      else store_f32(y, in.dtype, (row0 + r) * w.n + n, bias ? v + load_as_f32(bias, in.dtype, n) : v);
     }
     odd ^= 1;
   }
@@ -373,60 +537,67 @@ Weights make_weights(const uint8_t* packed, const void* scales, int scale_dtype,
 
 struct ForwardPlan {
   Shape sh;
-  int pass_rows, passes, nt, gb, grid, smem;
+  bool ints;
+  int parts, pass_rows, passes, nt, gb, grid, smem;
 };
 
-// Rows a pass: what 32 columns of a product hold.  The columns of the weight are cut
-// into slices where the staged rows would take more than 64 KB a CTA, and where
-// fewer than two tiles a SM would leave SMs without work.
+// Rows a pass: what 32 columns of a product hold.  16-bit rows go to the integer
+// products while one pass holds them; more of them take fewer columns as bf16 parts
+// (of measured bandwidth at 122,880 x 5120, group 64: see launch_forward).  The columns
+// of the weight are cut into slices where the staged rows would take more than 64 KB
+// a CTA, and where too few tiles would leave SMs without work.
 ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   ForwardPlan p{};
-  const int parts = parts_of(dtype);
-  p.pass_rows = (int)std::min<int64_t>(rows, 32 / parts);
+  p.ints = dtype != SPR_F32 && rows <= 32 / kLimbs;
+  p.parts = p.ints ? kLimbs : parts_of(dtype);
+  p.pass_rows = (int)std::min<int64_t>(rows, 32 / p.parts);
   p.passes = (int)((rows + p.pass_rows - 1) / p.pass_rows);
-  const int cols = p.pass_rows * parts;
+  const int cols = p.pass_rows * p.parts;
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  p.gb = w.group_blocks == 1 || w.group_blocks == 2 || w.group_blocks == 4 ? w.group_blocks : 0;
+  p.gb = w.group_blocks % 8 == 0 ? 8 : w.group_blocks % 4 == 0 ? 4 : w.group_blocks % 2 == 0 ? 2 : 1;
   const int chunks = (w.blocks + kBlocks - 1) / kBlocks;
   const int64_t tiles = (w.n + kTile - 1) / kTile;
-  const int chunk_bytes = kBlocks * cols * 64;
+  const int chunk_bytes = kBlocks * (p.ints ? cols * 32 + p.nt * 32 : cols * 64);
   const int64_t sms = sm_count();
   int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + 65535) / 65536));
   if (tiles * p.passes < sms) slices = std::max<int64_t>(slices, std::min<int64_t>(chunks / 4, sms / (tiles * p.passes)));
   p.sh.slice_chunks = (chunks + slices - 1) / slices;
   p.sh.slices = (chunks + p.sh.slice_chunks - 1) / p.sh.slice_chunks;
-  // Warps on a tile: the number that shares its chunks most evenly.
-  int along = 1;
-  for (int a = 2; a <= std::min(kWarps, p.sh.slice_chunks); ++a) {
-    const int steps_a = (p.sh.slice_chunks + a - 1) / a, steps = (p.sh.slice_chunks + along - 1) / along;
-    if (steps_a * a * 8 <= p.sh.slice_chunks * 9 || steps_a * a <= steps * along) along = a;
-  }
-  p.sh.along = along;
+  // Warps on a tile: few, so that the sums they join cost little, but so that neither
+  // the tiles over all teams nor the chunks over a team's warps leave many idle.
   const int64_t work = tiles * p.passes * p.sh.slices;
-  p.sh.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(kWarps / along, work / (2 * sms)));
-  const int warps = along * p.sh.tiles;
-  p.smem = warps * (kStages * kStageBytes + 2 * 32 * kMetaRegs(p.gb) * 8 + 2 * kTile * p.nt * 8 * 4) +
+  double best = 0;
+  for (int a = 1; a <= kWarps && a <= p.sh.slice_chunks; a *= 2) {
+    const double teams = (double)(2 * kWarps / a * sms), share = work / teams, steps = (double)p.sh.slice_chunks / a;
+    const double busy = share / ceil(share) * steps / ceil(steps);
+    if (busy > best * 1.04) {
+      best = busy;
+      p.sh.along = a;
+    }
+  }
+  p.sh.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(kWarps / p.sh.along, (work + sms - 1) / sms));
+  const int warps = p.sh.along * p.sh.tiles;
+  p.smem = warps * (kStages * kStageBytes + 2 * std::max(1, kBlocks / p.gb / 2) * 32 * 8 + 2 * kTile * p.nt * 8 * 4) +
            p.sh.slice_chunks * chunk_bytes;
   const int64_t teams = (tiles + p.sh.tiles - 1) / p.sh.tiles;
-  const int64_t fit = std::max(1, std::min(227 * 1024 / (p.smem + 1024), 16 / warps));  // 128 registers a thread
+  const int64_t fit = std::max(1, std::min(227 * 1024 / (p.smem + 2048), 16 / warps));  // 128 registers a thread
   p.grid = (int)std::min(teams, std::max<int64_t>(1, sms * fit / (p.passes * p.sh.slices)));
   return p;
 }
 
-template <int NT, int GB>
+template <int NT, int GB, bool kInt>
 int launch_forward(const ForwardPlan& p, const Weights& w, const void* x, int64_t x_stride, int dtype, int rows,
                    const void* bias, void* y, float* partial, cudaStream_t st) {
-  auto kern = int4_linear_kernel<NT, GB>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+  auto kern = int4_linear_kernel<NT, GB, kInt>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024) != cudaSuccess)
     return check_launch("int4 linear");
-  // A group's inner sum of up to 15*group values of x stays below the largest fp32
-  // number: x is taken times a power of two and the scale divided by it.
+  // A bf16 product's inner sum of up to 15*32*GB values of x stays below the largest
+  // fp32 number: x is taken times a power of two and the scale divided by it.
   int e = 4;
-  while ((1 << (e - 4)) < w.group_blocks * 32) ++e;
-  const dim3 grid(p.grid, p.passes, p.sh.slices);
-  kern<<<grid, p.sh.along * p.sh.tiles * 32, p.smem, st>>>(w, p.sh, x, x_stride, dtype, parts_of(dtype), rows,
-                                                           p.pass_rows, ldexpf(1.f, -e), ldexpf(1.f, e),
-                                                           partial ? nullptr : bias, y, partial);
+  while ((1 << (e - 4)) < GB * 32) ++e;
+  const Rows in{x, x_stride, dtype, p.parts, rows, p.pass_rows};
+  kern<<<dim3(p.grid, p.passes, p.sh.slices), p.sh.along * p.sh.tiles * 32, p.smem, st>>>(
+      w, p.sh, in, kInt ? 1.f : ldexpf(1.f, -e), kInt ? 1.f : ldexpf(1.f, e), partial ? nullptr : bias, y, partial);
   if (partial) {
     const int64_t size = (int64_t)rows * w.n;
     int4_join_kernel<<<(unsigned)((size + 255) / 256), 256, 0, st>>>(partial, p.sh.slices, size, w.n, bias, y, dtype);
@@ -434,13 +605,18 @@ int launch_forward(const ForwardPlan& p, const Weights& w, const void* x, int64_
   return check_launch("int4 linear");
 }
 
-template <int NT>
-int launch_forward_by_group(const ForwardPlan& p, const Weights& w, const void* x, int64_t x_stride, int dtype, int rows,
-                            const void* bias, void* y, float* partial, cudaStream_t st) {
-  if (p.gb == 1) return launch_forward<NT, 1>(p, w, x, x_stride, dtype, rows, bias, y, partial, st);
-  if (p.gb == 2) return launch_forward<NT, 2>(p, w, x, x_stride, dtype, rows, bias, y, partial, st);
-  if (p.gb == 4) return launch_forward<NT, 4>(p, w, x, x_stride, dtype, rows, bias, y, partial, st);
-  return launch_forward<NT, 0>(p, w, x, x_stride, dtype, rows, bias, y, partial, st);
+// Calls f(Int<NT>{}, Int<GB>{}, Int<integers>{}) for a plan.
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+template <typename F>
+int by_plan(const ForwardPlan& p, F f) {
+  auto by_group = [&](auto nt) {
+    auto by_kind = [&](auto gb) { return p.ints ? f(nt, gb, Int<1>{}) : f(nt, gb, Int<0>{}); };
+    return p.gb == 8 ? by_kind(Int<8>{}) : p.gb == 4 ? by_kind(Int<4>{}) : p.gb == 2 ? by_kind(Int<2>{}) : by_kind(Int<1>{});
+  };
+  return p.nt == 1 ? by_group(Int<1>{}) : p.nt == 2 ? by_group(Int<2>{}) : by_group(Int<4>{});
 }
 
 }  // namespace
@@ -469,9 +645,10 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
     return fail(SPR_ERR_WORKSPACE, "int4 linear: workspace %zu < %zu bytes", workspace_bytes, need);
   float* partial = need ? (float*)workspace : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
-  if (p.nt == 1) return launch_forward_by_group<1>(p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
-  if (p.nt == 2) return launch_forward_by_group<2>(p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
-  return launch_forward_by_group<4>(p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
+  return by_plan(p, [&](auto nt, auto gb, auto ints) {
+    return launch_forward<decltype(nt)::value, decltype(gb)::value, decltype(ints)::value != 0>(
+        p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
+  });
 }
 
 extern "C" size_t spr_int4_linear_grad_workspace_bytes(int64_t, int64_t, int64_t, int, int) { return 0; }
