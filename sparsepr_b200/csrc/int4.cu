@@ -23,7 +23,7 @@ namespace spr {
 
 namespace {
 
-constexpr int kWarps = 8;  // of a CTA, at most
+constexpr int most_warps(int nt) { return nt == 1 ? 16 : nt == 2 ? 12 : 8; }  // of a CTA: what shared memory holds
 constexpr int kTile = 16;  // weight rows of a product
 constexpr int kBlocks = 8;  // blocks of 32 codes in one stage of a warp's ring: 128 bytes of a row
 constexpr int kStages = 4;
@@ -120,37 +120,49 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[U]) {
   }
 }
 
-// Scale and zero of a stage's rows and segments (GB blocks, within one group), loaded
-// one stage ahead into registers, then put where the warp's lanes find them.
-template <int GB, bool kInt>
-struct Meta {
-  static constexpr int kRegs = kBlocks / GB * kTile / 32 > 0 ? kBlocks / GB * kTile / 32 : 1;
+// Scales and zeros of a warp's weight rows.  Where a row's lie in whole aligned pieces
+// of eight groups (kScale, their bytes), all that the warp needs of a tile is copied
+// with the tile's first chunk: neighbouring lanes take neighbouring pieces, so that a
+// row's are few memory requests.  Otherwise (kScale 0) the values of each chunk's
+// segments (GB blocks, within one group) are loaded one chunk ahead into registers.
+// A row's pieces and one more, if even, lie apart from the next row's: an odd number
+// keeps the rows in different banks.
+struct Pieces {
+  int first, count, pitch;  // of eight groups; pitch odd
+};
+constexpr int piece_bytes(int scale) { return 8 * (scale ? scale : 4) + 8; }
+
+template <int GB>
+struct Values {
+  static constexpr int kSegments = kBlocks / GB, kRegs = kSegments > 1 ? kSegments / 2 : 1;
   float scale[kRegs];
-  uint32_t zero[kRegs];
-  __device__ __forceinline__ void load(const Weights& w, int64_t row_at, int chunk, int lane, float up) {
-    // row_at: the lane's row's first group.
+  uint8_t zero[kRegs];
+  __device__ __forceinline__ void load(const Weights& w, int64_t row_at, int chunk, int lane) {
+    // row_at: the first group of weight row lane & 15
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) {
-      int g = chunk * (kBlocks / GB) + 2 * i + (lane >> 4);
-      if (w.group_blocks != GB) g = g * GB / w.group_blocks;
-      g = min(g, w.groups - 1);
-      scale[i] = load_as_f32(w.scales, w.scale_dtype, row_at + g) * up;
-      zero[i] = w.zeros ? (uint32_t)__ldg(w.zeros + row_at + g) : 8u;
+      const int g = min((chunk * kSegments + 2 * i + (lane >> 4)) * GB / w.group_blocks, w.groups - 1);
+      scale[i] = load_as_f32(w.scales, w.scale_dtype, row_at + g);
+      zero[i] = w.zeros ? __ldg(w.zeros + row_at + g) : 8;
     }
   }
-  __device__ __forceinline__ void store(float2* meta, int lane) const {
+  __device__ __forceinline__ void store(char* slot, int lane) const {  // as one piece a row, fp32
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      meta[i * 32 + lane] =
-          make_float2(scale[i], __uint_as_float(kInt ? zero[i] : 0x43004300u + 0x00010001u * zero[i]));
+    for (int i = 0; i < kRegs; ++i) {
+      const int at = (lane & 15) * 8 + 2 * i + (lane >> 4);
+      reinterpret_cast<float*>(slot)[at] = scale[i];
+      reinterpret_cast<uint8_t*>(slot + kTile * 32)[at] = zero[i];
+    }
   }
 };
 
-// Where a launch's warps work: `along` warps of a CTA share a tile, each with every
-// `along`-th chunk of the CTA's slice of the columns; `tiles` such teams to a CTA.
+// Where a launch's warps work: `along` warps of a CTA share a tile, each with
+// `warp_chunks` neighbouring chunks of the CTA's slice of the columns; `tiles` such
+// teams to a CTA.
 struct Shape {
-  int along, tiles;
+  int along, tiles, warp_chunks;
   int slice_chunks, slices;
+  int slots, slot_bytes;  // a warp's slots of scales and zeros
 };
 
 // Eight values of x from column k, zeros past the end.
@@ -166,6 +178,22 @@ __device__ __forceinline__ void load_x(const Rows& in, bool wide, int64_t at, in
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = k + e < k_end ? load_as_f32(in.x, in.dtype, at + e) : 0.f;
   }
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1,%2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
@@ -257,12 +285,11 @@ __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int 
 
 // y for up to NT*8 columns (a row's parts or bytes each one): warp products of 16 weight
 // rows by 32 columns of the weight a step.
-template <int NT, int GB, bool kInt>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+template <int NT, int GB, bool kInt, int kScale>
+__global__ void __launch_bounds__(most_warps(NT) * 32)
 int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, float up, const void* bias, void* y,
                    float* partial) {
-  using M = Meta<GB, kInt>;
-  constexpr int U = GB < 4 ? GB : 4, kMeta = M::kRegs * 32;
+  constexpr int U = GB < 4 ? GB : 4, kUnits = GB / U;  // a unit's blocks, a segment's units
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t largest[32];
   __shared__ int power[32], bad[32];
@@ -272,84 +299,119 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   const int c1 = min((w.blocks + kBlocks - 1) / kBlocks, c0 + sh.slice_chunks);
   const int b0 = c0 * kBlocks, nb = min(w.blocks, c1 * kBlocks) - b0;  // the slice's blocks
   char* ring = smem + warp * kStages * kStageBytes;
-  float2* meta = reinterpret_cast<float2*>(smem + warps * kStages * kStageBytes) + warp * 2 * kMeta;
-  float* red = reinterpret_cast<float*>(smem + warps * (kStages * kStageBytes + 2 * kMeta * 8));
+  char* slots = smem + warps * kStages * kStageBytes + warp * sh.slots * sh.slot_bytes;
+  float* red = reinterpret_cast<float*>(smem + warps * (kStages * kStageBytes + sh.slots * sh.slot_bytes));
   char* xs = reinterpret_cast<char*>(red + 2 * warps * kTile * NT * 8);
   int* sums = reinterpret_cast<int*>(xs + nb * cols * 32);  // integers only
 
   const int wt = warp / sh.along, wk = warp % sh.along;
   const int tiles = (int)((w.n + kTile - 1) / kTile), tile_step = gridDim.x * sh.tiles;
+  const int from_chunk = c0 + wk * sh.warp_chunks, to_chunk = min(c1, from_chunk + sh.warp_chunks);
   const int64_t pitch = (int64_t)w.blocks * 16;
-  // Three places in the warp's sequence of stages: being copied, its scales being
-  // loaded, being computed.
+  // Two places in the warp's sequence of chunks: being copied, being computed (and
+  // without kScale a third: its scales being loaded).  A warp without chunks passes
+  // over each tile once.
   struct Place {
     int tile, chunk;
   };
   auto next = [&](Place& p) {
-    p.chunk += sh.along;
-    if (p.chunk >= c1) {
-      p.chunk = c0 + wk;
-      p.tile += tile_step;
-      return true;
-    }
-    return false;
+    if (++p.chunk < to_chunk) return false;
+    p.chunk = from_chunk;
+    p.tile += tile_step;
+    return true;
   };
-  const Place start = {(int)(blockIdx.x * sh.tiles + wt), c0 + wk};
-  Place copy = start, load = start, at = start;
+  const Place start = {(int)(blockIdx.x * sh.tiles + wt), from_chunk};
+  Place copy = start, at = start, load = start;
 
-  const uint8_t* from[kTile / 4];  // the lane's 16 bytes in the first chunk of rows lane/8 + 4i
+  Pieces pc;
+  pc.first = from_chunk * kBlocks / w.group_blocks / 8;
+  pc.count = max(0, (min(w.blocks, to_chunk * kBlocks) - 1) / w.group_blocks / 8 + 1 - pc.first);
+  pc.pitch = kScale ? pc.count | 1 : 1;
+  const uint32_t inv_count = pc.count > 0 ? (65536 + pc.count - 1) / pc.count : 0;  // i / count for i < 16*count < 4096
+  const uint8_t* from[kTile / 4];  // the lane's 16 bytes of rows lane/8 + 4i, in the chunk to copy
   auto aim = [&]() {
 #pragma unroll
     for (int i = 0; i < kTile / 4; ++i)
-      from[i] = w.packed + min((int64_t)copy.tile * kTile + i * 4 + (lane >> 3), w.n - 1) * pitch + (lane & 7) * 16;
+      from[i] = w.packed + min((int64_t)copy.tile * kTile + i * 4 + (lane >> 3), w.n - 1) * pitch + (lane & 7) * 16 +
+                from_chunk * (kBlocks * 16);
   };
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), slot_at = (uint32_t)__cvta_generic_to_shared(slots);
   uint32_t to[kTile / 4];
 #pragma unroll
-  for (int i = 0; i < kTile / 4; ++i)
-    to[i] = (uint32_t)__cvta_generic_to_shared(ring) + piece(i * 4 + (lane >> 3), lane & 7);
+  for (int i = 0; i < kTile / 4; ++i) to[i] = ring_at + piece(i * 4 + (lane >> 3), lane & 7);
   aim();
+  int copy_slot = 0, use_slot = 0;
+  auto copy_scales = [&]() {
+    const uint32_t dst = slot_at + copy_slot * sh.slot_bytes, dst_zero = dst + kTile * pc.pitch * 8 * kScale;
+    copy_slot = copy_slot + 1 == sh.slots ? 0 : copy_slot + 1;
+    for (int i = lane; i < kTile * pc.count; i += 32) {
+      const int row = i * inv_count >> 16, p = i - row * pc.count;
+      const int64_t g = min((int64_t)copy.tile * kTile + row, w.n - 1) * w.groups + (pc.first + p) * 8;
+      const int slot = row * pc.pitch + p;
+#pragma unroll
+      for (int h = 0; h < kScale / 2; ++h)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + slot * 8 * kScale + h * 16),
+                     "l"((const char*)w.scales + g * kScale + h * 16)
+                     : "memory");
+      if (w.zeros)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst_zero + slot * 8), "l"(w.zeros + g) : "memory");
+    }
+  };
   auto fetch = [&](int stage) {
     if (copy.tile < tiles) {
-      if (copy.chunk * kBlocks + (lane & 7) < w.blocks)
+      if (copy.chunk * kBlocks + (lane & 7) < w.blocks && copy.chunk < to_chunk)
 #pragma unroll
         for (int i = 0; i < kTile / 4; ++i)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kStageBytes),
-                       "l"(from[i] + copy.chunk * (kBlocks * 16))
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kStageBytes), "l"(from[i])
                        : "memory");
+      if (kScale && copy.chunk == from_chunk) copy_scales();
+#pragma unroll
+      for (int i = 0; i < kTile / 4; ++i) from[i] += kBlocks * 16;
       if (next(copy)) aim();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
-  M mt;
-  int64_t load_at = min((int64_t)load.tile * kTile + (lane & 15), w.n - 1) * w.groups;
-  if (load.tile < tiles) mt.load(w, load_at, load.chunk, lane, up);
+  Values<GB> values;
+  int64_t load_at = 0;
+  if constexpr (!kScale) {
+    load_at = min((int64_t)load.tile * kTile + (lane & 15), w.n - 1) * w.groups;
+    if (load.tile < tiles) values.load(w, load_at, load.chunk, lane);
+  }
 
   const bool wide = in.dtype != SPR_F32 && in.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in.x) % 16 == 0;
   if constexpr (kInt)
     stage_int<U, GB>(w, in, row0, rows, b0, nb, wide, reinterpret_cast<uint2*>(xs), sums, NT * 8, largest, power, bad);
   else stage_bf16<U>(w, in, row0, rows, b0, nb, down, wide, reinterpret_cast<uint4*>(xs));
-  mt.store(meta, lane);
   __syncthreads();
-  auto advance_load = [&]() {
-    if (next(load)) load_at = min((int64_t)load.tile * kTile + (lane & 15), w.n - 1) * w.groups;
-  };
-  advance_load();
 
-  float acc[NT][4] = {};
-  int stage = 0, buffer = 0, odd = 0;
+  uint64_t acc[NT][2] = {};  // pairs of neighbouring columns, rows r8 and r8 + 8
+  int stage = 0, odd = 0;
   const int t = lane & 3, r8 = lane >> 2;
+  const char* lane_words = ring + r8 * 128;
+  int col_at[NT];  // a lane past the last column reads that one; its sums are not used
+#pragma unroll
+  for (int q = 0; q < NT; ++q) col_at[q] = (min(q * 8 + r8, cols - 1) * 4 + t) * (kInt ? 8 : 16);
+  const int block_bytes = cols * (kInt ? 32 : 64);
   while (at.tile < tiles) {
-    if (load.tile < tiles) mt.load(w, load_at, load.chunk, lane, up);
+    if constexpr (!kScale) {
+      values.store(slots + use_slot * sh.slot_bytes, lane);
+      if (next(load)) load_at = min((int64_t)load.tile * kTile + (lane & 15), w.n - 1) * w.groups;
+      if (load.tile < tiles) values.load(w, load_at, load.chunk, lane);
+    }
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();
-    const int first = at.chunk * kBlocks, here = min(kBlocks, w.blocks - first);
-    const char* words = ring + stage * kStageBytes + r8 * 128;
-    const float2* mp = meta + buffer * kMeta + r8;
-    const char* xb = xs + (((first - b0) * cols + r8) * 4 + t) * (kInt ? 8 : 16);
+    const int first = at.chunk * kBlocks, here = at.chunk < to_chunk ? min(kBlocks, w.blocks - first) : 0;
+    const char* words = lane_words + stage * kStageBytes;
+    const char* xb = xs + (first - b0) * block_bytes;
     const int* sb = sums + (first - b0) * (NT * 8) + 2 * t;
-    constexpr int kUnits = GB / U;  // of a segment
+    // The lane's rows' scales and zeros, from the chunk's first segment's group on.
+    const char* slot = slots + use_slot * sh.slot_bytes;
+    const int group0 = kScale ? (GB < 8 ? first / GB : first / w.group_blocks) - pc.first * 8 : 0;
+    const char* sp = slot + r8 * pc.pitch * 8 * (kScale ? kScale : 4) + group0 * (kScale ? kScale : 4);
+    const uint8_t* zp = reinterpret_cast<const uint8_t*>(slot) + kTile * pc.pitch * 8 * (kScale ? kScale : 4) +
+                        r8 * pc.pitch * 8 + group0;
     float2 m0, m1;
     float c[NT][4];
     int ci[NT][4];
@@ -357,17 +419,34 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
     for (int u = 0; u < kBlocks / U; ++u) {
       if (u * U >= here) break;
       if (u % kUnits == 0) {
-        m0 = mp[u / kUnits * 16];
-        m1 = mp[u / kUnits * 16 + 8];
+        const int g = u / kUnits;
+        if constexpr (kScale == 2) {
+          const uint16_t h0 = reinterpret_cast<const uint16_t*>(sp)[g];
+          const uint16_t h1 = reinterpret_cast<const uint16_t*>(sp + pc.pitch * 128)[g];
+          const bool bf = w.scale_dtype == SPR_BF16;
+          m0.x = bf ? __uint_as_float((uint32_t)h0 << 16) : __half2float(__ushort_as_half(h0));
+          m1.x = bf ? __uint_as_float((uint32_t)h1 << 16) : __half2float(__ushort_as_half(h1));
+        } else {
+          m0.x = reinterpret_cast<const float*>(sp)[g];
+          m1.x = reinterpret_cast<const float*>(sp + pc.pitch * 256)[g];
+        }
+        int z0 = 8, z1 = 8;
+        if (!kScale || w.zeros) {
+          z0 = zp[g];
+          z1 = zp[pc.pitch * 64 + g];
+        }
+        if constexpr (!kInt) {
+          m0.y = __int_as_float(0x43004300 + 0x00010001 * z0);
+          m1.y = __int_as_float(0x43004300 + 0x00010001 * z1);
+        }
 #pragma unroll
         for (int q = 0; q < NT; ++q) {
           if constexpr (kInt) {  // sums of x*(code - zero), as the low bits of 1.5*2^23
             const int2 xsum = *reinterpret_cast<const int2*>(sb + u * U * NT * 8 + q * 8);
-            const int z0 = -__float_as_int(m0.y), z1 = -__float_as_int(m1.y);
-            ci[q][0] = 0x4b400000 + z0 * xsum.x;
-            ci[q][1] = 0x4b400000 + z0 * xsum.y;
-            ci[q][2] = 0x4b400000 + z1 * xsum.x;
-            ci[q][3] = 0x4b400000 + z1 * xsum.y;
+            ci[q][0] = 0x4b400000 - z0 * xsum.x;
+            ci[q][1] = 0x4b400000 - z0 * xsum.y;
+            ci[q][2] = 0x4b400000 - z1 * xsum.x;
+            ci[q][3] = 0x4b400000 - z1 * xsum.y;
           } else {
             c[q][0] = c[q][1] = c[q][2] = c[q][3] = 0.f;
           }
@@ -380,14 +459,13 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
       load_words<U>(from0 + 1024, w1);
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int b = u * U + j;
+        const char* xj = xb + (u * U + j) * block_bytes;
         if constexpr (kInt) {
           const uint32_t a0 = w0[j] & 0x0f0f0f0fu, a1 = w1[j] & 0x0f0f0f0fu;
           const uint32_t a2 = w0[j] >> 4 & 0x0f0f0f0fu, a3 = w1[j] >> 4 & 0x0f0f0f0fu;
 #pragma unroll
           for (int q = 0; q < NT; ++q) {
-            uint2 v = make_uint2(0, 0);
-            if (q * 8 + r8 < cols) v = *reinterpret_cast<const uint2*>(xb + (b * cols + q * 8) * 32);
+            const uint2 v = *reinterpret_cast<const uint2*>(xj + col_at[q]);
             mma_int(ci[q], a0, a1, a2, a3, v.x, v.y);
           }
         } else {
@@ -398,8 +476,7 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
           const uint32_t d2 = codes<3>(w0[j], z0), d3 = codes<3>(w1[j], z1);
 #pragma unroll
           for (int q = 0; q < NT; ++q) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (q * 8 + r8 < cols) v = *reinterpret_cast<const uint4*>(xb + (b * cols + q * 8) * 64);
+            const uint4 v = *reinterpret_cast<const uint4*>(xj + col_at[q]);
             mma_bf16(c[q], a0, a1, a2, a3, v.x, v.y);
             mma_bf16(c[q], d0, d1, d2, d3, v.z, v.w);
           }
@@ -409,30 +486,29 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
 #pragma unroll
         for (int q = 0; q < NT; ++q)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v = kInt ? __int_as_float(ci[q][i]) - 12582912.f : c[q][i];
-            acc[q][i] = fmaf(v, i < 2 ? m0.x : m1.x, acc[q][i]);
+          for (int i = 0; i < 2; ++i) {
+            uint64_t v = kInt ? pair(__int_as_float(ci[q][2 * i]), __int_as_float(ci[q][2 * i + 1]))
+                              : pair(c[q][2 * i], c[q][2 * i + 1]);
+            if (kInt) v = add2(v, pair(-12582912.f, -12582912.f));
+            const float m = i ? m1.x : m0.x;
+            acc[q][i] = fma2(v, pair(m, m), acc[q][i]);
           }
       }
     }
     // The stage that this fetch fills was read in the round before.
     fetch(stage == 0 ? kStages - 1 : stage - 1);
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    buffer ^= 1;
-    mt.store(meta + buffer * kMeta, lane);
-    advance_load();
     const int tile = at.tile;
-    if (!next(at)) {
-      __syncwarp();
-      continue;
-    }
+    const bool done = next(at);
+    if (!kScale || done) use_slot = use_slot + 1 == sh.slots ? 0 : use_slot + 1;
+    if (!done) continue;
     // The tile is done: join the warps' sums and a row's columns.
     float* mine = red + ((odd * sh.tiles + wt) * sh.along + wk) * kTile * NT * 8;
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
-      *reinterpret_cast<float2*>(mine + r8 * NT * 8 + q * 8 + 2 * t) = make_float2(acc[q][0], acc[q][1]);
-      *reinterpret_cast<float2*>(mine + (r8 + 8) * NT * 8 + q * 8 + 2 * t) = make_float2(acc[q][2], acc[q][3]);
-      acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.f;
+      *reinterpret_cast<uint64_t*>(mine + r8 * NT * 8 + q * 8 + 2 * t) = acc[q][0];
+      *reinterpret_cast<uint64_t*>(mine + (r8 + 8) * NT * 8 + q * 8 + 2 * t) = acc[q][1];
+      acc[q][0] = acc[q][1] = 0;
     }
     if (sh.along > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(sh.along * 32) : "memory");
     else __syncwarp();
@@ -458,6 +534,8 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
             const int code = w.packed[n * pitch + k / 2] >> (k & 1) * 4 & 15;
             v += xv * ((float)(code - (w.zeros ? w.zeros[g] : 8)) * load_as_f32(w.scales, w.scale_dtype, g));
           }
+      } else {
+        v *= up;
       }
       if (partial) partial[((int64_t)blockIdx.z * in.all + row0 + r) * w.n + n] = v;
       else store_f32(y, in.dtype, (row0 + r) * w.n + n, bias ? v + load_as_f32(bias, in.dtype, n) : v);
@@ -535,16 +613,19 @@ Weights make_weights(const uint8_t* packed, const void* scales, int scale_dtype,
   return w;
 }
 
+constexpr int kSmem = 225 * 1024;  // of a CTA at most, less what a kernel declares itself
+
 struct ForwardPlan {
   Shape sh;
   bool ints;
+  int scale;  // bytes of a scale that is copied ahead, 0: none is
   int parts, pass_rows, passes, nt, gb, grid, smem;
 };
 
 // Rows a pass: what 32 columns of a product hold.  16-bit rows go to the integer
 // products while one pass holds them; more of them take fewer columns as bf16 parts
 // (of measured bandwidth at 122,880 x 5120, group 64: see launch_forward).  The columns
-// of the weight are cut into slices where the staged rows would take more than 64 KB
+// of the weight are cut into slices where the staged rows would take more than 36 KB
 // a CTA, and where too few tiles would leave SMs without work.
 ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   ForwardPlan p{};
@@ -559,7 +640,13 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   const int64_t tiles = (w.n + kTile - 1) / kTile;
   const int chunk_bytes = kBlocks * (p.ints ? cols * 32 + p.nt * 32 : cols * 64);
   const int64_t sms = sm_count();
-  int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + 65535) / 65536));
+  const int most = most_warps(p.nt);
+  // Pieces of eight scales, whole and aligned, and groups that a chunk does not straddle.
+  p.scale = w.groups % 8 == 0 && (kBlocks % w.group_blocks == 0 || w.group_blocks % kBlocks == 0) &&
+                    aligned(w.scales, 16) && aligned(w.zeros, 8)
+                ? dtype_bytes(w.scale_dtype)
+                : 0;
+  int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + 36863) / 36864));
   if (tiles * p.passes < sms) slices = std::max<int64_t>(slices, std::min<int64_t>(chunks / 4, sms / (tiles * p.passes)));
   p.sh.slice_chunks = (chunks + slices - 1) / slices;
   p.sh.slices = (chunks + p.sh.slice_chunks - 1) / p.sh.slice_chunks;
@@ -567,29 +654,35 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   // the tiles over all teams nor the chunks over a team's warps leave many idle.
   const int64_t work = tiles * p.passes * p.sh.slices;
   double best = 0;
-  for (int a = 1; a <= kWarps && a <= p.sh.slice_chunks; a *= 2) {
-    const double teams = (double)(2 * kWarps / a * sms), share = work / teams, steps = (double)p.sh.slice_chunks / a;
+  for (int a = 1; a <= std::min(8, most) && a <= p.sh.slice_chunks; a *= 2) {
+    const double teams = (double)(most / a * sms), share = work / teams, steps = (double)p.sh.slice_chunks / a;
     const double busy = share / ceil(share) * steps / ceil(steps);
     if (busy > best * 1.04) {
       best = busy;
       p.sh.along = a;
     }
   }
-  p.sh.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(kWarps / p.sh.along, (work + sms - 1) / sms));
+  p.sh.warp_chunks = (p.sh.slice_chunks + p.sh.along - 1) / p.sh.along;
+  // Slots: the tile at work and those that the copies may have reached.
+  const int pieces = p.scale ? (p.sh.warp_chunks * kBlocks - 1) / (w.group_blocks * 8) + 2 : 1;
+  p.sh.slot_bytes = kTile * (p.scale ? pieces | 1 : 1) * piece_bytes(p.scale);
+  p.sh.slots = p.scale ? 1 + (kStages - 1 + p.sh.warp_chunks - 1) / p.sh.warp_chunks : 2;
+  const int warp_bytes = kStages * kStageBytes + p.sh.slots * p.sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
+  const int fit_warps = (kSmem - p.sh.slice_chunks * chunk_bytes) / warp_bytes;
+  p.sh.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, fit_warps) / p.sh.along, (work + sms - 1) / sms));
   const int warps = p.sh.along * p.sh.tiles;
-  p.smem = warps * (kStages * kStageBytes + 2 * std::max(1, kBlocks / p.gb / 2) * 32 * 8 + 2 * kTile * p.nt * 8 * 4) +
-           p.sh.slice_chunks * chunk_bytes;
+  p.smem = warps * warp_bytes + p.sh.slice_chunks * chunk_bytes;
   const int64_t teams = (tiles + p.sh.tiles - 1) / p.sh.tiles;
   const int64_t fit = std::max(1, std::min(227 * 1024 / (p.smem + 2048), 16 / warps));  // 128 registers a thread
   p.grid = (int)std::min(teams, std::max<int64_t>(1, sms * fit / (p.passes * p.sh.slices)));
   return p;
 }
 
-template <int NT, int GB, bool kInt>
+template <int NT, int GB, bool kInt, int kScale>
 int launch_forward(const ForwardPlan& p, const Weights& w, const void* x, int64_t x_stride, int dtype, int rows,
                    const void* bias, void* y, float* partial, cudaStream_t st) {
-  auto kern = int4_linear_kernel<NT, GB, kInt>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024) != cudaSuccess)
+  auto kern = int4_linear_kernel<NT, GB, kInt, kScale>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
     return check_launch("int4 linear");
   // A bf16 product's inner sum of up to 15*32*GB values of x stays below the largest
   // fp32 number: x is taken times a power of two and the scale divided by it.
@@ -605,7 +698,7 @@ int launch_forward(const ForwardPlan& p, const Weights& w, const void* x, int64_
   return check_launch("int4 linear");
 }
 
-// Calls f(Int<NT>{}, Int<GB>{}, Int<integers>{}) for a plan.
+// Calls f(Int<NT>{}, Int<GB>{}, Int<integers>{}, Int<scale>{}) for a plan.
 template <int N>
 struct Int {
   static constexpr int value = N;
@@ -613,7 +706,12 @@ struct Int {
 template <typename F>
 int by_plan(const ForwardPlan& p, F f) {
   auto by_group = [&](auto nt) {
-    auto by_kind = [&](auto gb) { return p.ints ? f(nt, gb, Int<1>{}) : f(nt, gb, Int<0>{}); };
+    auto by_kind = [&](auto gb) {
+      auto by_scale = [&](auto ints) {
+        return p.scale == 2 ? f(nt, gb, ints, Int<2>{}) : p.scale == 4 ? f(nt, gb, ints, Int<4>{}) : f(nt, gb, ints, Int<0>{});
+      };
+      return p.ints ? by_scale(Int<1>{}) : by_scale(Int<0>{});
+    };
     return p.gb == 8 ? by_kind(Int<8>{}) : p.gb == 4 ? by_kind(Int<4>{}) : p.gb == 2 ? by_kind(Int<2>{}) : by_kind(Int<1>{});
   };
   return p.nt == 1 ? by_group(Int<1>{}) : p.nt == 2 ? by_group(Int<2>{}) : by_group(Int<4>{});
@@ -645,8 +743,9 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
     return fail(SPR_ERR_WORKSPACE, "int4 linear: workspace %zu < %zu bytes", workspace_bytes, need);
   float* partial = need ? (float*)workspace : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
-  return by_plan(p, [&](auto nt, auto gb, auto ints) {
-    return launch_forward<decltype(nt)::value, decltype(gb)::value, decltype(ints)::value != 0>(
+  return by_plan(p, [&](auto nt, auto gb, auto ints, auto scale) {
+    return launch_forward<decltype(nt)::value, decltype(gb)::value, decltype(ints)::value != 0,
+                          decltype(scale)::value>(
         p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
   });
 }
