@@ -555,28 +555,224 @@ int4_join_kernel(const float* partial, int slices, int64_t size, int64_t n, cons
   store_f32(y, dtype, i, bias ? v + load_as_f32(bias, dtype, i % n) : v);
 }
 
-// One warp per word column (eight k); a lane takes weight rows.
-__global__ void __launch_bounds__(256)
-int4_linear_grad_kernel(const void* dy, int64_t dy_stride, int dtype, int64_t rows, int64_t n, int64_t k, int group,
-                        const uint32_t* packed, const void* scales, int scale_dtype, const uint8_t* zeros, void* dx) {
-  const int64_t groups = (k + group - 1) / group, words = groups * group / 8;
-  const int64_t w = (int64_t)blockIdx.x * (256 / 32) + (threadIdx.x >> 5);
-  if (w >= words) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t g = w * 8 / group, r = blockIdx.y;
-  float acc[8] = {};
-  for (int64_t col = lane; col < n; col += 32) {
-    const uint32_t word = packed[col * words + w];
-    const float z = zeros ? (float)zeros[col * groups + g] : 8.f;
-    const float d = load_as_f32(dy, dtype, r * dy_stride + col) * load_as_f32(scales, scale_dtype, col * groups + g);
+// The gradient.  A warp takes 128 columns of the weight (a chunk) and walks down its
+// rows; the eight warps of a CTA take neighbouring chunks of the same rows, or rows
+// beside each other.  Products of 16 rows of parts (dy*scale of a row of dy, cut into
+// two or three bf16 parts: the first operand, formed once for 16 weight rows and a
+// group) by 16 weight rows by 8 columns: the codes are the second operand, pairs of
+// weight rows in a register.  A column of a product is a word of eight codes (or, for
+// groups of 32, one of four words and its even or odd codes), so that a product's
+// columns lie in one group.  Each walk's sums go to the workspace and are joined in a
+// fixed order.
+constexpr int kGradWarps = 8;
+constexpr int kGradRows = 32;    // weight rows of a stage
+constexpr int kGradBlocks = 4;   // blocks of 32 codes a row of a stage: 64 bytes
+constexpr int kGradStage = kGradRows * kGradBlocks * 16;
+constexpr int kGradBand = 256;   // weight rows whose scales and dy are in shared memory at a time
+
+// Two rows to 128 bytes; pieces turned so that rows 0, 2, 4, 6 (or 1, 3, 5, 7) and two
+// neighbouring pieces meet all banks.
+__device__ __forceinline__ int grad_piece(int row, int j) {
+  return (row >> 1) * 128 + ((((row & 1) << 2 | j) ^ ((row >> 1 & 3) << 1)) << 4);
+}
+
+struct GradShape {
+  int chunks, along;        // chunks of a row; warps of a CTA on neighbouring chunks
+  int walk;                 // weight rows of one walk, a multiple of kGradRows
+  int walks;                // of a chunk
+  int groups;               // of a CTA's chunks, at most
+  int pass, rows;           // rows of dy in a pass, and of all passes
+};
+
+template <int MT, int G, int PARTS>
+__global__ void __launch_bounds__(kGradWarps * 32, MT == 1 ? 2 : 1)
+int4_linear_grad_kernel(const Weights w, const GradShape sh, const void* dy, int64_t dy_stride, int dtype,
+                        float* partial) {
+  extern __shared__ __align__(128) char smem[];
+  constexpr int kTileRows = 16 / PARTS, kRowsMax = MT * kTileRows;  // rows of dy in a product, in all
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, beside = kGradWarps / sh.along;
+  const int row0 = blockIdx.z * sh.pass, rows = min(sh.pass, sh.rows - row0);
+  const int chunk0 = blockIdx.x * sh.along, chunk = chunk0 + warp % sh.along;
+  const int walk_id = blockIdx.y * beside + warp / sh.along;
+  // Bands of the CTA's walks, side by side: band row i*kGradBand/beside + ... is row i of a walk.
+  const int band = kGradBand / beside;
+  const int64_t n0 = (int64_t)walk_id * sh.walk, n1 = min(w.n, n0 + sh.walk);
+  const int steps = sh.walk / kGradRows;
+  char* ring = smem + warp * kStages * kGradStage;
+  float* scales = reinterpret_cast<float*>(smem + kGradWarps * kStages * kGradStage);
+  float* dys = scales + kGradBand * sh.groups;
+  uint8_t* zeros = reinterpret_cast<uint8_t*>(dys + kGradBand * kRowsMax);
+  const int group0 = chunk0 * kGradBlocks / w.group_blocks;
+  const int64_t pitch = (int64_t)w.blocks * 16;
+  const bool mine = chunk < sh.chunks;
+
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  uint32_t to[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(d, (float)((word >> (4 * j)) & 15) - z, acc[j]);
+  for (int i = 0; i < 4; ++i) to[i] = ring_at + grad_piece(8 * i + (lane >> 2), lane & 3);
+  const bool has_piece = mine && chunk * kGradBlocks + (lane & 3) < w.blocks;
+  const uint8_t* from = w.packed + (int64_t)chunk * (kGradBlocks * 16) + (lane & 3) * 16;
+  int fetched = 0;
+  auto fetch = [&](int stage) {
+    if (fetched < steps && has_piece)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t n = min(n0 + fetched * kGradRows + 8 * i + (lane >> 2), w.n - 1);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kGradStage), "l"(from + n * pitch)
+                     : "memory");
+      }
+    ++fetched;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+
+  const int t = lane & 3, c8 = lane >> 2;
+  constexpr int kTiles = kGradBlocks * 4;  // products' columns: 8 of the chunk's 128 each
+  float acc[MT][kTiles][4] = {};
+  int stage = 0;
+  for (int step = 0; step < steps; ++step) {
+    const int at = step * kGradRows % band;  // within the walk's share of the band
+    if (at == 0) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < kGradBand * sh.groups; i += kGradWarps * 32) {
+        const int row = i / sh.groups, g = group0 + i % sh.groups;
+        const int64_t walk0 = ((int64_t)blockIdx.y * beside + row / band) * sh.walk;
+        const int64_t n = walk0 + step * kGradRows + row % band;
+        const bool in = n < min(w.n, walk0 + sh.walk) && g < w.groups;
+        scales[i] = in ? load_as_f32(w.scales, w.scale_dtype, n * w.groups + g) : 0.f;
+        zeros[i] = in && w.zeros ? __ldg(w.zeros + n * w.groups + g) : 8;
+      }
+      for (int i = threadIdx.x; i < kGradBand * rows; i += kGradWarps * 32) {
+        const int row = i % kGradBand, r = i / kGradBand;
+        const int64_t walk0 = ((int64_t)blockIdx.y * beside + row / band) * sh.walk;
+        const int64_t n = walk0 + step * kGradRows + row % band;
+        dys[row * kRowsMax + r] =
+            n < min(w.n, walk0 + sh.walk) ? load_as_f32(dy, dtype, (int64_t)(row0 + r) * dy_stride + n) : 0.f;
+      }
+      __syncthreads();
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncwarp();
+    const char* codes_at = ring + stage * kGradStage;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int base = (warp / sh.along) * band + at + half * 16;  // band row of the first of 16 weight rows
+      float d[MT * 2][4];
+      bool low[MT * 2][2];
+#pragma unroll
+      for (int m = 0; m < MT * 2; ++m) {
+        const int rr = m % 2 * 8 + c8, r = m / 2 * kTileRows + rr / PARTS;
+        const bool in = rr < kTileRows * PARTS && r < rows;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[m][i] = in ? dys[(base + 2 * t + (i & 1) + (i >> 1) * 8) * kRowsMax + r] : 0.f;
+        low[m][0] = rr % PARTS == 1;
+        low[m][1] = rr % PARTS == 2;
+      }
+#pragma unroll
+      for (int gi = 0; gi < kGradBlocks / G; ++gi) {
+        const int block = chunk * kGradBlocks + gi * G;
+        if (block >= w.blocks || !mine) break;
+        const int g = (G < 4 && w.group_blocks == G ? block / G : block / w.group_blocks) - group0;
+        float s[4];
+        uint32_t z[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int q = (base + 2 * t + (i & 1) + (i >> 1) * 8) * sh.groups + g;
+          s[i] = scales[q];
+          z[i] = zeros[q];
+        }
+        const uint32_t z01 = 0x43004300u + (z[0] | z[1] << 16), z23 = 0x43004300u + (z[2] | z[3] << 16);
+        uint32_t a[MT * 2][2];
+#pragma unroll
+        for (int m = 0; m < MT * 2; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float f = d[m][2 * h + i] * s[2 * h + i];
+              const float hi = __uint_as_float(__float_as_uint(f) & 0xffff0000u);
+              float rest = f - hi;  // what is not finite is in the first part alone
+              if (rest != rest) rest = 0.f;
+              const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+              v[i] = __float_as_uint(low[m][0] ? (PARTS == 2 ? rest : mid) : f);
+              if (PARTS == 3 && low[m][1]) v[i] = __float_as_uint(rest - mid);
+            }
+            a[m][h] = bf16_pair(v[0], v[1]);
+          }
+        if constexpr (G == 1) {
+          const int b = gi, odd = c8 >> 2;
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = half * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+            v[i] = *reinterpret_cast<const uint32_t*>(codes_at + grad_piece(row, b) + (c8 & 3) * 4) >> (4 * odd);
+          }
+          const uint32_t l0 = __byte_perm(v[0], v[1], 0x5410), h0 = __byte_perm(v[0], v[1], 0x7632);
+          const uint32_t l1 = __byte_perm(v[2], v[3], 0x5410), h1 = __byte_perm(v[2], v[3], 0x7632);
+          const uint32_t b0[4] = {codes<0>(l0, z01), codes<2>(l0, z01), codes<0>(h0, z01), codes<2>(h0, z01)};
+          const uint32_t b1[4] = {codes<0>(l1, z23), codes<2>(l1, z23), codes<0>(h1, z23), codes<2>(h1, z23)};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              mma_bf16(acc[m][b * 4 + j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b0[j], b1[j]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < G / 2; ++u) {
+            const int b = gi * G / 2 + u;  // 64 columns
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = half * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+              v[i] = *reinterpret_cast<const uint32_t*>(codes_at + grad_piece(row, 2 * b + (c8 >> 2)) + (c8 & 3) * 4);
+            }
+            const uint32_t l0 = __byte_perm(v[0], v[1], 0x5410), h0 = __byte_perm(v[0], v[1], 0x7632);
+            const uint32_t l1 = __byte_perm(v[2], v[3], 0x5410), h1 = __byte_perm(v[2], v[3], 0x7632);
+            const uint32_t b0[8] = {codes<0>(l0, z01), codes<1>(l0, z01), codes<2>(l0, z01), codes<3>(l0, z01),
+                                    codes<0>(h0, z01), codes<1>(h0, z01), codes<2>(h0, z01), codes<3>(h0, z01)};
+            const uint32_t b1[8] = {codes<0>(l1, z23), codes<1>(l1, z23), codes<2>(l1, z23), codes<3>(l1, z23),
+                                    codes<0>(h1, z23), codes<1>(h1, z23), codes<2>(h1, z23), codes<3>(h1, z23)};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+                mma_bf16(acc[m][b * 8 + j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b0[j], b1[j]);
+          }
+        }
+      }
+    }
+    // The stage that this fetch fills was read in the round before.
+    fetch(stage == 0 ? kStages - 1 : stage - 1);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+  if (!mine || n0 >= n1) return;
+  // The warp's ring takes a product's sums in the order of the columns; a row's parts
+  // are added in their order.
+  float* out = reinterpret_cast<float*>(ring);  // [16][128]
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-    if (lane == 0 && w * 8 + j < k) store_f32(dx, dtype, r * k + w * 8 + j, acc[j]);
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = 2 * t + (i & 1);
+        const int k = G == 1 ? j / 4 * 32 + (col & 3) * 8 + j % 4 * 2 + (col >> 2) : j / 8 * 64 + col * 8 + j % 8;
+        out[(c8 + (i >> 1) * 8) * 128 + k] = acc[m][j][i];
+      }
+    __syncwarp();
+    for (int r = m * kTileRows; r < min(rows, (m + 1) * kTileRows); ++r)
+      for (int i = lane; i < 128; i += 32) {
+        const int k = chunk * 128 + i;
+        float v = 0.f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) v += out[((r - m * kTileRows) * PARTS + p) * 128 + i];
+        if (k < w.k) partial[((int64_t)walk_id * sh.rows + row0 + r) * w.k + k] = v;
+      }
+    __syncwarp();
   }
 }
 
@@ -717,6 +913,48 @@ int by_plan(const ForwardPlan& p, F f) {
   return p.nt == 1 ? by_group(Int<1>{}) : p.nt == 2 ? by_group(Int<2>{}) : by_group(Int<4>{});
 }
 
+struct GradPlan {
+  GradShape sh;
+  int mt, g, parts, walks, passes, smem;
+  dim3 grid;
+};
+
+// Two parts hold the product of two bf16 numbers exactly, three what fp32 holds.  Walks:
+// as many as fill the GPU, of at least 128 weight rows.
+GradPlan plan_grad(int64_t rows, const Weights& w, int dtype) {
+  GradPlan p{};
+  p.parts = dtype == SPR_BF16 && w.scale_dtype == SPR_BF16 ? 2 : 3;
+  const int tile_rows = 16 / p.parts;
+  p.mt = rows > tile_rows ? 2 : 1;
+  p.g = w.group_blocks % 4 == 0 ? 4 : w.group_blocks % 2 == 0 ? 2 : 1;
+  p.sh.rows = (int)rows;
+  p.sh.pass = (int)std::min<int64_t>(rows, p.mt * tile_rows);
+  p.passes = (int)((rows + p.sh.pass - 1) / p.sh.pass);
+  p.sh.chunks = (w.blocks + kGradBlocks - 1) / kGradBlocks;
+  p.sh.along = 1;
+  while (p.sh.along < kGradWarps && p.sh.along < p.sh.chunks) p.sh.along *= 2;
+  const int beside = kGradWarps / p.sh.along, across = (p.sh.chunks + p.sh.along - 1) / p.sh.along;
+  const int64_t ctas = (int64_t)sm_count() * (p.mt == 1 ? 2 : 1);
+  int64_t walks = std::max<int64_t>(1, ctas / (across * p.passes)) * beside;
+  walks = std::max<int64_t>(1, std::min(walks, w.n / 128));
+  p.sh.walk = (int)((w.n + walks - 1) / walks + kGradRows - 1) / kGradRows * kGradRows;
+  p.walks = (int)((w.n + p.sh.walk - 1) / p.sh.walk);
+  p.sh.groups = (p.sh.along * kGradBlocks - 1) / w.group_blocks + 2;
+  p.smem = kGradWarps * kStages * kGradStage + kGradBand * (p.sh.groups * 5 + p.mt * tile_rows * 4);
+  p.grid = dim3(across, (p.walks + beside - 1) / beside, p.passes);
+  return p;
+}
+
+template <int MT, int G, int PARTS>
+int launch_grad(const GradPlan& p, const Weights& w, const void* dy, int64_t dy_stride, int dtype, float* partial,
+                cudaStream_t st) {
+  auto kern = int4_linear_grad_kernel<MT, G, PARTS>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    return check_launch("int4 linear grad");
+  kern<<<p.grid, kGradWarps * 32, p.smem, st>>>(w, p.sh, dy, dy_stride, dtype, partial);
+  return check_launch("int4 linear grad");
+}
+
 }  // namespace
 
 }  // namespace spr
@@ -750,21 +988,44 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
   });
 }
 
-extern "C" size_t spr_int4_linear_grad_workspace_bytes(int64_t, int64_t, int64_t, int, int) { return 0; }
+extern "C" size_t spr_int4_linear_grad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype) {
+  if (rows <= 0 || n <= 0 || k <= 0 || group < 32) return 0;
+  size_t most = 0;
+  for (int scale_dtype : {SPR_F32, SPR_BF16}) {
+    const GradPlan p = plan_grad(rows, make_weights(nullptr, nullptr, scale_dtype, nullptr, n, k, group), dtype);
+    most = std::max(most, (size_t)p.walks * rows * k * sizeof(float));
+  }
+  return most;
+}
 
 extern "C" int spr_int4_linear_grad(const void* dy, int64_t dy_stride, int dtype, int64_t rows, int64_t n, int64_t k,
                                     int group, const uint8_t* packed, const void* scales, int scale_dtype,
                                     const uint8_t* zeros, void* dx, void* workspace, size_t workspace_bytes,
                                     void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (int rc = check_int4("int4 linear grad", dy_stride, dtype, rows, n, k, n, group, packed, scale_dtype)) return rc;
   if (rows == 0) return SPR_OK;
   if (!dx || (n && (!dy || !packed || !scales))) return fail(SPR_ERR_ARG, "int4 linear grad: null operand");
-  const int64_t words = (k + group - 1) / group * group / 8;
-  const dim3 grid((unsigned)((words + 256 / 32 - 1) / (256 / 32)), (unsigned)rows);
-  int4_linear_grad_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(dy, dy_stride, dtype, rows, n, k, group,
-                                                                       (const uint32_t*)packed, scales, scale_dtype,
-                                                                       zeros, dx);
+  const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
+  cudaStream_t st = (cudaStream_t)stream;
+  int walks = 0;
+  if (n) {
+    const GradPlan p = plan_grad(rows, w, dtype);
+    const size_t need = spr_int4_linear_grad_workspace_bytes(rows, n, k, group, dtype);
+    if (!workspace || workspace_bytes < need)
+      return fail(SPR_ERR_WORKSPACE, "int4 linear grad: workspace %zu < %zu bytes", workspace_bytes, need);
+    auto by_group = [&](auto mt, auto parts) {
+      constexpr int MT = decltype(mt)::value, PARTS = decltype(parts)::value;
+      float* out = (float*)workspace;
+      return p.g == 4   ? launch_grad<MT, 4, PARTS>(p, w, dy, dy_stride, dtype, out, st)
+             : p.g == 2 ? launch_grad<MT, 2, PARTS>(p, w, dy, dy_stride, dtype, out, st)
+                        : launch_grad<MT, 1, PARTS>(p, w, dy, dy_stride, dtype, out, st);
+    };
+    auto by_rows = [&](auto parts) { return p.mt == 1 ? by_group(Int<1>{}, parts) : by_group(Int<2>{}, parts); };
+    if (int rc = p.parts == 2 ? by_rows(Int<2>{}) : by_rows(Int<3>{})) return rc;
+    walks = p.walks;
+  }
+  const int64_t size = rows * k;
+  int4_join_kernel<<<(unsigned)((size + 255) / 256), 256, 0, st>>>((const float*)workspace, walks, size, k, nullptr, dx,
+                                                                   dtype);
   return check_launch("int4 linear grad");
 }
