@@ -105,6 +105,8 @@ _lib = None
 def load(path: str | None = None):
     """Load the shared library once and bind every prototype."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -16,8 +16,9 @@ normalised, so the norm reads what the residual stream holds.  Statistics and
 sums are fp32, and the gradients of shared vectors are summed in a fixed order.
 
 The gradients are of first order.  A call captured into a CUDA graph needs what
-any captured autograd call needs; :func:`sparsepr_b200.kernels.adaln_forward` and
-``adaln_backward`` are the same passes without autograd.
+any captured autograd call needs; :func:`operands` with
+:func:`sparsepr_b200.kernels.adaln_forward` and ``adaln_backward`` are the same passes
+without autograd.
 """
 
 from __future__ import annotations
@@ -60,113 +61,123 @@ def _split(shape, mod_shape, name):
     return runs[0][0], runs[1][0], runs[0][1], runs[1][1]
 
 
-def _rows(t, b, n, name):
-    """[b, n, C] view of a [..., C] tensor."""
+def _strides(t, b, n, name):
+    """Element strides of the [b, n, C] rows that a [..., C] tensor holds (0 for an extent of 1)."""
+    if t.is_contiguous():
+        c = t.shape[-1]
+        return (n * c if b > 1 else 0), (c if n > 1 else 0)
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise RuntimeError(f"{name}: channels must be contiguous, got strides {t.stride()}")
     try:
-        return t.view(b, n, t.shape[-1])
+        v = t.view(b, n, t.shape[-1])
     except RuntimeError:
         raise RuntimeError(f"{name}: axes of strides {t.stride()} cannot be viewed as [{b}, {n}, {t.shape[-1]}]; "
                            "make it contiguous") from None
+    return (v.stride(0) if b > 1 else 0), (v.stride(1) if n > 1 else 0)
 
 
-def _prepare(x, y, gate, shift, scale):
-    """Checked [B,N,C] views of all operands and the kept extents of the vectors."""
-    for name, t in (("x", x), ("y", y), ("gate", gate), ("shift", shift), ("scale", scale)):
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{name} is on {t.device}, x on {x.device}")
+_NONE = (0, 0)
+
+
+def operands(x, y, gate, shift, scale, scale_offset: float = 1.0):
+    """``(AdalnOperands, (batch or 1, tokens or 1) of the vectors)`` of checked tensors."""
     if not x.is_cuda:
         raise RuntimeError(f"sparsepr_b200 kernels need CUDA tensors, got a {x.device} tensor")
-    if x.dtype not in K._DT or x.dim() < 1:
-        raise RuntimeError(f"x must be [..., C] fp32/bf16/fp16, got {tuple(x.shape)} {x.dtype}")
-    c = x.shape[-1]
+    dt, shape = x.dtype, x.shape
+    if dt not in K._DT or not shape:
+        raise RuntimeError(f"x must be [..., C] fp32/bf16/fp16, got {tuple(shape)} {dt}")
+    c = shape[-1]
     if not 1 <= c <= 16384:
         raise RuntimeError(f"layer norm over {c} channels: 1 to 16384 are supported")
-    if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
-        raise RuntimeError(f"y must be {tuple(x.shape)} {x.dtype} as x is, got {tuple(y.shape)} {y.dtype}")
-    mods = [(n, t) for n, t in (("gate", gate), ("shift", shift), ("scale", scale)) if t is not None]
-    if mods:
-        name, first = mods[0]
-        if first.dtype not in (x.dtype, torch.float32):
-            raise RuntimeError(f"{name} must be {x.dtype} or fp32, got {first.dtype}")
-        for other, t in mods[1:]:
-            if t.shape != first.shape or t.dtype != first.dtype:
-                raise RuntimeError(f"{other} {tuple(t.shape)} {t.dtype} must be as {name}: {tuple(first.shape)} "
-                                   f"{first.dtype}")
-        b, n, keep_b, keep_n = _split(x.shape, first.shape, name)
-    else:
+    index = x.get_device()
+    if y is not None and (y.shape != shape or y.dtype != dt or y.get_device() != index):
+        raise RuntimeError(f"y must be {tuple(shape)} {dt} on {x.device} as x is, got {tuple(y.shape)} {y.dtype} on "
+                           f"{y.device}")
+    first = None
+    for name, t in (("gate", gate), ("shift", shift), ("scale", scale)):
+        if t is None:
+            continue
+        if t.get_device() != index:
+            raise RuntimeError(f"{name} is on {t.device}, x on {x.device}")
+        if first is None:
+            first, first_name = t, name
+            if t.dtype != dt and t.dtype != torch.float32:
+                raise RuntimeError(f"{name} must be {dt} or fp32, got {t.dtype}")
+        elif t.shape != first.shape or t.dtype != first.dtype:
+            raise RuntimeError(f"{name} {tuple(t.shape)} {t.dtype} must be as {first_name}: {tuple(first.shape)} "
+                               f"{first.dtype}")
+    if first is None or first.shape == (c,):
         b, n, keep_b, keep_n = 1, x.numel() // c, False, False
-    if b == 1 and not keep_n and x.dim() > 2 and not all(t is None or t.is_contiguous() for t in (x, y)):
-        # One vector for all rows: any two runs of x's axes will do.
-        b, n = math.prod(x.shape[:-2]), x.shape[-2]
-    xv = _rows(x, b, n, "x")
-    yv = None if y is None else _rows(y, b, n, "y")
+    else:
+        b, n, keep_b, keep_n = _split(shape, first.shape, first_name)
+    if b == 1 and not keep_n and not (x.is_contiguous() and (y is None or y.is_contiguous())) and len(shape) > 2:
+        b, n = math.prod(shape[:-2]), shape[-2]  # one vector for all rows: any two runs of x's axes will do
     mb, mn = (b if keep_b else 1), (n if keep_n else 1)
-    return xv, yv, *(None if t is None else _rows(t, mb, mn, k) for k, t in
-                     (("gate", gate), ("shift", shift), ("scale", scale))), (mb, mn)
-
-
-def _grad_rows(t, b, n):
-    """[b, n, C] view of an incoming gradient of any strides."""
-    if t is None:
-        return None
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t.view(b, n, t.shape[-1])
+    op = K.AdalnOperands(x, y, gate, shift, scale, b, n, c, _strides(x, b, n, "x"),
+                         _NONE if y is None else _strides(y, b, n, "y"),
+                         _NONE if shift is None else _strides(shift, mb, mn, "shift"),
+                         _NONE if scale is None else _strides(scale, mb, mn, "scale"),
+                         _NONE if gate is None else _strides(gate, mb, mn, "gate"),
+                         dt if first is None else first.dtype, scale_offset)
+    return op, (mb, mn)
 
 
 class _AdaLN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, shift, scale, eps, scale_offset):
-        xv, yv, gv, shv, scv, mod_shape = _prepare(x, y, gate, shift, scale)
-        z, h, mean, rstd = K.adaln_forward(xv, yv, gv, shv, scv, eps, scale_offset, True)
-        h = h.view(x.shape)
-        if z is not None:
-            z = z.view(x.shape)
-        ctx.save_for_backward(x if z is None else z, y, gate, scale, mean, rstd)
+        op, mod_shape = operands(x, y, gate, shift, scale, scale_offset)
+        z, h, stats = K.adaln_forward(op, eps, True)
+        ctx.save_for_backward(x if z is None else z, y, gate, scale, stats)
         ctx.set_materialize_grads(False)
-        ctx.layout = (xv.shape[0], xv.shape[1], mod_shape, scale_offset)
-        ctx.mod = next(((t.shape, t.dtype) for t in (gate, shift, scale) if t is not None), (None, None))
-        return (h,) if z is None else (z, h)
+        # What the backward pass needs of the operands apart from the tensors; z is dense.
+        dense = (op.tokens * op.channels if op.batch > 1 else 0, op.channels if op.tokens > 1 else 0)
+        ctx.op = op._replace(x=None, y=None, gate=None, shift=None, scale=None,
+                             x_strides=op.x_strides if z is None else dense)
+        ctx.mod_shape = mod_shape
+        ctx.vector = next((t.shape for t in (gate, shift, scale) if t is not None), None)
+        return h if z is None else (z, h)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        x, y, gate, scale, mean, rstd = ctx.saved_tensors
-        b, n, mod_shape, offset = ctx.layout
+        x, y, gate, scale, stats = ctx.saved_tensors
         dz, dh = grads if y is not None else (None, grads[0])
-        if dh is None and dz is None:
-            return (None,) * 7
-        dh = torch.zeros_like(x, memory_format=torch.contiguous_format) if dh is None else dh
-        mshape, mdtype = ctx.mod
-        view = lambda t, nb, nn: None if t is None else t.view(nb, nn, t.shape[-1])  # noqa: E731
-        dx, dy, dgate, dshift, dscale = K.adaln_backward(
-            view(x, b, n), view(y, b, n), view(gate, *mod_shape), view(scale, *mod_shape), mean, rstd,
-            _grad_rows(dh, b, n), _grad_rows(dz, b, n), offset, ctx.needs_input_grad[2:5], mod_shape, mdtype)
-        shaped = lambda t, s: None if t is None else t.view(s)  # noqa: E731
-        return (dx.view(x.shape), shaped(dy, x.shape), shaped(dgate, mshape), shaped(dshift, mshape),
-                shaped(dscale, mshape), None, None)
+        if dh is None:
+            if dz is None:
+                return (None,) * 7
+            dh = torch.zeros_like(dz, memory_format=torch.contiguous_format)
+        elif not dh.is_contiguous():
+            dh = dh.contiguous()
+        if dz is not None and not dz.is_contiguous():
+            dz = dz.contiguous()
+        op = ctx.op._replace(x=x, y=y, gate=gate, scale=scale)
+        dx, dy, dgate, dshift, dscale = K.adaln_backward(op, stats, dh, dz, ctx.needs_input_grad[2:5], ctx.mod_shape)
+        v = ctx.vector
+        return (dx, dy, None if dgate is None else dgate.view(v), None if dshift is None else dshift.view(v),
+                None if dscale is None else dscale.view(v), None, None)
 
 
-def _apply(x, y, gate, shift, scale, eps, scale_offset):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, gate, shift, scale)):
-        return _AdaLN.apply(x, y, gate, shift, scale, float(eps), scale_offset)
-    xv, yv, gv, shv, scv, _ = _prepare(x, y, gate, shift, scale)
-    z, h, _, _ = K.adaln_forward(xv, yv, gv, shv, scv, float(eps), scale_offset, False)
-    return (h.view(x.shape),) if z is None else (z.view(x.shape), h.view(x.shape))
+def _wants_grad(x, y, gate, shift, scale):
+    return torch.is_grad_enabled() and (x.requires_grad or (y is not None and y.requires_grad)
+                                        or (gate is not None and gate.requires_grad)
+                                        or (shift is not None and shift.requires_grad)
+                                        or (scale is not None and scale.requires_grad))
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-6) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis."""
-    return _apply(x, None, None, bias, weight, eps, 0.0)[0]
+    if _wants_grad(x, None, None, bias, weight):
+        return _AdaLN.apply(x, None, None, bias, weight, float(eps), 0.0)
+    return K.adaln_forward(operands(x, None, None, bias, weight, 0.0)[0], eps, False)[1]
 
 
 def modulated_layer_norm(x: torch.Tensor, shift: torch.Tensor | None, scale: torch.Tensor | None,
                          eps: float = 1e-6) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * (1 + scale) + shift`` over the last axis."""
-    return _apply(x, None, None, shift, scale, eps, 1.0)[0]
+    if _wants_grad(x, None, None, shift, scale):
+        return _AdaLN.apply(x, None, None, shift, scale, float(eps), 1.0)
+    return K.adaln_forward(operands(x, None, None, shift, scale)[0], eps, False)[1]
 
 
 def gated_residual_layer_norm(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None,
@@ -174,4 +185,6 @@ def gated_residual_layer_norm(x: torch.Tensor, y: torch.Tensor, gate: torch.Tens
                               eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """``(z, modulated_layer_norm(z, shift, scale))`` with ``z = x + gate * y`` (``gate`` None:
     ``x + y``), ``y`` of x's shape and type."""
-    return _apply(x, y, gate, shift, scale, eps, 1.0)
+    if _wants_grad(x, y, gate, shift, scale):
+        return _AdaLN.apply(x, y, gate, shift, scale, float(eps), 1.0)
+    return K.adaln_forward(operands(x, y, gate, shift, scale)[0], eps, False)[:2]

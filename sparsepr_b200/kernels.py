@@ -8,8 +8,8 @@ stream.  There is no CPU path: non-CUDA inputs raise ``RuntimeError``.
 from __future__ import annotations
 
 import contextlib
-
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -327,8 +327,6 @@ def block_sparse_attention(q_perm, k_perm, v_perm, q_offsets, k_offsets, sel_ids
     rs = None
     keep = ()
     if repair is not None:
-        import ctypes
-
         state, alpha, rows, dense = repair
         xm, xs, ym, left, basis = (t.to(torch.float32).contiguous() for t in state)
         if left.shape[-1] != 16 or left.shape[0] != b:
@@ -566,102 +564,119 @@ def ridge_cholesky(a: torch.Tensor, scale: torch.Tensor, relative_ridge: float, 
     return l, failed.bool()
 
 
-def _launch(dev: torch.device, name: str, *args) -> None:
-    """``_lib.call`` on ``dev``'s current stream, also where another device is current."""
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args, _stream(dev))
+def _launch(index: int, name: str, *args) -> None:
+    """``_lib.call`` on the current stream of device ``index``, also where another device is current."""
+    if torch.cuda.current_device() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, _stream(dev))
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _bt(t: torch.Tensor | None) -> tuple[int, int]:
-    """Element strides of the batch and token axes of a [B or 1, N or 1, C] view (0: broadcast)."""
-    if t is None:
-        return 0, 0
-    (b, n, _c), (sb, st, _sc) = t.shape, t.stride()
-    return (sb if b > 1 else 0), (st if n > 1 else 0)
+class AdalnOperands(NamedTuple):
+    """Operands of the adaLN passes as the kernels read them: tensors, the rows as [batch][tokens][channels]
+    with (batch, token) element strides, and the vectors' strides (0: broadcast along that axis)."""
+
+    x: torch.Tensor
+    y: torch.Tensor | None
+    gate: torch.Tensor | None
+    shift: torch.Tensor | None
+    scale: torch.Tensor | None
+    batch: int
+    tokens: int
+    channels: int
+    x_strides: tuple[int, int]
+    y_strides: tuple[int, int]
+    shift_strides: tuple[int, int]
+    scale_strides: tuple[int, int]
+    gate_strides: tuple[int, int]
+    mod_dtype: torch.dtype
+    scale_offset: float
+
+    def struct(self, eps: float, z, h, mean, rstd) -> _lib.SprAdaln:
+        return _lib.SprAdaln(_DT[self.x.dtype], _DT[self.mod_dtype], self.batch, self.tokens, self.channels, eps,
+                             self.scale_offset, self.x.data_ptr(), _p(self.y), _p(self.shift), _p(self.scale),
+                             _p(self.gate), *self.x_strides, *self.y_strides, *self.shift_strides,
+                             *self.scale_strides, *self.gate_strides, z, h, mean, rstd)
 
 
-def _adaln_op(x, y, gate, shift, scale, eps, scale_offset, z, h, mean, rstd) -> _lib.SprAdaln:
-    mod = next((m for m in (shift, scale, gate) if m is not None), None)
-    b, n, c = x.shape
-    return _lib.SprAdaln(_DT[x.dtype], _DT[x.dtype if mod is None else mod.dtype], b, n, c, eps, scale_offset, _p(x),
-                         _p(y), _p(shift), _p(scale), _p(gate), *_bt(x), *_bt(y), *_bt(shift), *_bt(scale),
-                         *_bt(gate), _p(z), _p(h), _p(mean), _p(rstd))
+def adaln_forward(op: AdalnOperands, eps: float, stats: bool):
+    """Modulated layer norm of [batch][tokens][channels] rows with an optional gated residual
+    (``op.y``): ``z = x + gate*y``, ``h = LN(z)*(scale_offset + scale) + shift``.
 
-
-def adaln_forward(x, y, gate, shift, scale, eps: float, scale_offset: float, stats: bool):
-    """Modulated layer norm of [B,N,C] rows with an optional gated residual (``y``):
-    ``z = x + gate*y``, ``h = LN(z)*(scale_offset + scale) + shift``.
-
-    ``shift``, ``scale`` and ``gate`` are [B or 1, N or 1, C] views of one type (the
-    rows' or fp32) or None.  Returns ``(z, h, mean, rstd)``, ``z`` None without ``y``
-    and the row statistics fp32 [B*N] or None without ``stats``.  The shapes are
-    checked by :mod:`sparsepr_b200.adaln`."""
-    dev = _cuda(x, y, gate, shift, scale)
-    b, n, c = x.shape
-    h = torch.empty((b, n, c), dtype=x.dtype, device=dev)
-    z = None if y is None else torch.empty_like(h)
-    mean = rstd = None
+    :func:`sparsepr_b200.adaln.operands` makes ``op`` from checked tensors.  Returns
+    ``(z, h, stats)``: ``z`` and ``h`` dense in x's shape, ``z`` None without ``y``, and the row means and
+    reciprocal deviations fp32 [2, batch*tokens], None unless asked for."""
+    x = op.x
+    h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    z = None if op.y is None else torch.empty_like(h)
+    st = mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2, b * n), dtype=torch.float32, device=dev).unbind(0)
-    op = _adaln_op(x, y, gate, shift, scale, eps, scale_offset, z, h, mean, rstd)
+        rows = op.batch * op.tokens
+        st = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean = st.data_ptr()
+        rstd = mean + 4 * rows
+    s = op.struct(eps, _p(z), h.data_ptr(), mean, rstd)
     _count(1)
-    _launch(dev, "spr_adaln_forward", ctypes.addressof(op))
-    return z, h, mean, rstd
+    _launch(x.get_device(), "spr_adaln_forward", ctypes.addressof(s))
+    return z, h, st
 
 
-def adaln_backward(x, y, gate, scale, mean, rstd, dh, dz, scale_offset: float, needs=(True, True, True),
-                   mod_shape=(1, 1), mod_dtype: torch.dtype | None = None):
-    """Backward pass of :func:`adaln_forward` from its ``z`` (``x`` without a branch) and
-    row statistics: ``(dx, dy, dgate, dshift, dscale)``.
+def adaln_backward(op: AdalnOperands, stats: torch.Tensor, dh, dz=None, needs=(True, True, True),
+                   mod_shape=(1, 1)):
+    """Backward pass of :func:`adaln_forward`: ``(dx, dy, dgate, dshift, dscale)``.
 
-    ``needs`` says which of (dgate, dshift, dscale) are formed; they are
-    ``mod_shape + (C,)`` with ``mod_shape`` (B or 1, N or 1) and summed over the
-    axes of extent 1, in a fixed order.  The workspace belongs to this call alone,
-    so that calls on several streams and captured graphs share none."""
-    dev = _cuda(x, y, gate, scale, mean, rstd, dh, dz)
-    b, n, c = x.shape
-    mdt = x.dtype if mod_dtype is None else mod_dtype
-    dx = torch.empty((b, n, c), dtype=x.dtype, device=dev)
-    dy = None if y is None else torch.empty_like(dx)
-    keep = (int(mod_shape[0] > 1), int(mod_shape[1] > 1))
-    dgate, dshift, dscale = (torch.empty((*mod_shape, c), dtype=mdt, device=dev) if need else None for need in needs)
-    if b * n == 0:
+    ``op.x`` is the forward pass's ``z`` (its ``x`` without a branch); ``dh`` and ``dz`` (None:
+    no gradient) are dense in its shape.  ``needs`` says which of (dgate, dshift, dscale) are
+    formed: [*mod_shape, channels] with ``mod_shape`` (batch or 1, tokens or 1), summed over the
+    axes of extent 1 in a fixed order.  The workspace belongs to this call alone, so
+    that calls on several streams and captured graphs share none."""
+    x = op.x
+    b, n, c = op.batch, op.tokens, op.channels
+    dx = torch.empty_like(dh)
+    dy = None if op.y is None else torch.empty_like(dh)
+    dgate, dshift, dscale = (x.new_empty((*mod_shape, c), dtype=op.mod_dtype) if need else None for need in needs)
+    rows = b * n
+    if rows == 0:
         for t in (dgate, dshift, dscale):
             if t is not None:
                 t.zero_()
         return dx, dy, dgate, dshift, dscale
-    op = _adaln_op(x, y, gate, None, scale, 0.0, scale_offset, None, None, mean, rstd)
-    op.mod_dtype = _DT[mdt]
-    gr = _lib.SprAdalnGrad(_p(dh), _p(dz), *_bt(dh), *_bt(dz), _p(dx), _p(dy), _p(dshift), _p(dscale), _p(dgate),
-                           *keep)
-    nbytes = _lib.query("spr_adaln_backward_workspace_bytes", b, n, c, *keep)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _count(2)
-    _launch(dev, "spr_adaln_backward", ctypes.addressof(op), ctypes.addressof(gr), _p(ws), nbytes)
+    mean = stats.data_ptr()
+    s = op.struct(0.0, None, None, mean, mean + 4 * rows)
+    keep_b, keep_n = int(mod_shape[0] > 1), int(mod_shape[1] > 1)
+    gr = _lib.SprAdalnGrad(dh.data_ptr(), _p(dz), n * c, c, n * c, c, dx.data_ptr(), _p(dy), _p(dshift), _p(dscale),
+                           _p(dgate), keep_b, keep_n)
+    index = x.get_device()
+    nbytes = _lib.query("spr_adaln_backward_workspace_bytes", b, n, c, keep_b, keep_n)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _count(2 if nbytes else 1)
+    _launch(index, "spr_adaln_backward", ctypes.addressof(s), ctypes.addressof(gr), _p(ws), nbytes)
     return dx, dy, dgate, dshift, dscale
 
 
 def _int4_checks(what, rows2d, length, packed, scales, zeros):
-    """(n, k rounded up to whole groups, group) of the weights; raises on what the kernels do not take."""
+    """(n, group) of the weights; raises on what the kernels do not take."""
     if rows2d.dtype not in _DT or scales.dtype not in _DT:
         raise RuntimeError(f"{what}: rows and scales must be fp32/bf16/fp16, got {rows2d.dtype} and {scales.dtype}")
-    if packed.dtype != torch.uint8 or packed.dim() != 2 or scales.dim() != 2 or scales.shape[0] != packed.shape[0]:
+    pshape, sshape = packed.shape, scales.shape
+    if packed.dtype != torch.uint8 or len(pshape) != 2 or len(sshape) != 2 or sshape[0] != pshape[0]:
         raise RuntimeError(f"{what}: packed codes must be uint8 [N, K/2] and scales [N, groups], got {packed.dtype} "
-                           f"{tuple(packed.shape)} and {tuple(scales.shape)}")
-    n, kp, groups = packed.shape[0], 2 * packed.shape[1], scales.shape[1]
+                           f"{tuple(pshape)} and {tuple(sshape)}")
+    n, kp, groups = pshape[0], 2 * pshape[1], sshape[1]
     if groups == 0 or kp % (32 * groups):
         raise RuntimeError(f"{what}: {kp} codes a row in {groups} groups; a group must be a multiple of 32 codes")
     group = kp // groups
     if not kp - group < length <= kp:
         raise RuntimeError(f"{what}: {length} input features do not end in the last of {groups} groups of {group}")
-    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
-        raise RuntimeError(f"{what}: zeros must be uint8 {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
-    for name, t in (("packed", packed), ("scales", scales), ("zeros", zeros)):
-        if t is not None:
-            _contig(f"{what}: {name}", t)
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != sshape):
+        raise RuntimeError(f"{what}: zeros must be uint8 {tuple(sshape)}, got {zeros.dtype} {tuple(zeros.shape)}")
+    if not (packed.is_contiguous() and scales.is_contiguous() and (zeros is None or zeros.is_contiguous())):
+        raise RuntimeError(f"{what}: packed codes, scales and zeros must be contiguous")
+    index = rows2d.get_device()
+    if packed.get_device() != index or scales.get_device() != index or (zeros is not None and
+                                                                        zeros.get_device() != index):
+        raise RuntimeError(f"{what}: the weight is on {packed.device}, the rows on {rows2d.device}")
     if rows2d.shape[1] > 1 and rows2d.stride(1) != 1:
         raise RuntimeError(f"{what}: the last dimension must be contiguous, got strides {rows2d.stride()}")
     return n, group
@@ -674,31 +689,31 @@ def int4_linear(x, packed, scales, zeros=None, bias=None) -> torch.Tensor:
     ``packed`` uint8 [N, groups*group/2]: two 4-bit codes a byte, the even column in
     the low half; ``scales`` [N, groups]; ``zeros`` uint8 [N, groups] (None: 8).  The
     group size is a multiple of 32; codes of columns >= K are ignored."""
-    dev = _cuda(x, packed, scales, zeros, bias)
+    _cuda(x, packed, scales, zeros, bias)
     r, k = x.shape
     n, group = _int4_checks("int4_linear", x, k, packed, scales, zeros)
     if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or (n > 1 and bias.stride(0) != 1)):
         raise RuntimeError(f"int4_linear: bias must be contiguous {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
-    y = torch.empty((r, n), dtype=x.dtype, device=dev)
+    y = x.new_empty((r, n))
     nbytes = _lib.query("spr_int4_linear_workspace_bytes", r, n, k, group, _DT[x.dtype])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _count(1)
-    _launch(dev, "spr_int4_linear", _p(x), x.stride(0), _DT[x.dtype], r, n, k, group, _p(packed), _p(scales),
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _count(2 if nbytes else 1)
+    _launch(x.get_device(), "spr_int4_linear", _p(x), x.stride(0), _DT[x.dtype], r, n, k, group, _p(packed), _p(scales),
             _DT[scales.dtype], _p(zeros), _p(bias), _p(y), _p(ws), nbytes)
     return y
 
 
 def int4_linear_grad(dy, packed, scales, zeros, in_features: int) -> torch.Tensor:
     """Gradient of :func:`int4_linear` with respect to its rows: ``dy`` [R,N] -> [R, in_features]."""
-    dev = _cuda(dy, packed, scales, zeros)
+    _cuda(dy, packed, scales, zeros)
     n, group = _int4_checks("int4_linear_grad", dy, in_features, packed, scales, zeros)
     r = dy.shape[0]
     if dy.shape[1] != n:
         raise RuntimeError(f"int4_linear_grad: dy {tuple(dy.shape)} does not match {n} weight rows")
-    dx = torch.empty((r, in_features), dtype=dy.dtype, device=dev)
+    dx = dy.new_empty((r, in_features))
     nbytes = _lib.query("spr_int4_linear_grad_workspace_bytes", r, n, in_features, group, _DT[dy.dtype])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _count(1)
-    _launch(dev, "spr_int4_linear_grad", _p(dy), dy.stride(0), _DT[dy.dtype], r, n, in_features, group, _p(packed),
+    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _count(2)
+    _launch(dy.get_device(), "spr_int4_linear_grad", _p(dy), dy.stride(0), _DT[dy.dtype], r, n, in_features, group, _p(packed),
             _p(scales), _DT[scales.dtype], _p(zeros), _p(dx), _p(ws), nbytes)
     return dx

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import sparsepr_b200 as spr
-from sparsepr_b200.adaln import _split
+from sparsepr_b200.adaln import _split, operands
 
 EPS32 = 2.0 ** -24
 K_STEPS = 32
@@ -70,7 +70,7 @@ def test_c_entries_refuse_before_any_launch():
         _lib.call("spr_adaln_forward", None, None)
     fwd(op(tokens=0))  # nothing to do, nothing launched
     gr = _lib.SprAdalnGrad(dh=256, dx=256, dshift=256)
-    o = op(mean=256, rstd=256)
+    o = op(tokens=4096, mean=256, rstd=256)
     with pytest.raises(RuntimeError, match="SPR_ERR_WORKSPACE"):
         _lib.call("spr_adaln_backward", ctypes.addressof(o), ctypes.addressof(gr), None, 0, None)
     with pytest.raises(RuntimeError, match="SPR_ERR_ARG"):
@@ -387,18 +387,17 @@ def test_two_captured_graphs_replayed_together(cuda):
     runs = []
     for seed in (1, 2):
         v = _inputs(cuda, 1, 3000, 1280, BF, FP, "vector", seed=seed)
-        vec = {k: v[k].view(1, 1, -1) for k in ("gate", "shift", "scale")}
+        op, vectors = operands(v["x"], v["y"], v["gate"], v["shift"], v["scale"])
 
-        def step(v=v, vec=vec):
-            z, h, mean, rstd = K.adaln_forward(v["x"], v["y"], vec["gate"], vec["shift"], vec["scale"], 1e-6, 1.0, True)
-            return (z, h, *K.adaln_backward(z, v["y"], vec["gate"], vec["scale"], mean, rstd, v["dh"], v["dz"], 1.0,
-                                            mod_dtype=FP))
+        def step(op=op, v=v):
+            z, h, stats = K.adaln_forward(op, 1e-6, True)
+            return (z, h, *K.adaln_backward(op._replace(x=z), stats, v["dh"], v["dz"], mod_shape=vectors))
         want = [t.clone() for t in step()]
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             got = step()
-        runs.append((g, got, want, torch.cuda.Stream(), (v, vec)))  # a graph reads its inputs where they were
+        runs.append((g, got, want, torch.cuda.Stream(), v))  # a graph reads its inputs where they were
     for _ in range(5):
         for g, got, _w, s, _in in runs:
             with torch.cuda.stream(s):
