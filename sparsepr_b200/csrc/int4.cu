@@ -256,17 +256,19 @@ __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int 
     if (m > largest[r]) atomicMax(&largest[r], m);
   }
   __syncthreads();
-  if (threadIdx.x < rows) power[threadIdx.x] = 21 - ((int)(largest[threadIdx.x] >> 23) - 127);
+  if (threadIdx.x < rows) power[threadIdx.x] = 21 - ((int)(largest[threadIdx.x] >> 23) - 127);  // -106 .. 148
   __syncthreads();
   for (int i = threadIdx.x; i < words * rows; i += blockDim.x) {
     const int r = i / words, b = i % words >> 2, word = i & 3, k = (b0 + b) * 32 + word * 8;
     float v[8];
     load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
+    const int half = power[r] / 2;  // 2^power may be past fp32: two factors, each exact
+    const float f0 = __int_as_float((127 + half) << 23), f1 = __int_as_float((127 + power[r] - half) << 23);
     uint32_t d[kLimbs][2] = {};
     int total[kLimbs] = {};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      int q = finite(v[e]) ? __float2int_rn(scalbnf(v[e], power[r])) : 0;
+      int q = finite(v[e]) ? __float2int_rn(v[e] * f0 * f1) : 0;
 #pragma unroll
       for (int l = 0; l < kLimbs; ++l) {
         const int byte = l == kLimbs - 1 ? q : (int)(int8_t)(q & 255);
@@ -545,14 +547,30 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Joins the slices in their order.
+// Joins slices (or walks) of `size` sums.  Where they are many (blockDim.y 8), 32 sums
+// by 8 threads, each every eighth slice in its order.
 __global__ void __launch_bounds__(256)
 int4_join_kernel(const float* partial, int slices, int64_t size, int64_t n, const void* bias, void* y, int dtype) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= size) return;
+  __shared__ float part[8][32];
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   float v = 0.f;
-  for (int s = 0; s < slices; ++s) v += partial[s * size + i];
-  store_f32(y, dtype, i, bias ? v + load_as_f32(bias, dtype, i % n) : v);
+  if (i < size)
+#pragma unroll 4
+    for (int s = threadIdx.y; s < slices; s += blockDim.y) v += partial[s * size + i];
+  if (blockDim.y > 1) {
+    part[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0)
+#pragma unroll
+      for (int q = 1; q < 8; ++q) v += part[q][threadIdx.x];
+  }
+  if (threadIdx.y == 0 && i < size) store_f32(y, dtype, i, bias ? v + load_as_f32(bias, dtype, i % n) : v);
+}
+
+void join_slices(const float* partial, int slices, int64_t size, int64_t n, const void* bias, void* y, int dtype,
+                 cudaStream_t st) {
+  const dim3 block = slices > 8 ? dim3(32, 8) : dim3(256, 1);
+  int4_join_kernel<<<(unsigned)((size + block.x - 1) / block.x), block, 0, st>>>(partial, slices, size, n, bias, y, dtype);
 }
 
 // The gradient.  A warp takes 128 columns of the weight (a chunk) and walks down its
@@ -564,11 +582,15 @@ int4_join_kernel(const float* partial, int slices, int64_t size, int64_t n, cons
 // groups of 32, one of four words and its even or odd codes), so that a product's
 // columns lie in one group.  Each walk's sums go to the workspace and are joined in a
 // fixed order.
+// The scales and zeros of the next band of weight rows are copied into shared memory
+// meanwhile (in whole pieces of eight groups, where they lie so); each thread widens
+// what it has copied itself.
 constexpr int kGradWarps = 8;
 constexpr int kGradRows = 32;    // weight rows of a stage
 constexpr int kGradBlocks = 4;   // blocks of 32 codes a row of a stage: 64 bytes
 constexpr int kGradStage = kGradRows * kGradBlocks * 16;
-constexpr int kGradBand = 256;   // weight rows whose scales and dy are in shared memory at a time
+constexpr int kGradThreads = kGradWarps * 32;
+static_assert(kStages == 4, "the waits for a band's pieces count the ring's stages");
 
 // Two rows to 128 bytes; pieces turned so that rows 0, 2, 4, 6 (or 1, 3, 5, 7) and two
 // neighbouring pieces meet all banks.
@@ -578,178 +600,276 @@ __device__ __forceinline__ int grad_piece(int row, int j) {
 
 struct GradShape {
   int chunks, along;        // chunks of a row; warps of a CTA on neighbouring chunks
-  int walk;                 // weight rows of one walk, a multiple of kGradRows
-  int walks;                // of a chunk
+  int beside;               // and on walks beside each other: 1, 2 or 4
+  int band;                 // weight rows, of all the CTA's walks, in shared memory at a time
+  int walk;                 // weight rows of one walk, a multiple of its share of a band
   int groups;               // of a CTA's chunks, at most
+  int scale, pieces;        // bytes of a scale that is copied ahead (0: none is); a row's pieces of eight
   int pass, rows;           // rows of dy in a pass, and of all passes
 };
 
-template <int MT, int G, int PARTS>
-__global__ void __launch_bounds__(kGradWarps * 32, MT == 1 ? 2 : 1)
+// HALVES: eights of a product's 16 rows that are used (1 with MT 1 and few rows).
+template <int MT, int HALVES, int G, int PARTS>
+__global__ void __launch_bounds__(kGradThreads, MT == 1 ? 2 : 1)
 int4_linear_grad_kernel(const Weights w, const GradShape sh, const void* dy, int64_t dy_stride, int dtype,
                         float* partial) {
   extern __shared__ __align__(128) char smem[];
-  constexpr int kTileRows = 16 / PARTS, kRowsMax = MT * kTileRows;  // rows of dy in a product, in all
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, beside = kGradWarps / sh.along;
+  constexpr int kTileRows = HALVES * 8 / PARTS, kRowsMax = MT * kTileRows;  // rows of dy in a product, in all
+  constexpr int kEights = MT * HALVES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, beside = sh.beside;
   const int row0 = blockIdx.z * sh.pass, rows = min(sh.pass, sh.rows - row0);
-  const int chunk0 = blockIdx.x * sh.along, chunk = chunk0 + warp % sh.along;
-  const int walk_id = blockIdx.y * beside + warp / sh.along;
-  // Bands of the CTA's walks, side by side: band row i*kGradBand/beside + ... is row i of a walk.
-  const int band = kGradBand / beside;
+  const int chunk0 = blockIdx.x * sh.along;
+  const int all = sh.band, band = all / beside, bands = sh.walk / band;  // band: a walk's rows of it
+  float2* meta = reinterpret_cast<float2*>(smem + kGradWarps * kStages * kGradStage);  // [band row][group]
+  float* dys = reinterpret_cast<float*>(meta + all * sh.groups);                        // [row of dy][band row]
+  char* raw = reinterpret_cast<char*>(dys + all * kRowsMax);  // [band row][piece] of scales, then of zeros
+  const int group0 = chunk0 * kGradBlocks / w.group_blocks, piece0 = group0 / 8;
+  const uint32_t raw_at = (uint32_t)__cvta_generic_to_shared(raw), raw_zero = all * sh.pieces * 8 * sh.scale;
+  // The weight row of a band row, -1 past the end of its walk.
+  auto weight_row = [&](int b, int br) {
+    const int64_t walk0 = ((int64_t)blockIdx.y * beside + br / band) * sh.walk, n = walk0 + b * band + br % band;
+    return n < min(w.n, walk0 + sh.walk) ? n : (int64_t)-1;
+  };
+  auto copy_raw = [&](int b) {
+    if (sh.scale)
+      for (int i = threadIdx.x; i < all * sh.pieces; i += kGradThreads) {
+        const int br = i / sh.pieces, p = min(piece0 + i % sh.pieces, w.groups / 8 - 1);
+        const int64_t n = weight_row(b, br), g = (n < 0 ? w.n - 1 : n) * w.groups + p * 8;
+        for (int h = 0; h < sh.scale / 2; ++h)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(raw_at + i * 8 * sh.scale + h * 16),
+                       "l"((const char*)w.scales + g * sh.scale + h * 16)
+                       : "memory");
+        if (w.zeros)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(raw_at + raw_zero + i * 8), "l"(w.zeros + g)
+                       : "memory");
+      }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  constexpr int kDyRegs = (kRowsMax + 1) / 2;  // of 128 band rows
+  float dy_next[kDyRegs];
+  auto load_dy = [&](int b) {
+#pragma unroll
+    for (int j = 0; j < kDyRegs; ++j) {
+      const int i = threadIdx.x + j * kGradThreads, br = i % all, r = i / all;
+      const int64_t n = r < rows ? weight_row(b, br) : -1;
+      dy_next[j] = n < 0 ? 0.f : load_as_f32(dy, dtype, (int64_t)(row0 + r) * dy_stride + n);
+    }
+  };
+  // The band's values in the form that the products take; whether any is so large (or
+  // not finite) that a product may leave fp32.
+  auto widen = [&](int b) {
+    bool large = false;
+    auto put = [&](int br, int g, float v, uint32_t z) {
+      if (g < 0 || g >= sh.groups) return;
+      meta[br * sh.groups + g] = make_float2(v, __uint_as_float(0x4300u + z));
+      large |= !(fabsf(v) < 0x1p60f);
+    };
+    if (sh.scale) {
+      for (int i = threadIdx.x; i < all * sh.pieces; i += kGradThreads) {
+        const int br = i / sh.pieces, g = (piece0 + i % sh.pieces) * 8 - group0;
+        const bool in = weight_row(b, br) >= 0;
+        const uint2 z8 = w.zeros ? *reinterpret_cast<const uint2*>(raw + raw_zero + i * 8)
+                                 : make_uint2(0x08080808u, 0x08080808u);
+        const char* from = raw + i * 8 * sh.scale;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v;
+          if (sh.scale == 4) {
+            v = reinterpret_cast<const float*>(from)[e];
+          } else {
+            const uint16_t h = reinterpret_cast<const uint16_t*>(from)[e];
+            v = w.scale_dtype == SPR_BF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+          }
+          put(br, g + e, in ? v : 0.f, (e < 4 ? z8.x >> 8 * e : z8.y >> 8 * (e - 4)) & 0xffu);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < all * sh.groups; i += kGradThreads) {
+        const int br = i / sh.groups, g = i % sh.groups;
+        const int64_t n = weight_row(b, br), at = n * w.groups + group0 + g;
+        const bool in = n >= 0 && group0 + g < w.groups;
+        put(br, g, in ? load_as_f32(w.scales, w.scale_dtype, at) : 0.f, in && w.zeros ? __ldg(w.zeros + at) : 8u);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kDyRegs; ++j) {
+      const int i = threadIdx.x + j * kGradThreads;
+      if (i < all * kRowsMax) dys[i] = dy_next[j];
+      large |= !(fabsf(dy_next[j]) < 0x1p60f);
+    }
+    return large;
+  };
+
+  const int chunk = chunk0 + warp % sh.along, walk_id = blockIdx.y * beside + warp / sh.along;
   const int64_t n0 = (int64_t)walk_id * sh.walk, n1 = min(w.n, n0 + sh.walk);
-  const int steps = sh.walk / kGradRows;
+  const bool mine = chunk < sh.chunks && warp < sh.along * beside && n0 < n1;
+  const int steps = mine ? (int)(n1 - n0 + kGradRows - 1) / kGradRows : 0;
   char* ring = smem + warp * kStages * kGradStage;
-  float* scales = reinterpret_cast<float*>(smem + kGradWarps * kStages * kGradStage);
-  float* dys = scales + kGradBand * sh.groups;
-  uint8_t* zeros = reinterpret_cast<uint8_t*>(dys + kGradBand * kRowsMax);
-  const int group0 = chunk0 * kGradBlocks / w.group_blocks;
   const int64_t pitch = (int64_t)w.blocks * 16;
-  const bool mine = chunk < sh.chunks;
 
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   uint32_t to[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) to[i] = ring_at + grad_piece(8 * i + (lane >> 2), lane & 3);
   const bool has_piece = mine && chunk * kGradBlocks + (lane & 3) < w.blocks;
-  const uint8_t* from = w.packed + (int64_t)chunk * (kGradBlocks * 16) + (lane & 3) * 16;
+  const uint8_t* from = w.packed + (n0 + (lane >> 2)) * pitch + (int64_t)chunk * (kGradBlocks * 16) + (lane & 3) * 16;
   int fetched = 0;
   auto fetch = [&](int stage) {
     if (fetched < steps && has_piece)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t n = min(n0 + fetched * kGradRows + 8 * i + (lane >> 2), w.n - 1);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kGradStage), "l"(from + n * pitch)
-                     : "memory");
+        if (n0 + fetched * kGradRows + 8 * i + (lane >> 2) < w.n)  // past the end: whatever the stage holds, times 0
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kGradStage),
+                       "l"(from + i * 8 * pitch)
+                       : "memory");
       }
+    from += kGradRows * pitch;
     ++fetched;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  copy_raw(0);
+  load_dy(0);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
 
   const int t = lane & 3, c8 = lane >> 2;
   constexpr int kTiles = kGradBlocks * 4;  // products' columns: 8 of the chunk's 128 each
   float acc[MT][kTiles][4] = {};
-  int stage = 0;
-  for (int step = 0; step < steps; ++step) {
-    const int at = step * kGradRows % band;  // within the walk's share of the band
-    if (at == 0) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < kGradBand * sh.groups; i += kGradWarps * 32) {
-        const int row = i / sh.groups, g = group0 + i % sh.groups;
-        const int64_t walk0 = ((int64_t)blockIdx.y * beside + row / band) * sh.walk;
-        const int64_t n = walk0 + step * kGradRows + row % band;
-        const bool in = n < min(w.n, walk0 + sh.walk) && g < w.groups;
-        scales[i] = in ? load_as_f32(w.scales, w.scale_dtype, n * w.groups + g) : 0.f;
-        zeros[i] = in && w.zeros ? __ldg(w.zeros + n * w.groups + g) : 8;
-      }
-      for (int i = threadIdx.x; i < kGradBand * rows; i += kGradWarps * 32) {
-        const int row = i % kGradBand, r = i / kGradBand;
-        const int64_t walk0 = ((int64_t)blockIdx.y * beside + row / band) * sh.walk;
-        const int64_t n = walk0 + step * kGradRows + row % band;
-        dys[row * kRowsMax + r] =
-            n < min(w.n, walk0 + sh.walk) ? load_as_f32(dy, dtype, (int64_t)(row0 + r) * dy_stride + n) : 0.f;
-      }
-      __syncthreads();
+  // The lane's rows of parts, one of each eight: its row of dy and which bits of a value
+  // the parts before its own hold.
+  int dy_row[kEights];
+  uint32_t cut0[kEights], cut1[kEights];
+#pragma unroll
+  for (int m = 0; m < kEights; ++m) {
+    const int rr = m % HALVES * 8 + c8, r = m / HALVES * kTileRows + rr / PARTS;
+    const bool in = rr < kTileRows * PARTS && r < rows;
+    dy_row[m] = in ? r * all : -1;
+    cut0[m] = rr % PARTS > 0 ? 0xffff0000u : 0u;
+    cut1[m] = rr % PARTS > 1 ? 0xffff0000u : 0u;
+  }
+  // Words of rows 2t (+1) and pieces: grad_piece of row 16h + 2t + 8q + o, piece 2b + ... is
+  // (8h + 4q + t)*128 + place[o][b].
+  int place[2][2];
+#pragma unroll
+  for (int o = 0; o < 2; ++o)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      place[o][b] = t * 128 + (((o * 4 + 2 * b) ^ (2 * t)) + (G == 1 ? 0 : c8 >> 2)) * 16 + (c8 & 3) * 4;
+  const int first_block = chunk * kGradBlocks;
+  int stage = 0, step = 0;
+  for (int b = 0; b < bands; ++b) {
+    // The band's pieces were copied before the ring's last `band / kGradRows` stages (at
+    // first its first three).
+    if (b == 0 || band >= 3 * kGradRows) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (band == 2 * kGradRows) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();  // the last readers of the band before are done
+    const bool large = widen(b);
+    if (b + 1 < bands) {
+      copy_raw(b + 1);
+      load_dy(b + 1);
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncwarp();
-    const char* codes_at = ring + stage * kGradStage;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int base = (warp / sh.along) * band + at + half * 16;  // band row of the first of 16 weight rows
-      float d[MT * 2][4];
-      bool low[MT * 2][2];
-#pragma unroll
-      for (int m = 0; m < MT * 2; ++m) {
-        const int rr = m % 2 * 8 + c8, r = m / 2 * kTileRows + rr / PARTS;
-        const bool in = rr < kTileRows * PARTS && r < rows;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[m][i] = in ? dys[(base + 2 * t + (i & 1) + (i >> 1) * 8) * kRowsMax + r] : 0.f;
-        low[m][0] = rr % PARTS == 1;
-        low[m][1] = rr % PARTS == 2;
+    const bool any_wild = __syncthreads_or(large);
+    const float* dband = dys;
+    for (int at = 0; at < band; at += kGradRows, ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();
+      if (step >= steps) {  // past the walk's end: the groups of copies go on being counted
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        continue;
       }
+      const char* codes_at = ring + stage * kGradStage;
 #pragma unroll
-      for (int gi = 0; gi < kGradBlocks / G; ++gi) {
-        const int block = chunk * kGradBlocks + gi * G;
-        if (block >= w.blocks || !mine) break;
-        const int g = (G < 4 && w.group_blocks == G ? block / G : block / w.group_blocks) - group0;
-        float s[4];
-        uint32_t z[4];
+      for (int half = 0; half < 2; ++half) {
+        const int base = warp / sh.along * band + at + half * 16 + 2 * t;  // band row of the lane's first weight row
+        float2 d[kEights][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int q = (base + 2 * t + (i & 1) + (i >> 1) * 8) * sh.groups + g;
-          s[i] = scales[q];
-          z[i] = zeros[q];
-        }
-        const uint32_t z01 = 0x43004300u + (z[0] | z[1] << 16), z23 = 0x43004300u + (z[2] | z[3] << 16);
-        uint32_t a[MT * 2][2];
+        for (int m = 0; m < kEights; ++m)
 #pragma unroll
-        for (int m = 0; m < MT * 2; ++m)
+          for (int q = 0; q < 2; ++q)
+            d[m][q] = dy_row[m] < 0 ? make_float2(0.f, 0.f)
+                                    : *reinterpret_cast<const float2*>(dband + dy_row[m] + base + 8 * q);
+        const float2* mp = meta + base * sh.groups;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[2];
+        for (int gi = 0; gi < kGradBlocks / G; ++gi) {
+          const int block = first_block + gi * G;
+          if (block >= w.blocks) break;
+          const int g = (G < 4 ? block / G : block / w.group_blocks) - group0;
+          const int gg = G < 4 && w.group_blocks != G ? block / w.group_blocks - group0 : g;
+          const float2 s[4] = {mp[gg], mp[gg + sh.groups], mp[gg + 8 * sh.groups], mp[gg + 9 * sh.groups]};
+          const uint32_t z01 = __byte_perm(__float_as_uint(s[0].y), __float_as_uint(s[1].y), 0x5410);
+          const uint32_t z23 = __byte_perm(__float_as_uint(s[2].y), __float_as_uint(s[3].y), 0x5410);
+          uint32_t a[MT * 2][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float f = d[m][2 * h + i] * s[2 * h + i];
-              const float hi = __uint_as_float(__float_as_uint(f) & 0xffff0000u);
-              float rest = f - hi;  // what is not finite is in the first part alone
-              if (rest != rest) rest = 0.f;
-              const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-              v[i] = __float_as_uint(low[m][0] ? (PARTS == 2 ? rest : mid) : f);
-              if (PARTS == 3 && low[m][1]) v[i] = __float_as_uint(rest - mid);
+          for (int m = 0; m < MT * 2; ++m)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              if (m % 2 >= HALVES) {
+                a[m][q] = 0;
+                continue;
+              }
+              const int e = m / 2 * HALVES + m % 2;
+              float v[2] = {d[e][q].x * s[2 * q].x, d[e][q].y * s[2 * q + 1].x};
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float all = v[i];
+                v[i] -= __uint_as_float(__float_as_uint(v[i]) & cut0[e]);
+                if (PARTS == 3) v[i] -= __uint_as_float(__float_as_uint(v[i]) & cut1[e]);
+                if (any_wild && !finite(all)) v[i] = cut0[e] ? 0.f : all;  // in the first part alone
+              }
+              a[m][q] = bf16_pair(__float_as_uint(v[0]), __float_as_uint(v[1]));
             }
-            a[m][h] = bf16_pair(v[0], v[1]);
-          }
-        if constexpr (G == 1) {
-          const int b = gi, odd = c8 >> 2;
-          uint32_t v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = half * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-            v[i] = *reinterpret_cast<const uint32_t*>(codes_at + grad_piece(row, b) + (c8 & 3) * 4) >> (4 * odd);
-          }
-          const uint32_t l0 = __byte_perm(v[0], v[1], 0x5410), h0 = __byte_perm(v[0], v[1], 0x7632);
-          const uint32_t l1 = __byte_perm(v[2], v[3], 0x5410), h1 = __byte_perm(v[2], v[3], 0x7632);
-          const uint32_t b0[4] = {codes<0>(l0, z01), codes<2>(l0, z01), codes<0>(h0, z01), codes<2>(h0, z01)};
-          const uint32_t b1[4] = {codes<0>(l1, z23), codes<2>(l1, z23), codes<0>(h1, z23), codes<2>(h1, z23)};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-              mma_bf16(acc[m][b * 4 + j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b0[j], b1[j]);
-        } else {
-#pragma unroll
-          for (int u = 0; u < G / 2; ++u) {
-            const int b = gi * G / 2 + u;  // 64 columns
+          if constexpr (G == 1) {
+            const int odd = (c8 >> 2) * 4;
             uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = half * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-              v[i] = *reinterpret_cast<const uint32_t*>(codes_at + grad_piece(row, 2 * b + (c8 >> 2)) + (c8 & 3) * 4);
-            }
+            for (int i = 0; i < 4; ++i)
+              v[i] = *reinterpret_cast<const uint32_t*>(codes_at + (8 * half + 4 * (i >> 1)) * 128 +
+                                                        (place[i & 1][gi >> 1] ^ (gi & 1) * 16)) >>
+                     odd;
             const uint32_t l0 = __byte_perm(v[0], v[1], 0x5410), h0 = __byte_perm(v[0], v[1], 0x7632);
             const uint32_t l1 = __byte_perm(v[2], v[3], 0x5410), h1 = __byte_perm(v[2], v[3], 0x7632);
-            const uint32_t b0[8] = {codes<0>(l0, z01), codes<1>(l0, z01), codes<2>(l0, z01), codes<3>(l0, z01),
-                                    codes<0>(h0, z01), codes<1>(h0, z01), codes<2>(h0, z01), codes<3>(h0, z01)};
-            const uint32_t b1[8] = {codes<0>(l1, z23), codes<1>(l1, z23), codes<2>(l1, z23), codes<3>(l1, z23),
-                                    codes<0>(h1, z23), codes<1>(h1, z23), codes<2>(h1, z23), codes<3>(h1, z23)};
+            const uint32_t b0[4] = {codes<0>(l0, z01), codes<2>(l0, z01), codes<0>(h0, z01), codes<2>(h0, z01)};
+            const uint32_t b1[4] = {codes<0>(l1, z23), codes<2>(l1, z23), codes<0>(h1, z23), codes<2>(h1, z23)};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
               for (int m = 0; m < MT; ++m)
-                mma_bf16(acc[m][b * 8 + j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b0[j], b1[j]);
+                mma_bf16(acc[m][gi * 4 + j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b0[j], b1[j]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < G / 2; ++u) {
+              const int b64 = gi * G / 2 + u;  // 64 columns
+              uint32_t v[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                v[i] = *reinterpret_cast<const uint32_t*>(codes_at + (8 * half + 4 * (i >> 1)) * 128 +
+                                                          place[i & 1][b64]);
+              const uint32_t l0 = __byte_perm(v[0], v[1], 0x5410), h0 = __byte_perm(v[0], v[1], 0x7632);
+              const uint32_t l1 = __byte_perm(v[2], v[3], 0x5410), h1 = __byte_perm(v[2], v[3], 0x7632);
+              const uint32_t b0[8] = {codes<0>(l0, z01), codes<1>(l0, z01), codes<2>(l0, z01), codes<3>(l0, z01),
+                                      codes<0>(h0, z01), codes<1>(h0, z01), codes<2>(h0, z01), codes<3>(h0, z01)};
+              const uint32_t b1[8] = {codes<0>(l1, z23), codes<1>(l1, z23), codes<2>(l1, z23), codes<3>(l1, z23),
+                                      codes<0>(h1, z23), codes<1>(h1, z23), codes<2>(h1, z23), codes<3>(h1, z23)};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                  mma_bf16(acc[m][b64 * 8 + j], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b0[j],
+                           b1[j]);
+            }
           }
         }
       }
+      // The stage that this fetch fills was read in the round before.
+      fetch(stage == 0 ? kStages - 1 : stage - 1);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-    // The stage that this fetch fills was read in the round before.
-    fetch(stage == 0 ? kStages - 1 : stage - 1);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
-  if (!mine || n0 >= n1) return;
+  if (!mine) return;
   // The warp's ring takes a product's sums in the order of the columns; a row's parts
   // are added in their order.
   float* out = reinterpret_cast<float*>(ring);  // [16][128]
@@ -821,8 +941,8 @@ struct ForwardPlan {
 // Rows a pass: what 32 columns of a product hold.  16-bit rows go to the integer
 // products while one pass holds them; more of them take fewer columns as bf16 parts
 // (of measured bandwidth at 122,880 x 5120, group 64: see launch_forward).  The columns
-// of the weight are cut into slices where the staged rows would take more than 36 KB
-// a CTA, and where too few tiles would leave SMs without work.
+// of the weight are cut into slices where the staged rows would leave no room for the
+// rings of twelve warps (eight of the widest products), and where too few tiles would leave SMs without work.
 ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   ForwardPlan p{};
   p.ints = dtype != SPR_F32 && rows <= 32 / kLimbs;
@@ -842,7 +962,8 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
                     aligned(w.scales, 16) && aligned(w.zeros, 8)
                 ? dtype_bytes(w.scale_dtype)
                 : 0;
-  int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + 36863) / 36864));
+  const int x_bytes = kSmem - std::min(12, most) * (kStages * kStageBytes + 3072 + 2 * kTile * p.nt * 8 * 4);
+  int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + x_bytes - 1) / x_bytes));
   if (tiles * p.passes < sms) slices = std::max<int64_t>(slices, std::min<int64_t>(chunks / 4, sms / (tiles * p.passes)));
   p.sh.slice_chunks = (chunks + slices - 1) / slices;
   p.sh.slices = (chunks + p.sh.slice_chunks - 1) / p.sh.slice_chunks;
@@ -889,7 +1010,7 @@ int launch_forward(const ForwardPlan& p, const Weights& w, const void* x, int64_
       w, p.sh, in, kInt ? 1.f : ldexpf(1.f, -e), kInt ? 1.f : ldexpf(1.f, e), partial ? nullptr : bias, y, partial);
   if (partial) {
     const int64_t size = (int64_t)rows * w.n;
-    int4_join_kernel<<<(unsigned)((size + 255) / 256), 256, 0, st>>>(partial, p.sh.slices, size, w.n, bias, y, dtype);
+    join_slices(partial, p.sh.slices, size, w.n, bias, y, dtype, st);
   }
   return check_launch("int4 linear");
 }
@@ -915,7 +1036,7 @@ int by_plan(const ForwardPlan& p, F f) {
 
 struct GradPlan {
   GradShape sh;
-  int mt, g, parts, walks, passes, smem;
+  int mt, halves, g, parts, walks, passes, smem;
   dim3 grid;
 };
 
@@ -924,34 +1045,40 @@ struct GradPlan {
 GradPlan plan_grad(int64_t rows, const Weights& w, int dtype) {
   GradPlan p{};
   p.parts = dtype == SPR_BF16 && w.scale_dtype == SPR_BF16 ? 2 : 3;
-  const int tile_rows = 16 / p.parts;
+  p.halves = rows * p.parts <= 8 ? 1 : 2;
+  const int tile_rows = p.halves * 8 / p.parts;
   p.mt = rows > tile_rows ? 2 : 1;
   p.g = w.group_blocks % 4 == 0 ? 4 : w.group_blocks % 2 == 0 ? 2 : 1;
   p.sh.rows = (int)rows;
   p.sh.pass = (int)std::min<int64_t>(rows, p.mt * tile_rows);
   p.passes = (int)((rows + p.sh.pass - 1) / p.sh.pass);
   p.sh.chunks = (w.blocks + kGradBlocks - 1) / kGradBlocks;
-  p.sh.along = 1;
-  while (p.sh.along < kGradWarps && p.sh.along < p.sh.chunks) p.sh.along *= 2;
-  const int beside = kGradWarps / p.sh.along, across = (p.sh.chunks + p.sh.along - 1) / p.sh.along;
+  p.sh.along = p.sh.chunks >= 8 ? 8 : p.sh.chunks >= 4 ? 4 : 2;
+  p.sh.beside = kGradWarps / p.sh.along;
+  p.sh.groups = (p.sh.along * kGradBlocks - 1) / w.group_blocks + 2;
+  p.sh.band = p.sh.groups > 20 && p.sh.beside <= 2 ? 64 : 128;
+  p.sh.scale = w.groups % 8 == 0 && aligned(w.scales, 16) && aligned(w.zeros, 8) ? dtype_bytes(w.scale_dtype) : 0;
+  p.sh.pieces = (p.sh.groups + 6) / 8 + 1;
+  const int beside = p.sh.beside, across = (p.sh.chunks + p.sh.along - 1) / p.sh.along;
+  const int band = p.sh.band / beside;
   const int64_t ctas = (int64_t)sm_count() * (p.mt == 1 ? 2 : 1);
   int64_t walks = std::max<int64_t>(1, ctas / (across * p.passes)) * beside;
   walks = std::max<int64_t>(1, std::min(walks, w.n / 128));
-  p.sh.walk = (int)((w.n + walks - 1) / walks + kGradRows - 1) / kGradRows * kGradRows;
+  p.sh.walk = (int)(((w.n + walks - 1) / walks + band - 1) / band * band);
   p.walks = (int)((w.n + p.sh.walk - 1) / p.sh.walk);
-  p.sh.groups = (p.sh.along * kGradBlocks - 1) / w.group_blocks + 2;
-  p.smem = kGradWarps * kStages * kGradStage + kGradBand * (p.sh.groups * 5 + p.mt * tile_rows * 4);
+  p.smem = kGradWarps * kStages * kGradStage +
+           p.sh.band * (p.sh.groups * 8 + p.mt * tile_rows * 4 + (p.sh.scale ? p.sh.pieces * (8 * p.sh.scale + 8) : 0));
   p.grid = dim3(across, (p.walks + beside - 1) / beside, p.passes);
   return p;
 }
 
-template <int MT, int G, int PARTS>
+template <int MT, int HALVES, int G, int PARTS>
 int launch_grad(const GradPlan& p, const Weights& w, const void* dy, int64_t dy_stride, int dtype, float* partial,
                 cudaStream_t st) {
-  auto kern = int4_linear_grad_kernel<MT, G, PARTS>;
+  auto kern = int4_linear_grad_kernel<MT, HALVES, G, PARTS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
     return check_launch("int4 linear grad");
-  kern<<<p.grid, kGradWarps * 32, p.smem, st>>>(w, p.sh, dy, dy_stride, dtype, partial);
+  kern<<<p.grid, kGradThreads, p.smem, st>>>(w, p.sh, dy, dy_stride, dtype, partial);
   return check_launch("int4 linear grad");
 }
 
@@ -1013,19 +1140,22 @@ extern "C" int spr_int4_linear_grad(const void* dy, int64_t dy_stride, int dtype
     const size_t need = spr_int4_linear_grad_workspace_bytes(rows, n, k, group, dtype);
     if (!workspace || workspace_bytes < need)
       return fail(SPR_ERR_WORKSPACE, "int4 linear grad: workspace %zu < %zu bytes", workspace_bytes, need);
-    auto by_group = [&](auto mt, auto parts) {
-      constexpr int MT = decltype(mt)::value, PARTS = decltype(parts)::value;
+    auto by_group = [&](auto mt, auto halves, auto parts) {
+      constexpr int MT = decltype(mt)::value, H = decltype(halves)::value, PARTS = decltype(parts)::value;
       float* out = (float*)workspace;
-      return p.g == 4   ? launch_grad<MT, 4, PARTS>(p, w, dy, dy_stride, dtype, out, st)
-             : p.g == 2 ? launch_grad<MT, 2, PARTS>(p, w, dy, dy_stride, dtype, out, st)
-                        : launch_grad<MT, 1, PARTS>(p, w, dy, dy_stride, dtype, out, st);
+      return p.g == 4   ? launch_grad<MT, H, 4, PARTS>(p, w, dy, dy_stride, dtype, out, st)
+             : p.g == 2 ? launch_grad<MT, H, 2, PARTS>(p, w, dy, dy_stride, dtype, out, st)
+                        : launch_grad<MT, H, 1, PARTS>(p, w, dy, dy_stride, dtype, out, st);
     };
-    auto by_rows = [&](auto parts) { return p.mt == 1 ? by_group(Int<1>{}, parts) : by_group(Int<2>{}, parts); };
+    auto by_rows = [&](auto parts) {
+      return p.halves == 1 ? by_group(Int<1>{}, Int<1>{}, parts)
+             : p.mt == 1   ? by_group(Int<1>{}, Int<2>{}, parts)
+                           : by_group(Int<2>{}, Int<2>{}, parts);
+    };
     if (int rc = p.parts == 2 ? by_rows(Int<2>{}) : by_rows(Int<3>{})) return rc;
     walks = p.walks;
   }
   const int64_t size = rows * k;
-  int4_join_kernel<<<(unsigned)((size + 255) / 256), 256, 0, st>>>((const float*)workspace, walks, size, k, nullptr, dx,
-                                                                   dtype);
+  join_slices((const float*)workspace, walks, size, k, nullptr, dx, dtype, st);
   return check_launch("int4 linear grad");
 }
