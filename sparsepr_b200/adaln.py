@@ -122,39 +122,47 @@ def operands(x, y, gate, shift, scale, scale_offset: float = 1.0):
     return op, (mb, mn)
 
 
+def _backward(ctx, *grads):
+    x, y, gate, scale, stats = ctx.saved_tensors
+    dz, dh = grads if y is not None else (None, grads[0])
+    if dh is None:
+        if dz is None:
+            return (None,) * 7
+        dh = torch.zeros_like(dz, memory_format=torch.contiguous_format)
+    elif not dh.is_contiguous():
+        dh = dh.contiguous()
+    if dz is not None and not dz.is_contiguous():
+        dz = dz.contiguous()
+    s, mod_shape, vector_shape, mod_dtype = ctx.operands
+    s = type(s).from_buffer_copy(s)
+    s.x = x.data_ptr()
+    if y is not None:  # the norm's input is z, which is dense
+        s.y, s.x_sb, s.x_st = y.data_ptr(), s.tokens * s.channels, s.channels
+    s.gate = None if gate is None else gate.data_ptr()
+    s.scale = None if scale is None else scale.data_ptr()
+    mean = stats.data_ptr()
+    s.mean, s.rstd = mean, mean + 4 * stats.shape[1]
+    return *K.adaln_backward_struct(s, y is not None, dh, dz, ctx.needs_input_grad[2:5], mod_shape, vector_shape, mod_dtype), None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _AdaLN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, shift, scale, eps, scale_offset):
         op, mod_shape = operands(x, y, gate, shift, scale, scale_offset)
-        z, h, stats = K.adaln_forward(op, eps, True)
+        z, h, stats, struct = K.adaln_forward_struct(op, eps, True)
         ctx.save_for_backward(x if z is None else z, y, gate, scale, stats)
         ctx.set_materialize_grads(False)
-        # What the backward pass needs of the operands apart from the tensors; z is dense.
-        dense = (op.tokens * op.channels if op.batch > 1 else 0, op.channels if op.tokens > 1 else 0)
-        ctx.op = op._replace(x=None, y=None, gate=None, shift=None, scale=None,
-                             x_strides=op.x_strides if z is None else dense)
-        ctx.mod_shape = mod_shape
-        ctx.vector = next((t.shape for t in (gate, shift, scale) if t is not None), None)
+        vector = gate if gate is not None else shift if shift is not None else scale
+        ctx.operands = struct, mod_shape, None if vector is None else vector.shape, op.mod_dtype
         return h if z is None else (z, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
-        x, y, gate, scale, stats = ctx.saved_tensors
-        dz, dh = grads if y is not None else (None, grads[0])
-        if dh is None:
-            if dz is None:
-                return (None,) * 7
-            dh = torch.zeros_like(dz, memory_format=torch.contiguous_format)
-        elif not dh.is_contiguous():
-            dh = dh.contiguous()
-        if dz is not None and not dz.is_contiguous():
-            dz = dz.contiguous()
-        op = ctx.op._replace(x=x, y=y, gate=gate, scale=scale)
-        dx, dy, dgate, dshift, dscale = K.adaln_backward(op, stats, dh, dz, ctx.needs_input_grad[2:5], ctx.mod_shape)
-        v = ctx.vector
-        return (dx, dy, None if dgate is None else dgate.view(v), None if dshift is None else dshift.view(v),
-                None if dscale is None else dscale.view(v), None, None)
+        # The wrapper that refuses second derivatives, where a graph of this pass is asked for.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, *grads)
 
 
 def _wants_grad(x, y, gate, shift, scale):

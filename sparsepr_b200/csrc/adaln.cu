@@ -850,7 +850,7 @@ int check_adaln(const SprAdaln* op) {
   if (op->mod_dtype != op->dtype && op->mod_dtype != SPR_F32)
     return fail(SPR_ERR_DTYPE, "adaln: shift/scale/gate dtype %d must be the element type %d or fp32", op->mod_dtype,
                 op->dtype);
-  if (op->gate && !op->y) return fail(SPR_ERR_ARG, "adaln: a gate without a branch");
+  if (op->gate && !op->y && op->batch * op->tokens) return fail(SPR_ERR_ARG, "adaln: a gate without a branch");
   return SPR_OK;
 }
 

@@ -121,15 +121,12 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[U]) {
 }
 
 // Scales and zeros of a warp's weight rows.  Where a row's lie in whole aligned pieces
-// of eight groups (kScale, their bytes), all that the warp needs of a tile is copied
-// with the tile's first chunk: neighbouring lanes take neighbouring pieces, so that a
-// row's are few memory requests.  Otherwise (kScale 0) the values of each chunk's
-// segments (GB blocks, within one group) are loaded one chunk ahead into registers.
-// A row's pieces and one more, if even, lie apart from the next row's: an odd number
+// of eight groups (kScale, their bytes), those of a span of at least four chunks are
+// copied with the span's first chunk: neighbouring lanes take neighbouring pieces, so
+// that a row's are few memory requests.  Otherwise (kScale 0) the values of each
+// chunk's segments (GB blocks, within one group) are loaded one chunk ahead into
+// registers.  A slot holds a span; a row's pieces take an odd number of places, which
 // keeps the rows in different banks.
-struct Pieces {
-  int first, count, pitch;  // of eight groups; pitch odd
-};
 constexpr int piece_bytes(int scale) { return 8 * (scale ? scale : 4) + 8; }
 
 template <int GB>
@@ -162,7 +159,8 @@ struct Values {
 struct Shape {
   int along, tiles, warp_chunks;
   int slice_chunks, slices;
-  int slots, slot_bytes;  // a warp's slots of scales and zeros
+  int span, pieces, places;  // chunks of a span, its pieces a row, the places they take
+  int slots, slot_bytes;     // a warp's slots of scales and zeros
 };
 
 // Eight values of x from column k, zeros past the end.
@@ -226,61 +224,82 @@ __device__ __forceinline__ void stage_bf16(const Weights& w, const Rows& in, int
   }
 }
 
-// Integers round(x * 2^power[r]) below 2^22 in magnitude, as bytes d0 + 256 d1 + 65536 d2;
-// sums[segment's first block][column]: the bytes of a segment added up.  What is not
-// finite counts as 0 and sets bad[r].
-template <int U, int GB>
-__device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, bool wide,
-                                          uint2* xs, int* sums, int sum_cols, uint32_t* largest, int* power, int* bad) {
-  const int cols = rows * kLimbs;
+// Each row's largest magnitude of the slice's x, and whether any is not finite.
+__device__ __forceinline__ void scan_x(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, bool wide,
+                                       uint32_t* largest, int* bad) {
+  const int words = nb * 4;
   if (threadIdx.x < 32) {
     largest[threadIdx.x] = 0;
     bad[threadIdx.x] = 0;
   }
-  for (int i = threadIdx.x; i < nb * sum_cols; i += blockDim.x) sums[i] = 0;
   __syncthreads();
-  const int words = nb * 4;
-  for (int i = threadIdx.x; i < words * rows; i += blockDim.x) {
-    const int r = i / words, k = b0 * 32 + i % words * 8;
-    float v[8];
-    load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
-    uint32_t m = 0;
-    bool any = false;
+  for (int r = 0; r < rows; ++r) {
+    uint32_t most = 0, any = 0;
+    for (int i = threadIdx.x; i < words; i += blockDim.x) {
+      const int k = b0 * 32 + i * 8;
+      float v[8];
+      load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t u = __float_as_uint(v[e]) & 0x7fffffffu;
-      any |= u >= 0x7f800000u;
-      m = max(m, u >= 0x7f800000u ? 0u : u);
-    }
-    if (any) bad[r] = 1;
-    if (m > largest[r]) atomicMax(&largest[r], m);
-  }
-  __syncthreads();
-  if (threadIdx.x < rows) power[threadIdx.x] = 21 - ((int)(largest[threadIdx.x] >> 23) - 127);  // -106 .. 148
-  __syncthreads();
-  for (int i = threadIdx.x; i < words * rows; i += blockDim.x) {
-    const int r = i / words, b = i % words >> 2, word = i & 3, k = (b0 + b) * 32 + word * 8;
-    float v[8];
-    load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
-    const int half = power[r] / 2;  // 2^power may be past fp32: two factors, each exact
-    const float f0 = __int_as_float((127 + half) << 23), f1 = __int_as_float((127 + power[r] - half) << 23);
-    uint32_t d[kLimbs][2] = {};
-    int total[kLimbs] = {};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      int q = finite(v[e]) ? __float2int_rn(v[e] * f0 * f1) : 0;
-#pragma unroll
-      for (int l = 0; l < kLimbs; ++l) {
-        const int byte = l == kLimbs - 1 ? q : (int)(int8_t)(q & 255);
-        q = (q - byte) >> 8;
-        d[l][e & 1] |= (uint32_t)(byte & 255) << (8 * (e >> 1));
-        total[l] += byte;
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t u = __float_as_uint(v[e]) & 0x7fffffffu;
+        any |= u >= 0x7f800000u;
+        most = max(most, u >= 0x7f800000u ? 0u : u);
       }
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    any = __reduce_or_sync(0xffffffffu, any);
+    if ((threadIdx.x & 31) == 0) {
+      if (any) bad[r] = 1;
+      if (most > largest[r]) atomicMax(&largest[r], most);
+    }
+  }
+  __syncthreads();
+}
+
+// Integers q = round(x * 2^power[r]) below 2^22 in magnitude, as signed bytes d0 + 256 d1
+// + 65536 d2: the bytes of q + 0x808080 less 128 each.  sums[segment's first block]
+// [column]: the bytes of a segment added up.  What is not finite counts as 0 and sets
+// bad[r].
+template <int U, int GB>
+__device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, bool wide,
+                                          uint2* xs, int* sums, int sum_cols, const uint32_t* largest, int* power,
+                                          const int* bad) {
+  const int cols = rows * kLimbs, words = nb * 4;
+  for (int r = 0; r < rows; ++r) {
+    const int p = 21 - ((int)(largest[r] >> 23) - 127), half = p / 2;  // -106 .. 148: two factors, each exact
+    if (threadIdx.x == 0) power[r] = p;
+    const float f0 = __int_as_float((127 + half) << 23), f1 = __int_as_float((127 + p - half) << 23);
+    const bool check = bad[r];
+    for (int first = 0; first < words; first += blockDim.x) {
+      const int i = first + threadIdx.x, b = i >> 2, word = i & 3, k = b0 * 32 + i * 8;
+      uint32_t u[8];
+      if (i < words) {
+        float v[8];
+        load_x(in, wide, (int64_t)(row0 + r) * in.stride + k, k, w.k, v);
 #pragma unroll
-    for (int l = 0; l < kLimbs; ++l) {
-      xs[x_place<U>(b, word, cols, r * kLimbs + l)] = make_uint2(d[l][0], d[l][1]);
-      atomicAdd(&sums[b / GB * GB * sum_cols + r * kLimbs + l], total[l]);  // whole numbers: any order
+        for (int e = 0; e < 8; ++e) {
+          if (check && !finite(v[e])) v[e] = 0.f;
+          u[e] = 0x808080 + __float2int_rn(v[e] * f0 * f1);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = 0x808080;
+      }
+#pragma unroll
+      for (int l = 0; l < kLimbs; ++l) {
+        constexpr uint32_t pick[kLimbs] = {0x40, 0x51, 0x62};
+        const uint32_t d0 = __byte_perm(__byte_perm(u[0], u[2], pick[l]), __byte_perm(u[4], u[6], pick[l]), 0x5410) ^
+                            0x80808080u;
+        const uint32_t d1 = __byte_perm(__byte_perm(u[1], u[3], pick[l]), __byte_perm(u[5], u[7], pick[l]), 0x5410) ^
+                            0x80808080u;
+        int total = __dp4a((int)d0, 0x01010101, __dp4a((int)d1, 0x01010101, 0));
+#pragma unroll
+        for (int o = 1; o < 4 * GB; o *= 2) total += __shfl_xor_sync(0xffffffffu, total, o);  // a segment's words
+        if (i < words) {
+          xs[x_place<U>(b, word, cols, r * kLimbs + l)] = make_uint2(d0, d1);
+          if (i % (4 * GB) == 0) sums[b * sum_cols + r * kLimbs + l] = total;
+        }
+      }
     }
   }
 }
@@ -295,7 +314,8 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t largest[32];
   __shared__ int power[32], bad[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = sh.along * sh.tiles;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: the same in all lanes
+  const int warps = sh.along * sh.tiles;
   const int row0 = blockIdx.y * in.pass, rows = min(in.pass, in.all - row0), cols = rows * in.parts;
   const int c0 = blockIdx.z * sh.slice_chunks;
   const int c1 = min((w.blocks + kBlocks - 1) / kBlocks, c0 + sh.slice_chunks);
@@ -325,11 +345,9 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   const Place start = {(int)(blockIdx.x * sh.tiles + wt), from_chunk};
   Place copy = start, at = start, load = start;
 
-  Pieces pc;
-  pc.first = from_chunk * kBlocks / w.group_blocks / 8;
-  pc.count = max(0, (min(w.blocks, to_chunk * kBlocks) - 1) / w.group_blocks / 8 + 1 - pc.first);
-  pc.pitch = kScale ? pc.count | 1 : 1;
-  const uint32_t inv_count = pc.count > 0 ? (65536 + pc.count - 1) / pc.count : 0;  // i / count for i < 16*count < 4096
+  // A span's chunks lie between multiples of its length; the first of a tile may start within.
+  const int lead = kScale ? from_chunk % sh.span : 0;
+  const uint32_t inv_pieces = kScale ? (65536 + sh.pieces - 1) / sh.pieces : 0;  // i / pieces for i below 16*pieces
   const uint8_t* from[kTile / 4];  // the lane's 16 bytes of rows lane/8 + 4i, in the chunk to copy
   auto aim = [&]() {
 #pragma unroll
@@ -342,21 +360,22 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
 #pragma unroll
   for (int i = 0; i < kTile / 4; ++i) to[i] = ring_at + piece(i * 4 + (lane >> 3), lane & 7);
   aim();
-  int copy_slot = 0, use_slot = 0;
+  int copy_slot = 0, use_slot = 0, copy_at = lead, use_at = lead;  // chunks from the span's start
   auto copy_scales = [&]() {
-    const uint32_t dst = slot_at + copy_slot * sh.slot_bytes, dst_zero = dst + kTile * pc.pitch * 8 * kScale;
+    const uint32_t dst = slot_at + copy_slot * sh.slot_bytes, dst_zero = dst + kTile * sh.places * 8 * kScale;
     copy_slot = copy_slot + 1 == sh.slots ? 0 : copy_slot + 1;
-    for (int i = lane; i < kTile * pc.count; i += 32) {
-      const int row = i * inv_count >> 16, p = i - row * pc.count;
-      const int64_t g = min((int64_t)copy.tile * kTile + row, w.n - 1) * w.groups + (pc.first + p) * 8;
-      const int slot = row * pc.pitch + p;
+    const int first = (copy.chunk - copy_at) / w.group_blocks;  // piece: eight groups of group_blocks/8 chunks
+    for (int i = lane; i < kTile * sh.pieces; i += 32) {
+      const int row = i * inv_pieces >> 16, p = i - row * sh.pieces;
+      const int64_t g = min((int64_t)copy.tile * kTile + row, w.n - 1) * w.groups + min(first + p, w.groups / 8 - 1) * 8;
+      const int place = row * sh.places + p;
 #pragma unroll
       for (int h = 0; h < kScale / 2; ++h)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + slot * 8 * kScale + h * 16),
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + place * 8 * kScale + h * 16),
                      "l"((const char*)w.scales + g * kScale + h * 16)
                      : "memory");
       if (w.zeros)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst_zero + slot * 8), "l"(w.zeros + g) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst_zero + place * 8), "l"(w.zeros + g) : "memory");
     }
   };
   auto fetch = [&](int stage) {
@@ -366,13 +385,21 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
         for (int i = 0; i < kTile / 4; ++i)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kStageBytes), "l"(from[i])
                        : "memory");
-      if (kScale && copy.chunk == from_chunk) copy_scales();
+      if (kScale && (copy.chunk == from_chunk || copy_at == 0) && copy.chunk < to_chunk) copy_scales();
 #pragma unroll
       for (int i = 0; i < kTile / 4; ++i) from[i] += kBlocks * 16;
-      if (next(copy)) aim();
+      copy_at = copy_at + 1 == sh.span ? 0 : copy_at + 1;
+      if (next(copy)) {
+        aim();
+        copy_at = lead;
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // x first: behind the rings' first copies its loads would wait for 100 KB an SM.
+  const bool wide = in.dtype != SPR_F32 && in.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in.x) % 16 == 0;
+  if constexpr (kInt) scan_x(w, in, row0, rows, b0, nb, wide, largest, bad);
+  else stage_bf16<U>(w, in, row0, rows, b0, nb, down, wide, reinterpret_cast<uint4*>(xs));
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
   Values<GB> values;
@@ -382,10 +409,8 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
     if (load.tile < tiles) values.load(w, load_at, load.chunk, lane);
   }
 
-  const bool wide = in.dtype != SPR_F32 && in.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in.x) % 16 == 0;
   if constexpr (kInt)
     stage_int<U, GB>(w, in, row0, rows, b0, nb, wide, reinterpret_cast<uint2*>(xs), sums, NT * 8, largest, power, bad);
-  else stage_bf16<U>(w, in, row0, rows, b0, nb, down, wide, reinterpret_cast<uint4*>(xs));
   __syncthreads();
 
   uint64_t acc[NT][2] = {};  // pairs of neighbouring columns, rows r8 and r8 + 8
@@ -409,11 +434,12 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
     const char* xb = xs + (first - b0) * block_bytes;
     const int* sb = sums + (first - b0) * (NT * 8) + 2 * t;
     // The lane's rows' scales and zeros, from the chunk's first segment's group on.
+    constexpr int kBytes = kScale ? kScale : 4;
     const char* slot = slots + use_slot * sh.slot_bytes;
-    const int group0 = kScale ? (GB < 8 ? first / GB : first / w.group_blocks) - pc.first * 8 : 0;
-    const char* sp = slot + r8 * pc.pitch * 8 * (kScale ? kScale : 4) + group0 * (kScale ? kScale : 4);
-    const uint8_t* zp = reinterpret_cast<const uint8_t*>(slot) + kTile * pc.pitch * 8 * (kScale ? kScale : 4) +
-                        r8 * pc.pitch * 8 + group0;
+    const int places = kScale ? sh.places : 1;
+    const int group0 = !kScale ? 0 : GB < 8 ? use_at * (8 / GB) : use_at * kBlocks / w.group_blocks;
+    const char* sp = slot + (r8 * places * 8 + group0) * kBytes;
+    const uint8_t* zp = reinterpret_cast<const uint8_t*>(slot) + kTile * places * 8 * kBytes + r8 * places * 8 + group0;
     float2 m0, m1;
     float c[NT][4];
     int ci[NT][4];
@@ -424,18 +450,18 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
         const int g = u / kUnits;
         if constexpr (kScale == 2) {
           const uint16_t h0 = reinterpret_cast<const uint16_t*>(sp)[g];
-          const uint16_t h1 = reinterpret_cast<const uint16_t*>(sp + pc.pitch * 128)[g];
+          const uint16_t h1 = reinterpret_cast<const uint16_t*>(sp + places * 128)[g];
           const bool bf = w.scale_dtype == SPR_BF16;
           m0.x = bf ? __uint_as_float((uint32_t)h0 << 16) : __half2float(__ushort_as_half(h0));
           m1.x = bf ? __uint_as_float((uint32_t)h1 << 16) : __half2float(__ushort_as_half(h1));
         } else {
           m0.x = reinterpret_cast<const float*>(sp)[g];
-          m1.x = reinterpret_cast<const float*>(sp + pc.pitch * 256)[g];
+          m1.x = reinterpret_cast<const float*>(sp + places * 256)[g];
         }
         int z0 = 8, z1 = 8;
         if (!kScale || w.zeros) {
           z0 = zp[g];
-          z1 = zp[pc.pitch * 64 + g];
+          z1 = zp[places * 64 + g];
         }
         if constexpr (!kInt) {
           m0.y = __int_as_float(0x43004300 + 0x00010001 * z0);
@@ -502,7 +528,8 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
     stage = stage + 1 == kStages ? 0 : stage + 1;
     const int tile = at.tile;
     const bool done = next(at);
-    if (!kScale || done) use_slot = use_slot + 1 == sh.slots ? 0 : use_slot + 1;
+    use_at = done ? lead : use_at + 1 == sh.span ? 0 : use_at + 1;
+    if (!kScale || done || use_at == 0) use_slot = use_slot + 1 == sh.slots ? 0 : use_slot + 1;
     if (!done) continue;
     // The tile is done: join the warps' sums and a row's columns.
     float* mine = red + ((odd * sh.tiles + wt) * sh.along + wk) * kTile * NT * 8;
@@ -962,7 +989,7 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
                     aligned(w.scales, 16) && aligned(w.zeros, 8)
                 ? dtype_bytes(w.scale_dtype)
                 : 0;
-  const int x_bytes = kSmem - std::min(12, most) * (kStages * kStageBytes + 3072 + 2 * kTile * p.nt * 8 * 4);
+  const int x_bytes = kSmem - std::min(12, most) * (kStages * kStageBytes + 4096 + 2 * kTile * p.nt * 8 * 4);
   int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + x_bytes - 1) / x_bytes));
   if (tiles * p.passes < sms) slices = std::max<int64_t>(slices, std::min<int64_t>(chunks / 4, sms / (tiles * p.passes)));
   p.sh.slice_chunks = (chunks + slices - 1) / slices;
@@ -980,10 +1007,14 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
     }
   }
   p.sh.warp_chunks = (p.sh.slice_chunks + p.sh.along - 1) / p.sh.along;
-  // Slots: the tile at work and those that the copies may have reached.
-  const int pieces = p.scale ? (p.sh.warp_chunks * kBlocks - 1) / (w.group_blocks * 8) + 2 : 1;
-  p.sh.slot_bytes = kTile * (p.scale ? pieces | 1 : 1) * piece_bytes(p.scale);
-  p.sh.slots = p.scale ? 1 + (kStages - 1 + p.sh.warp_chunks - 1) / p.sh.warp_chunks : 2;
+  // Slots: the span at work and those that the copies, three chunks ahead, may have
+  // reached; a tile's first and last span may be short.
+  p.sh.span = w.group_blocks * ((3 + w.group_blocks) / w.group_blocks);
+  p.sh.pieces = p.sh.span / w.group_blocks;
+  p.sh.places = p.scale ? p.sh.pieces | 1 : 1;
+  p.sh.slot_bytes = kTile * p.sh.places * piece_bytes(p.scale);
+  const bool even = p.sh.warp_chunks % p.sh.span == 0 && p.sh.slice_chunks % p.sh.span == 0;
+  p.sh.slots = !p.scale || even ? 2 : 4;
   const int warp_bytes = kStages * kStageBytes + p.sh.slots * p.sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
   const int fit_warps = (kSmem - p.sh.slice_chunks * chunk_bytes) / warp_bytes;
   p.sh.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, fit_warps) / p.sh.along, (work + sms - 1) / sms));

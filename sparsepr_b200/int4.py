@@ -65,26 +65,32 @@ def dequantize_int4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Ten
     return w.view(n, -1)[:, :in_features].to(dtype)
 
 
+def _backward(ctx, dy):
+    packed, scales, zeros = ctx.saved_tensors
+    dx = dbias = None
+    if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
+        dy = dy.contiguous()
+    if ctx.needs_input_grad[0]:
+        dx = K.int4_linear_grad(dy, packed, scales, zeros, ctx.in_features)
+    if ctx.needs_input_grad[4]:
+        dbias = dy.sum(0)  # 16-bit sums are fp32 inside and rounded once
+    return dx, None, None, None, dbias
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _Int4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, packed, scales, zeros, bias):
         ctx.save_for_backward(packed, scales, zeros)
-        ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.in_features = x.shape[1]
         return K.int4_linear(x, packed, scales, zeros, bias)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        packed, scales, zeros = ctx.saved_tensors
-        dx = dbias = None
-        if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
-            dy = dy.contiguous()
-        if ctx.needs_input_grad[0]:
-            dx = K.int4_linear_grad(dy, packed, scales, zeros, ctx.in_features)
-        if ctx.needs_input_grad[4]:
-            dbias = dy.sum(0, dtype=torch.float32).to(ctx.bias_dtype)
-        return dx, None, None, None, dbias
+        # The wrapper that refuses second derivatives, where a graph of this pass is asked for.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dy)
 
 
 def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,

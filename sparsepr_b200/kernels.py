@@ -600,13 +600,8 @@ class AdalnOperands(NamedTuple):
                              *self.scale_strides, *self.gate_strides, z, h, mean, rstd)
 
 
-def adaln_forward(op: AdalnOperands, eps: float, stats: bool):
-    """Modulated layer norm of [batch][tokens][channels] rows with an optional gated residual
-    (``op.y``): ``z = x + gate*y``, ``h = LN(z)*(scale_offset + scale) + shift``.
-
-    :func:`sparsepr_b200.adaln.operands` makes ``op`` from checked tensors.  Returns
-    ``(z, h, stats)``: ``z`` and ``h`` dense in x's shape, ``z`` None without ``y``, and the row means and
-    reciprocal deviations fp32 [2, batch*tokens], None unless asked for."""
+def adaln_forward_struct(op: AdalnOperands, eps: float, stats: bool):
+    """:func:`adaln_forward` with the operands as the C ABI took them: ``(z, h, stats, struct)``."""
     x = op.x
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
     z = None if op.y is None else torch.empty_like(h)
@@ -619,7 +614,41 @@ def adaln_forward(op: AdalnOperands, eps: float, stats: bool):
     s = op.struct(eps, _p(z), h.data_ptr(), mean, rstd)
     _count(1)
     _launch(x.get_device(), "spr_adaln_forward", ctypes.addressof(s))
-    return z, h, st
+    return z, h, st, s
+
+
+def adaln_forward(op: AdalnOperands, eps: float, stats: bool):
+    """Modulated layer norm of [batch][tokens][channels] rows with an optional gated residual
+    (``op.y``): ``z = x + gate*y``, ``h = LN(z)*(scale_offset + scale) + shift``.
+
+    :func:`sparsepr_b200.adaln.operands` makes ``op`` from checked tensors.  Returns
+    ``(z, h, stats)``: ``z`` and ``h`` dense in x's shape, ``z`` None without ``y``, and the row means and
+    reciprocal deviations fp32 [2, batch*tokens], None unless asked for."""
+    return adaln_forward_struct(op, eps, stats)[:3]
+
+
+def adaln_backward_struct(s: _lib.SprAdaln, branch: bool, dh, dz, needs, mod_shape, vector_shape, mod_dtype):
+    """The backward pass of operands ``s`` whose ``x`` is the forward pass's ``z``; ``dh`` and ``dz`` dense."""
+    b, n, c = s.batch, s.tokens, s.channels
+    dx = torch.empty_like(dh)
+    dy = torch.empty_like(dh) if branch else None
+    new = dh.new_empty
+    dgate = new(vector_shape, dtype=mod_dtype) if needs[0] else None
+    dshift = new(vector_shape, dtype=mod_dtype) if needs[1] else None
+    dscale = new(vector_shape, dtype=mod_dtype) if needs[2] else None
+    if b * n == 0:
+        for t in (dgate, dshift, dscale):
+            if t is not None:
+                t.zero_()
+        return dx, dy, dgate, dshift, dscale
+    keep_b, keep_n = int(mod_shape[0] > 1), int(mod_shape[1] > 1)
+    gr = _lib.SprAdalnGrad(dh.data_ptr(), _p(dz), n * c, c, n * c, c, dx.data_ptr(), _p(dy), _p(dshift), _p(dscale),
+                           _p(dgate), keep_b, keep_n)
+    nbytes = _lib.query("spr_adaln_backward_workspace_bytes", b, n, c, keep_b, keep_n)
+    ws = new(nbytes, dtype=torch.uint8) if nbytes else None
+    _count(2 if nbytes else 1)
+    _launch(dh.get_device(), "spr_adaln_backward", ctypes.addressof(s), ctypes.addressof(gr), _p(ws), nbytes)
+    return dx, dy, dgate, dshift, dscale
 
 
 def adaln_backward(op: AdalnOperands, stats: torch.Tensor, dh, dz=None, needs=(True, True, True),
@@ -631,28 +660,9 @@ def adaln_backward(op: AdalnOperands, stats: torch.Tensor, dh, dz=None, needs=(T
     formed: [*mod_shape, channels] with ``mod_shape`` (batch or 1, tokens or 1), summed over the
     axes of extent 1 in a fixed order.  The workspace belongs to this call alone, so
     that calls on several streams and captured graphs share none."""
-    x = op.x
-    b, n, c = op.batch, op.tokens, op.channels
-    dx = torch.empty_like(dh)
-    dy = None if op.y is None else torch.empty_like(dh)
-    dgate, dshift, dscale = (x.new_empty((*mod_shape, c), dtype=op.mod_dtype) if need else None for need in needs)
-    rows = b * n
-    if rows == 0:
-        for t in (dgate, dshift, dscale):
-            if t is not None:
-                t.zero_()
-        return dx, dy, dgate, dshift, dscale
     mean = stats.data_ptr()
-    s = op.struct(0.0, None, None, mean, mean + 4 * rows)
-    keep_b, keep_n = int(mod_shape[0] > 1), int(mod_shape[1] > 1)
-    gr = _lib.SprAdalnGrad(dh.data_ptr(), _p(dz), n * c, c, n * c, c, dx.data_ptr(), _p(dy), _p(dshift), _p(dscale),
-                           _p(dgate), keep_b, keep_n)
-    index = x.get_device()
-    nbytes = _lib.query("spr_adaln_backward_workspace_bytes", b, n, c, keep_b, keep_n)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _count(2 if nbytes else 1)
-    _launch(index, "spr_adaln_backward", ctypes.addressof(s), ctypes.addressof(gr), _p(ws), nbytes)
-    return dx, dy, dgate, dshift, dscale
+    s = op.struct(0.0, None, None, mean, mean + 4 * op.batch * op.tokens)
+    return adaln_backward_struct(s, op.y is not None, dh, dz, needs, mod_shape, (*mod_shape, op.channels), op.mod_dtype)
 
 
 def _int4_checks(what, rows2d, length, packed, scales, zeros):

@@ -317,6 +317,9 @@ def test_empty_rows(cuda):
     assert h.shape == x.shape
     dx, dw = torch.autograd.grad(h, (x, w), torch.zeros_like(h))
     assert dx.shape == x.shape and torch.equal(dw, torch.zeros_like(w))
+    z, h = spr.gated_residual_layer_norm(x, x * 2, w, w, w)
+    dx, dw = torch.autograd.grad((z, h), (x, w), (torch.zeros_like(h),) * 2)
+    assert dx.shape == x.shape and torch.equal(dw, torch.zeros_like(w))
 
 
 @pytest.mark.gpu
@@ -340,6 +343,40 @@ def test_gradient_against_differences(cuda):
             diff = ((loss(hi) - loss(lo)) / (2 * step)).item()
         want = (grad.double() * d.double()).sum().item()
         assert abs(diff - want) <= 2e-3 * (grad.double().norm() * d.double().norm()).item(), (name, diff, want)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused_and_graphs_kept(cuda):
+    x = torch.randn(3, 40, device=cuda, requires_grad=True)
+    h = spr.layer_norm(x)
+    first, = torch.autograd.grad(h, x, torch.ones_like(h), retain_graph=True)
+    again, = torch.autograd.grad(h, x, torch.ones_like(h), retain_graph=True)  # the saved operands stay
+    assert torch.equal(first, again)
+    g, = torch.autograd.grad(h.square().sum(), x, create_graph=True)  # asking for a graph is no error by itself
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_saved_operands_may_be_moved(cuda):
+    """Hooks that keep saved tensors elsewhere give back other memory."""
+    v = _inputs(cuda, 1, 50, 256, BF, FP, "vector", seed=4)
+    leaves = [v[k].detach().requires_grad_() for k in ("x", "y", "gate", "shift", "scale")]
+
+    def grads():
+        z, h = spr.gated_residual_layer_norm(*leaves)
+        return torch.autograd.grad((z, h), leaves, (v["dz"], v["dh"]))
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    z, h = spr.gated_residual_layer_norm(*leaves)
+    with torch.no_grad():
+        z += 1.0  # the saved stream is the result itself
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, leaves[0], v["dh"])
 
 
 @pytest.mark.gpu
