@@ -831,6 +831,9 @@ int sm_count() {
   return sms[dev];
 }
 
+// Threads of a CTA that takes whole rows: whole warps.
+int cta_for(int vectors, int per) { return ((vectors + per - 1) / per + 31) / 32 * 32; }
+
 // Threads a row: a power of two of lanes up to a warp, whole warps above.
 int team_for(int vectors) {
   if (vectors > 32) return (vectors + 31) / 32 * 32;
@@ -975,7 +978,7 @@ template <typename T, typename MT, bool kRes, int P, bool kFull, int kThreads, i
 int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
   constexpr int kIn = kRes ? 2 : 1, kStages = ring_stages(kIn * P * kThreads * 16);
   auto kern = adaln_forward_stream_kernel<T, MT, P, kRes, kFull, kThreads, kMin, kStages>;
-  const int team = team_for((op->channels / kVec<T> + P - 1) / P);
+  const int team = cta_for(op->channels / kVec<T>, P);
   const int smem = kStages * kIn * P * team * 16;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * kIn * P * kThreads * 16) !=
       cudaSuccess)
@@ -988,8 +991,8 @@ int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
 
 // Whether P/2 vectors a thread leave fewer idle places in a CTA of at most 512.
 bool half_fits_better(int nvec, int P) {
-  const int half = team_for((nvec + P / 2 - 1) / (P / 2));
-  return half <= 512 && half * (P / 2) < team_for((nvec + P - 1) / P) * P;
+  const int half = cta_for(nvec, P / 2);
+  return half <= 512 && half * (P / 2) < cta_for(nvec, P) * P;
 }
 
 template <typename T, typename MT, bool kRes>
@@ -1036,7 +1039,7 @@ template <typename T, typename MT, bool kRes, int P, bool kFull, bool kAgain, in
 int launch_backward_stream(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, float* partial, cudaStream_t st) {
   constexpr int kIn = kRes ? 4 : 2, kStages = std::min(kRes ? 4 : 3, ring_stages(R * kIn * P * kThreads * 16));
   auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kFull, kAgain, R, kThreads, kStages>;
-  const int team = team_for((op->channels / kVec<T> + P - 1) / P);
+  const int team = cta_for(op->channels / kVec<T>, P);
   const int smem = kStages * R * kIn * P * team * 16;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * R * kIn * P * kThreads * 16) !=
       cudaSuccess)

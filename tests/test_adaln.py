@@ -208,6 +208,15 @@ BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
     (1, 700, 5120, BF, FP, "vector"),
     (3, 11, 4097, BF, BF, "sample"),
     (1, 9, 8192, FP, FP, "vector"),
+    (1, 50, 256, FP, FP, "vector"),
+    (2, 40, 132, FP, FP, "sample"),
+    (1, 90, 508, FP, FP, "vector"),
+    (1, 40, 384, FP, FP, "vector"),
+    (1, 60, 272, BF, FP, "vector"),
+    (2, 33, 6144, BF, BF, "sample"),
+    (1, 20, 5128, FP, FP, "vector"),
+    (1, 77, 8192, HF, FP, "vector"),
+    (3, 41, 8200, BF, BF, "vector"),
     (1, 5, 16384, BF, BF, "vector"),
     (1, 3, 16383, FP, FP, "sample"),
     (2, 4, 16384, FP, FP, "shared"),
