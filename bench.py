@@ -442,9 +442,11 @@ def run_dit(args):
         torch.cuda.set_device(local)
         dist.init_process_group("nccl", device_id=torch.device("cuda", local))
     dev = torch.device("cuda", local if world > 1 else 0)
-    cfg = HunyuanDiTConfig()
+    cfg = HunyuanDiTConfig(fused_adaln=args.fused_adaln, modulation_bits=args.modulation_bits)
     model = HunyuanDiT(cfg, dev, seed=0)  # same seed on every rank: same weights
     params = sum(w.numel() for w in _dit_tensors(model))
+    if model.mod4 is not None:
+        params += model.mod4[1].numel() * (cfg.hidden + 1)
     g = torch.Generator(device=dev).manual_seed(1)
     latent = torch.randn(cfg.in_channels, 33, 90, 160, device=dev, generator=g)
     text = torch.randn(256, cfg.text_dim, device=dev, generator=g)
@@ -484,6 +486,7 @@ def run_dit(args):
             "video_tokens": n_video, "text_tokens": 256, "heads": cfg.heads, "blocks": cfg.double_blocks + cfg.single_blocks,
             "params": params, "parallelism": f"video tokens sequence-sharded x{world} (Ulysses)" if world > 1 else "1 GPU",
             "sparsepr": "svg_ear_value, 200/1000 clusters, 10 Lloyd iterations, keep 30%, repair (64 probes, rank 16)",
+            "fused_adaln": cfg.fused_adaln, "modulation_bits": cfg.modulation_bits,
             "data": "random-init bf16 weights, latent ~ N(0,1), text ~ N(0,1)", "out_tokens_per_rank": int(out.shape[0]),
             "timing": "eager, CUDA events, max over ranks", "steps": steps, "clocks": clocks.summary()}}), flush=True)
     if world > 1:
@@ -502,7 +505,7 @@ def _dit_tensors(model):
                 yield from walk(y)
 
     for name, val in vars(model).items():
-        if name not in ("cfg", "device", "dtype"):
+        if name not in ("cfg", "device", "dtype", "mod4"):
             yield from walk(val)
 
 
@@ -663,6 +666,10 @@ def main():
                     help="(torchrun, N > 1) time the sequence-sharded Ulysses variant instead of the bench line")
     ap.add_argument("--route-reuse", action="store_true",
                     help="time a refreshed and a cached-route (temporal reuse) layer call instead of the bench line")
+    ap.add_argument("--fused-adaln", action="store_true",
+                    help="with --config 4: norms, modulations and gated residuals of the DiT as fused passes")
+    ap.add_argument("--modulation-bits", type=int, default=16, choices=(4, 16),
+                    help="with --config 4: bits of the DiT's modulation weights")
     ap.add_argument("--kernel-table", action="store_true",
                     help="print per-kernel device times of one layer (torch profiler) instead of the bench line")
     args = ap.parse_args()

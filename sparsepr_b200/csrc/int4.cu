@@ -966,10 +966,10 @@ struct ForwardPlan {
 };
 
 // Rows a pass: what 32 columns of a product hold.  16-bit rows go to the integer
-// products while one pass holds them; more of them take fewer columns as bf16 parts
-// (of measured bandwidth at 122,880 x 5120, group 64: see launch_forward).  The columns
-// of the weight are cut into slices where the staged rows would leave no room for the
-// rings of twelve warps (eight of the widest products), and where too few tiles would leave SMs without work.
+// products while one pass holds them; more of them take fewer columns as bf16 parts.
+// The rest weighs, by estimates of the time: slices of the weight's columns (each CTA
+// then stages less of x, which leaves room for more warps, but the slices' sums have to
+// be joined) against warps on a tile (idle warps at the last round, and sums to join).
 ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   ForwardPlan p{};
   p.ints = dtype != SPR_F32 && rows <= 32 / kLimbs;
@@ -979,50 +979,56 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   const int cols = p.pass_rows * p.parts;
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.gb = w.group_blocks % 8 == 0 ? 8 : w.group_blocks % 4 == 0 ? 4 : w.group_blocks % 2 == 0 ? 2 : 1;
-  const int chunks = (w.blocks + kBlocks - 1) / kBlocks;
-  const int64_t tiles = (w.n + kTile - 1) / kTile;
-  const int chunk_bytes = kBlocks * (p.ints ? cols * 32 + p.nt * 32 : cols * 64);
-  const int64_t sms = sm_count();
-  const int most = most_warps(p.nt);
   // Pieces of eight scales, whole and aligned, and groups that a chunk does not straddle.
   p.scale = w.groups % 8 == 0 && (kBlocks % w.group_blocks == 0 || w.group_blocks % kBlocks == 0) &&
                     aligned(w.scales, 16) && aligned(w.zeros, 8)
                 ? dtype_bytes(w.scale_dtype)
                 : 0;
-  const int x_bytes = kSmem - std::min(12, most) * (kStages * kStageBytes + 4096 + 2 * kTile * p.nt * 8 * 4);
-  int slices = std::max(1, (int)(((int64_t)chunks * chunk_bytes + x_bytes - 1) / x_bytes));
-  if (tiles * p.passes < sms) slices = std::max<int64_t>(slices, std::min<int64_t>(chunks / 4, sms / (tiles * p.passes)));
-  p.sh.slice_chunks = (chunks + slices - 1) / slices;
-  p.sh.slices = (chunks + p.sh.slice_chunks - 1) / p.sh.slice_chunks;
-  // Warps on a tile: few, so that the sums they join cost little, but so that neither
-  // the tiles over all teams nor the chunks over a team's warps leave many idle.
-  const int64_t work = tiles * p.passes * p.sh.slices;
-  double best = 0;
-  for (int a = 1; a <= std::min(8, most) && a <= p.sh.slice_chunks; a *= 2) {
-    const double teams = (double)(most / a * sms), share = work / teams, steps = (double)p.sh.slice_chunks / a;
-    const double busy = share / ceil(share) * steps / ceil(steps);
-    if (busy > best * 1.04) {
-      best = busy;
-      p.sh.along = a;
+  Shape& sh = p.sh;
+  sh.span = w.group_blocks * ((3 + w.group_blocks) / w.group_blocks);
+  sh.pieces = sh.span / w.group_blocks;
+  sh.places = p.scale ? sh.pieces | 1 : 1;
+  sh.slot_bytes = kTile * sh.places * piece_bytes(p.scale);
+
+  const int chunks = (w.blocks + kBlocks - 1) / kBlocks;
+  const int64_t tiles = (w.n + kTile - 1) / kTile, sms = sm_count();
+  const int chunk_bytes = kBlocks * (p.ints ? cols * 32 + p.nt * 32 : cols * 64);
+  const int warp_most = kStages * kStageBytes + 4 * sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
+  const int least = std::max(1, (int)(((int64_t)chunks * chunk_bytes + kSmem - 8 * warp_most - 1) /
+                                      (kSmem - 8 * warp_most)));  // slices that leave room for eight warps
+  double best = 1e30;
+  for (int slices = least; slices <= std::min(chunks, 2 * least + 3); ++slices) {
+    const int slice_chunks = (chunks + slices - 1) / slices;
+    if ((chunks + slice_chunks - 1) / slice_chunks != slices) continue;
+    const int64_t work = tiles * p.passes * slices;
+    for (int along = 1; along <= 8 && along <= slice_chunks; along *= 2) {
+      const int warp_chunks = (slice_chunks + along - 1) / along;
+      // The span at work and those that the copies, three chunks ahead, may have reached;
+      // a tile's first and last span may be short.
+      const int slots = !p.scale || (warp_chunks % sh.span == 0 && slice_chunks % sh.span == 0) ? 2 : 4;
+      const int warp_bytes = kStages * kStageBytes + slots * sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
+      const int fit = std::min(most_warps(p.nt), (kSmem - slice_chunks * chunk_bytes) / warp_bytes);
+      const int64_t team_tiles = std::min<int64_t>(fit / along, (work + sms - 1) / sms);
+      if (team_tiles < 1) continue;
+      // Microseconds: a chunk of a warp (more where many warps share the schedulers), a
+      // round's end, the join.
+      const int64_t rounds = (work + team_tiles * sms - 1) / (team_tiles * sms);
+      const double chunk = (p.ints ? 0.7 : 0.9) * (1 + 0.25 * (p.nt - 1)) * std::max(1.0, along * team_tiles / 12.0);
+      const double time = rounds * (warp_chunks * chunk + 0.5) +
+                          (slices > 1 ? 3 + slices * (double)rows * (double)w.n * 8 / 5e6 : 0);
+      if (time >= best * 0.98) continue;
+      best = time;
+      sh.along = along;
+      sh.tiles = (int)team_tiles;
+      sh.warp_chunks = warp_chunks;
+      sh.slice_chunks = slice_chunks;
+      sh.slices = slices;
+      sh.slots = slots;
+      p.smem = along * (int)team_tiles * warp_bytes + slice_chunks * chunk_bytes;
     }
   }
-  p.sh.warp_chunks = (p.sh.slice_chunks + p.sh.along - 1) / p.sh.along;
-  // Slots: the span at work and those that the copies, three chunks ahead, may have
-  // reached; a tile's first and last span may be short.
-  p.sh.span = w.group_blocks * ((3 + w.group_blocks) / w.group_blocks);
-  p.sh.pieces = p.sh.span / w.group_blocks;
-  p.sh.places = p.scale ? p.sh.pieces | 1 : 1;
-  p.sh.slot_bytes = kTile * p.sh.places * piece_bytes(p.scale);
-  const bool even = p.sh.warp_chunks % p.sh.span == 0 && p.sh.slice_chunks % p.sh.span == 0;
-  p.sh.slots = !p.scale || even ? 2 : 4;
-  const int warp_bytes = kStages * kStageBytes + p.sh.slots * p.sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
-  const int fit_warps = (kSmem - p.sh.slice_chunks * chunk_bytes) / warp_bytes;
-  p.sh.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(most, fit_warps) / p.sh.along, (work + sms - 1) / sms));
-  const int warps = p.sh.along * p.sh.tiles;
-  p.smem = warps * warp_bytes + p.sh.slice_chunks * chunk_bytes;
-  const int64_t teams = (tiles + p.sh.tiles - 1) / p.sh.tiles;
-  const int64_t fit = std::max(1, std::min(227 * 1024 / (p.smem + 2048), 16 / warps));  // 128 registers a thread
-  p.grid = (int)std::min(teams, std::max<int64_t>(1, sms * fit / (p.passes * p.sh.slices)));
+  const int64_t teams = (tiles + sh.tiles - 1) / sh.tiles;
+  p.grid = (int)std::min(teams, std::max<int64_t>(1, sms / (p.passes * sh.slices)));
   return p;
 }
 

@@ -29,6 +29,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from .adaln import gated_residual_layer_norm, modulated_layer_norm
+
 __all__ = ["HunyuanDiTConfig", "HunyuanDiT", "JointAttention", "SparsePRBlocks", "rope_3d"]
 
 
@@ -46,12 +48,20 @@ class HunyuanDiTConfig:
     vec_dim: int = 768
     rope_axes: tuple = (16, 56, 56)
     rope_theta: float = 256.0
+    # CUDA only: the norms, modulations and gated residuals as one pass each
+    # (sparsepr_b200.adaln) instead of one tensor operation after the other, and the
+    # modulation weights in 4 bits under group scales, all blocks' in one product.
+    fused_adaln: bool = False
+    modulation_bits: int = 16
+    modulation_group: int = 64
 
     def validate(self) -> None:
         if self.heads * self.head_dim != self.hidden:
             raise ValueError(f"heads x head_dim = {self.heads * self.head_dim} must equal hidden {self.hidden}.")
         if sum(self.rope_axes) != self.head_dim or any(a % 2 for a in self.rope_axes):
             raise ValueError(f"rope axes {self.rope_axes} must be even and sum to head_dim {self.head_dim}.")
+        if self.modulation_bits not in (4, 16):
+            raise ValueError(f"modulation_bits must be 4 or 16, got {self.modulation_bits}.")
 
 
 def rope_3d(grid, positions, axes, theta, device):
@@ -121,6 +131,8 @@ class HunyuanDiT:
 
     def __init__(self, config: HunyuanDiTConfig, device, dtype=torch.bfloat16, seed: int = 0):
         config.validate()
+        if (config.fused_adaln or config.modulation_bits == 4) and torch.device(device).type != "cuda":
+            raise ValueError(f"fused_adaln and 4-bit modulation run on CUDA devices, got {device}.")
         self.cfg = config
         self.device, self.dtype = device, dtype
         g = torch.Generator(device=device).manual_seed(seed)
@@ -145,6 +157,7 @@ class HunyuanDiT:
                        for _ in range(config.single_blocks)]
         self.final_mod = W.linear(2 * c, c)
         self.final = W.linear(config.in_channels * pv, c)
+        self.mod4 = self._quantise_modulation() if config.modulation_bits == 4 else None
 
     # -- pieces ------------------------------------------------------------------
     @staticmethod
@@ -160,6 +173,58 @@ class HunyuanDiT:
         c, t, h, w = latent.shape
         x = latent.reshape(c, t // pt, pt, h // ph, ph, w // pw, pw).permute(1, 3, 5, 0, 2, 4, 6)
         return x.reshape((t // pt) * (h // ph) * (w // pw), c * pt * ph * pw), (t // pt, h // ph, w // pw)
+
+    def _modulation_layers(self):
+        """Every modulation layer's (rows, owner, key) in the order of the blocks: a double
+        block's video and text ones, the single blocks', the output layer's."""
+        for blk in self.double:
+            for s in ("img", "txt"):
+                yield blk[s], "mod"
+        for blk in self.single:
+            yield blk, "mod"
+        yield self.__dict__, "final_mod"
+
+    def _quantise_modulation(self):
+        """One stacked 4-bit weight in place of the modulation layers' own, and their biases."""
+        from .int4 import Int4Weight, quantize_int4
+
+        parts, biases = [], []
+        for owner, key in self._modulation_layers():
+            w, b = owner[key]
+            parts.append(quantize_int4(w, self.cfg.modulation_group))
+            biases.append(b)
+            owner[key] = None  # the 16-bit weight is not kept
+        return Int4Weight(*(torch.cat(t) for t in zip(*parts))), torch.cat(biases)
+
+    def _modulations(self, svec):
+        """Per double block {stream: (shift, scale, gate) of the attention and of the MLP},
+        per single block (shift, scale, gate), and the output layer's (shift, scale)."""
+        c = self.cfg.hidden
+        if self.mod4 is not None:
+            from .int4 import int4_linear
+
+            weight, bias = self.mod4
+            rows = int4_linear(svec.view(1, -1), *weight, bias).view(-1, c).unbind(0)
+            nd, ns = len(self.double), len(self.single)
+            double = [{"img": rows[12 * i:12 * i + 6], "txt": rows[12 * i + 6:12 * i + 12]} for i in range(nd)]
+            single = [rows[12 * nd + 3 * j:12 * nd + 3 * j + 3] for j in range(ns)]
+            return double, single, rows[12 * nd + 3 * ns:]
+        return ([{s: self._lin(svec, blk[s]["mod"]).chunk(6) for s in ("img", "txt")} for blk in self.double],
+                [self._lin(svec, blk["mod"]).chunk(3) for blk in self.single],
+                self._lin(svec, self.final_mod).chunk(2))
+
+    def _norm(self, x, shift, scale):
+        """The modulated norm in front of a branch."""
+        if self.cfg.fused_adaln:
+            return modulated_layer_norm(x, shift, scale, eps=1e-6)
+        return _modulate(_ln(x), shift, scale)
+
+    def _residual_norm(self, x, branch, gate, shift, scale):
+        """The end of a branch and the norm in front of the next one."""
+        if self.cfg.fused_adaln:
+            return gated_residual_layer_norm(x, branch, gate, shift, scale, eps=1e-6)
+        x = x + gate * branch
+        return x, _modulate(_ln(x), shift, scale)
 
     # -- forward -------------------------------------------------------------------
     def forward(self, latent, text, t, pooled, guidance, attention, rank: int = 0, world: int = 1):
@@ -177,43 +242,43 @@ class HunyuanDiT:
                + self._mlp2(_timestep_embedding(guidance.view(1)).to(self.dtype), self.guid_in)
                + self._mlp2(pooled.to(self.dtype).view(1, -1), self.vec_in)).view(-1)
         svec = F.silu(vec)
-        nt = txt.shape[0]
+        double, single, final = self._modulations(svec)
+        after = [*double, {"img": single[0], "txt": single[0]} if single else {"img": final, "txt": final}]
+        x = {"img": img, "txt": txt}
+        h = {s: self._norm(x[s], *after[0][s][:2]) for s in x}
         for i, blk in enumerate(self.double):
-            mods = {s: self._lin(svec, blk[s]["mod"]).chunk(6) for s in ("img", "txt")}
             qkv = {}
-            for s, x in (("img", img), ("txt", txt)):
-                sh1, sc1 = mods[s][0], mods[s][1]
-                h = self._lin(_modulate(_ln(x), sh1, sc1), blk[s]["qkv"])
-                q, k, v = h.view(x.shape[0], 3, cfg.heads, cfg.head_dim).unbind(1)
+            for s in x:
+                q, k, v = self._lin(h[s], blk[s]["qkv"]).view(x[s].shape[0], 3, cfg.heads, cfg.head_dim).unbind(1)
                 q, k = _rms(q, blk[s]["qn"]), _rms(k, blk[s]["kn"])
                 if s == "img":
                     q, k = _apply_rope(q, cos, sin), _apply_rope(k, cos, sin)
                 qkv[s] = (q, k, v)
             o_img, o_txt = attention(i, *qkv["img"], *qkv["txt"])
-            outs = {"img": o_img, "txt": o_txt}
-            new = {}
-            for s, x in (("img", img), ("txt", txt)):
-                sh1, sc1, g1, sh2, sc2, g2 = mods[s]
-                x = x + g1 * self._lin(outs[s].reshape(x.shape[0], cfg.hidden), blk[s]["proj"])
-                h = self._lin(_modulate(_ln(x), sh2, sc2), blk[s]["fc1"])
-                new[s] = x + g2 * self._lin(F.gelu(h, approximate="tanh"), blk[s]["fc2"])
-            img, txt = new["img"], new["txt"]
+            for s, o in (("img", o_img), ("txt", o_txt)):
+                _, _, g1, sh2, sc2, g2 = double[i][s]
+                branch = self._lin(o.reshape(x[s].shape[0], cfg.hidden), blk[s]["proj"])
+                x[s], m = self._residual_norm(x[s], branch, g1, sh2, sc2)
+                branch = self._lin(F.gelu(self._lin(m, blk[s]["fc1"]), approximate="tanh"), blk[s]["fc2"])
+                x[s], h[s] = self._residual_norm(x[s], branch, g2, *after[i + 1][s][:2])
+        if not self.single:
+            return self._lin(h["img"], self.final)
         mlp = int(cfg.hidden * cfg.mlp_ratio)
+        x, h = torch.cat((x["img"], x["txt"]), dim=0), torch.cat((h["img"], h["txt"]), dim=0)
         for j, blk in enumerate(self.single):
-            sh, sc, g = self._lin(svec, blk["mod"]).chunk(3)
-            x = torch.cat((img, txt), dim=0)
-            h = self._lin(_modulate(_ln(x), sh, sc), blk["lin1"])
-            qkv, m = h.split((3 * cfg.hidden, mlp), dim=-1)
+            qkv, m = self._lin(h, blk["lin1"]).split((3 * cfg.hidden, mlp), dim=-1)
             q, k, v = qkv.view(x.shape[0], 3, cfg.heads, cfg.head_dim).unbind(1)
             q, k = _rms(q, blk["qn"]), _rms(k, blk["kn"])
             q = torch.cat((_apply_rope(q[:ns], cos, sin), q[ns:]))
             k = torch.cat((_apply_rope(k[:ns], cos, sin), k[ns:]))
             o_img, o_txt = attention(len(self.double) + j, q[:ns], k[:ns], v[:ns], q[ns:], k[ns:], v[ns:])
             o = torch.cat((o_img, o_txt), dim=0).reshape(x.shape[0], cfg.hidden)
-            x = x + g * self._lin(torch.cat((o, F.gelu(m, approximate="tanh")), dim=-1), blk["lin2"])
-            img, txt = x[:ns], x[ns:]
-        sh, sc = self._lin(svec, self.final_mod).chunk(2)
-        return self._lin(_modulate(_ln(img), sh, sc), self.final)
+            branch = self._lin(torch.cat((o, F.gelu(m, approximate="tanh")), dim=-1), blk["lin2"])
+            last = j + 1 == len(self.single)
+            if last:  # the output layer takes the video tokens alone
+                x, branch = x[:ns], branch[:ns]
+            x, h = self._residual_norm(x, branch, single[j][2], *(final if last else single[j + 1][:2]))
+        return self._lin(h, self.final)
 
 
 class JointAttention:
