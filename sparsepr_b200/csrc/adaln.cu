@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
 // (512 threads have 128 registers each; held, they spill).
 constexpr int kStatRows = 256;  // rows whose statistics are in shared memory at a time
 template <typename T, typename MT, int P, bool kRes, bool kFull, bool kAgain, int R, int kThreads, int kStages>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1)
 adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups gp, float* partial) {
   constexpr int V = kVec<T>, kIn = kRes ? 4 : 2, e = sizeof(T);
   __shared__ uint64_t red[2][R][16];
@@ -1004,6 +1004,13 @@ int launch_forward(const SprAdaln* op, cudaStream_t st) {
                                kept(op->scale_st, op->shift_st, op->gate_st));
   constexpr int P = 16 / kVec<T>;  // 16 values a thread, or 8 where that leaves fewer threads idle
   if (vec && nvec > 32 && nvec <= 512 * P && g.rows >= 8 && even_rows(g, op->batch)) {
+    // 32 values a thread from 128 threads on: fewer warps pay a row's fixed instructions,
+    // which bound the pass at the clocks of a sustained load (75,600 x 5120 bf16: 271 us
+    // with 16 values, 250 us with 32).  With a branch the vectors leave no room for that
+    // (490 and 513 us).
+    if constexpr (!kRes)
+      if (nvec % (64 * P) == 0 && nvec >= 256 * P && nvec <= 320 * P)
+        return launch_forward_stream<T, MT, false, 2 * P, true, 160, 3>(op, g, st);
     if (nvec % (32 * P) == 0)
       return nvec <= 320 * P ? launch_forward_stream<T, MT, kRes, P, true, 320, 2>(op, g, st)
                              : launch_forward_stream<T, MT, kRes, P, true, 512, 1>(op, g, st);

@@ -307,7 +307,7 @@ __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int 
 // y for up to NT*8 columns (a row's parts or bytes each one): warp products of 16 weight
 // rows by 32 columns of the weight a step.
 template <int NT, int GB, bool kInt, int kScale>
-__global__ void __launch_bounds__(most_warps(NT) * 32)
+__global__ void __launch_bounds__(most_warps(NT) * 32, 1)
 int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, float up, const void* bias, void* y,
                    float* partial) {
   constexpr int U = GB < 4 ? GB : 4, kUnits = GB / U;  // a unit's blocks, a segment's units
@@ -348,18 +348,21 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   // A span's chunks lie between multiples of its length; the first of a tile may start within.
   const int lead = kScale ? from_chunk % sh.span : 0;
   const uint32_t inv_pieces = kScale ? (65536 + sh.pieces - 1) / sh.pieces : 0;  // i / pieces for i below 16*pieces
-  const uint8_t* from[kTile / 4];  // the lane's 16 bytes of rows lane/8 + 4i, in the chunk to copy
+  const uint8_t* from = nullptr;  // the tile's first row, in the chunk to copy
+  uint32_t row_at[kTile / 4];     // the lane's 16 bytes of rows lane/8 + 4i
   auto aim = [&]() {
+    const int64_t n = (int64_t)copy.tile * kTile;
+    from = w.packed + n * pitch + from_chunk * (kBlocks * 16);
+    const int last = (int)min((int64_t)kTile, w.n - n) - 1;  // past the last row: that one again
 #pragma unroll
     for (int i = 0; i < kTile / 4; ++i)
-      from[i] = w.packed + min((int64_t)copy.tile * kTile + i * 4 + (lane >> 3), w.n - 1) * pitch + (lane & 7) * 16 +
-                from_chunk * (kBlocks * 16);
+      row_at[i] = (uint32_t)min(i * 4 + (lane >> 3), last) * (uint32_t)pitch + (lane & 7) * 16;
   };
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), slot_at = (uint32_t)__cvta_generic_to_shared(slots);
   uint32_t to[kTile / 4];
 #pragma unroll
   for (int i = 0; i < kTile / 4; ++i) to[i] = ring_at + piece(i * 4 + (lane >> 3), lane & 7);
-  aim();
+  if (copy.tile < tiles) aim();
   int copy_slot = 0, use_slot = 0, copy_at = lead, use_at = lead;  // chunks from the span's start
   auto copy_scales = [&]() {
     const uint32_t dst = slot_at + copy_slot * sh.slot_bytes, dst_zero = dst + kTile * sh.places * 8 * kScale;
@@ -383,14 +386,13 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
       if (copy.chunk * kBlocks + (lane & 7) < w.blocks && copy.chunk < to_chunk)
 #pragma unroll
         for (int i = 0; i < kTile / 4; ++i)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kStageBytes), "l"(from[i])
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to[i] + stage * kStageBytes), "l"(from + row_at[i])
                        : "memory");
       if (kScale && (copy.chunk == from_chunk || copy_at == 0) && copy.chunk < to_chunk) copy_scales();
-#pragma unroll
-      for (int i = 0; i < kTile / 4; ++i) from[i] += kBlocks * 16;
+      from += kBlocks * 16;
       copy_at = copy_at + 1 == sh.span ? 0 : copy_at + 1;
       if (next(copy)) {
-        aim();
+        if (copy.tile < tiles) aim();
         copy_at = lead;
       }
     }
@@ -927,7 +929,7 @@ int check_int4(const char* what, int64_t stride, int dtype, int64_t rows, int64_
                int group, const void* packed, int scale_dtype) {
   if (rows < 0 || n < 0 || k < 1)
     return fail(SPR_ERR_SHAPE, "%s: rows=%lld n=%lld k=%lld", what, (long long)rows, (long long)n, (long long)k);
-  if (rows > 65535 || n > 0x7fffffffLL || k > 0x7fffffffLL - (1 << 20))
+  if (rows > 65535 || n > 0x7fffffffLL || k > (1 << 27))
     return fail(SPR_ERR_SHAPE, "%s: rows=%lld n=%lld k=%lld too large", what, (long long)rows, (long long)n,
                 (long long)k);
   if (group < 32 || group % 32 || group > (1 << 20))
