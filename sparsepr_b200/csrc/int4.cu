@@ -347,9 +347,18 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
 
   // A span's chunks lie between multiples of its length; the first of a tile may start within.
   const int lead = kScale ? from_chunk % sh.span : 0;
-  const uint32_t inv_pieces = kScale ? (65536 + sh.pieces - 1) / sh.pieces : 0;  // i / pieces for i below 16*pieces
+  const int span_chunks = GB < 8 ? GB : w.group_blocks;  // of a piece
   const uint8_t* from = nullptr;  // the tile's first row, in the chunk to copy
   uint32_t row_at[kTile / 4];     // the lane's 16 bytes of rows lane/8 + 4i
+  // A lane's pieces of a span: piece_row[j] of the tile, pieces side by side in neighbouring
+  // lanes.  Byte offsets from the tile's first row, for scales of one byte.
+  constexpr int kPieces = GB < 4 ? 4 / GB : 1, kCopies = (kTile * kPieces + 31) / 32;
+  uint32_t piece_at[kCopies];
+  auto aim_scales = [&](int last) {
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j)
+      piece_at[j] = (uint32_t)min((lane + 32 * j) / kPieces, last) * (uint32_t)w.groups + (lane + 32 * j) % kPieces * 8;
+  };
   auto aim = [&]() {
     const int64_t n = (int64_t)copy.tile * kTile;
     from = w.packed + n * pitch + from_chunk * (kBlocks * 16);
@@ -357,6 +366,7 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
 #pragma unroll
     for (int i = 0; i < kTile / 4; ++i)
       row_at[i] = (uint32_t)min(i * 4 + (lane >> 3), last) * (uint32_t)pitch + (lane & 7) * 16;
+    if constexpr (kScale != 0) aim_scales(last);
   };
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), slot_at = (uint32_t)__cvta_generic_to_shared(slots);
   uint32_t to[kTile / 4];
@@ -367,18 +377,21 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   auto copy_scales = [&]() {
     const uint32_t dst = slot_at + copy_slot * sh.slot_bytes, dst_zero = dst + kTile * sh.places * 8 * kScale;
     copy_slot = copy_slot + 1 == sh.slots ? 0 : copy_slot + 1;
-    const int first = (copy.chunk - copy_at) / w.group_blocks;  // piece: eight groups of group_blocks/8 chunks
-    for (int i = lane; i < kTile * sh.pieces; i += 32) {
-      const int row = i * inv_pieces >> 16, p = i - row * sh.pieces;
-      const int64_t g = min((int64_t)copy.tile * kTile + row, w.n - 1) * w.groups + min(first + p, w.groups / 8 - 1) * 8;
-      const int place = row * sh.places + p;
+    const int first = (copy.chunk - copy_at) / span_chunks;  // piece: eight groups, of group_blocks chunks
+    const char* scales = (const char*)w.scales + ((int64_t)copy.tile * kTile * w.groups + first * 8) * kScale;
+    const uint8_t* zeros = w.zeros + (int64_t)copy.tile * kTile * w.groups + first * 8;
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j) {
+      const int p = (lane + 32 * j) % kPieces, place = (lane + 32 * j) / kPieces * sh.places + p;
+      if ((kTile * kPieces < 32 && lane >= kTile * kPieces) || (first + p) * 8 >= w.groups) continue;
 #pragma unroll
       for (int h = 0; h < kScale / 2; ++h)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + place * 8 * kScale + h * 16),
-                     "l"((const char*)w.scales + g * kScale + h * 16)
+                     "l"(scales + piece_at[j] * (uint32_t)kScale + h * 16)
                      : "memory");
       if (w.zeros)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst_zero + place * 8), "l"(w.zeros + g) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst_zero + place * 8), "l"(zeros + piece_at[j])
+                     : "memory");
     }
   };
   auto fetch = [&](int stage) {
@@ -967,12 +980,19 @@ struct ForwardPlan {
   int parts, pass_rows, passes, nt, gb, grid, smem;
 };
 
+// Bytes of a scale that can be copied ahead: pieces of eight, whole and aligned, and
+// groups that a chunk does not straddle; else 0.
+int scale_ahead(const Weights& w) {
+  const bool whole = w.groups % 8 == 0 && (kBlocks % w.group_blocks == 0 || w.group_blocks % kBlocks == 0);
+  return whole && aligned(w.scales, 16) && aligned(w.zeros, 8) ? dtype_bytes(w.scale_dtype) : 0;
+}
+
 // Rows a pass: what 32 columns of a product hold.  16-bit rows go to the integer
 // products while one pass holds them; more of them take fewer columns as bf16 parts.
 // The rest weighs, by estimates of the time: slices of the weight's columns (each CTA
 // then stages less of x, which leaves room for more warps, but the slices' sums have to
 // be joined) against warps on a tile (idle warps at the last round, and sums to join).
-ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
+ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype, int scale) {
   ForwardPlan p{};
   p.ints = dtype != SPR_F32 && rows <= 32 / kLimbs;
   p.parts = p.ints ? kLimbs : parts_of(dtype);
@@ -981,11 +1001,7 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
   const int cols = p.pass_rows * p.parts;
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.gb = w.group_blocks % 8 == 0 ? 8 : w.group_blocks % 4 == 0 ? 4 : w.group_blocks % 2 == 0 ? 2 : 1;
-  // Pieces of eight scales, whole and aligned, and groups that a chunk does not straddle.
-  p.scale = w.groups % 8 == 0 && (kBlocks % w.group_blocks == 0 || w.group_blocks % kBlocks == 0) &&
-                    aligned(w.scales, 16) && aligned(w.zeros, 8)
-                ? dtype_bytes(w.scale_dtype)
-                : 0;
+  p.scale = scale;
   Shape& sh = p.sh;
   sh.span = w.group_blocks * ((3 + w.group_blocks) / w.group_blocks);
   sh.pieces = sh.span / w.group_blocks;
@@ -1013,10 +1029,10 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype) {
       const int64_t team_tiles = std::min<int64_t>(fit / along, (work + sms - 1) / sms);
       if (team_tiles < 1) continue;
       // Microseconds: a chunk of a warp (more where many warps share the schedulers), a
-      // round's end, the join.
+      // round's end (with a wait for the tile's other warps), the join.
       const int64_t rounds = (work + team_tiles * sms - 1) / (team_tiles * sms);
       const double chunk = (p.ints ? 0.7 : 0.9) * (1 + 0.25 * (p.nt - 1)) * std::max(1.0, along * team_tiles / 12.0);
-      const double time = rounds * (warp_chunks * chunk + 0.5) +
+      const double time = rounds * (warp_chunks * chunk + (along > 1 ? 1.5 : 0.3)) +
                           (slices > 1 ? 3 + slices * (double)rows * (double)w.n * 8 / 5e6 : 0);
       if (time >= best * 0.98) continue;
       best = time;
@@ -1129,8 +1145,13 @@ using namespace spr;
 
 extern "C" size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype) {
   if (rows <= 0 || n <= 0 || k <= 0 || group < 32) return 0;
-  const ForwardPlan p = plan_forward(rows, make_weights(nullptr, nullptr, 0, nullptr, n, k, group), dtype);
-  return p.sh.slices > 1 ? (size_t)p.sh.slices * rows * n * sizeof(float) : 0;
+  const Weights w = make_weights(nullptr, nullptr, 0, nullptr, n, k, group);
+  size_t most = 0;
+  for (int scale : {0, 2, 4}) {  // whatever the scales' type and alignment will be
+    const ForwardPlan p = plan_forward(rows, w, dtype, scale);
+    if (p.sh.slices > 1) most = std::max(most, (size_t)p.sh.slices * rows * n * sizeof(float));
+  }
+  return most;
 }
 
 extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64_t rows, int64_t n, int64_t k,
@@ -1141,7 +1162,7 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
   if (rows == 0 || n == 0) return SPR_OK;
   if (!x || !packed || !scales || !y) return fail(SPR_ERR_ARG, "int4 linear: null operand");
   const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
-  const ForwardPlan p = plan_forward(rows, w, dtype);
+  const ForwardPlan p = plan_forward(rows, w, dtype, scale_ahead(w));
   const size_t need = p.sh.slices > 1 ? (size_t)p.sh.slices * rows * n * sizeof(float) : 0;
   if (need && (!workspace || workspace_bytes < need))
     return fail(SPR_ERR_WORKSPACE, "int4 linear: workspace %zu < %zu bytes", workspace_bytes, need);
