@@ -110,8 +110,9 @@ def operands(x, y, gate, shift, scale, scale_offset: float = 1.0):
         b, n, keep_b, keep_n = 1, x.numel() // c, False, False
     else:
         b, n, keep_b, keep_n = _split(shape, first.shape, first_name)
-    if b == 1 and not keep_n and not (x.is_contiguous() and (y is None or y.is_contiguous())) and len(shape) > 2:
-        b, n = math.prod(shape[:-2]), shape[-2]  # one vector for all rows: any two runs of x's axes will do
+    if b == 1 and len(shape) > 2 and not all(t is None or t.is_contiguous() for t in (x, y, gate, shift, scale)):
+        # One vector for all rows, or one for each: any two runs of x's axes will do.
+        b, n, keep_b = math.prod(shape[:-2]), shape[-2], keep_n
     mb, mn = (b if keep_b else 1), (n if keep_n else 1)
     op = K.AdalnOperands(x, y, gate, shift, scale, b, n, c, _strides(x, b, n, "x"),
                          _NONE if y is None else _strides(y, b, n, "y"),

@@ -5,6 +5,8 @@
 //   dshift = sum dh,  dscale = sum dh*n,  dgate = sum g*y   over the rows of a group
 // Statistics and sums are fp32.
 #include <atomic>
+#include <tuple>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -366,14 +368,76 @@ struct Run {
   }
 };
 
+// Vectors of a row's own (scale, shift, gate) in a ring beside the rows: of M bytes an
+// element, kM 16-byte pieces for a vector of the row's elements.
+template <typename T, typename MT>
+constexpr int row_pieces = kVec<T> * (int)sizeof(MT) / 16;
+enum Vector { kScaleVector, kShiftVector, kGateVector };
+template <typename T, typename MT, int P, bool kRow, Vector... kWhich>
+struct RowVectors {
+  static constexpr int kM = row_pieces<T, MT>, kVectors = sizeof...(kWhich);
+  const char* at[kVectors];
+  int64_t step[kVectors];
+  __device__ __forceinline__ RowVectors(const SprAdaln& op, const Run& run) {
+    if constexpr (kRow) {
+      constexpr Vector which[kVectors] = {kWhich...};
+      const void* base[3] = {op.scale, op.shift, op.gate};
+      const int64_t sb[3] = {op.scale_sb, op.shift_sb, op.gate_sb}, st[3] = {op.scale_st, op.shift_st, op.gate_st};
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        const int k = which[j];
+        at[j] = base[k] ? (const char*)base[k] + (run.first.b * sb[k] + run.first.t * st[k]) * (int)sizeof(MT) +
+                              threadIdx.x * kM * 16
+                        : nullptr;
+        step[j] = st[k] * (int)sizeof(MT);
+      }
+    }
+  }
+  template <typename Mine>
+  __device__ __forceinline__ void copy(uint4* to, int team, Mine mine) {
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) {
+      if (!at[j]) continue;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (mine(p))
+#pragma unroll
+          for (int h = 0; h < kM; ++h)
+            copy16_async(to + ((j * kM + h) * P + p) * team, at[j] + (p * team * kM + h) * 16);
+      at[j] += step[j];
+    }
+  }
+  // Vector j of the row in a slot, `offset` added, or `missing` without it.
+  __device__ __forceinline__ void read(const uint4* slot, int team, int p, int j, float offset, float missing,
+                                       Vals<kVec<T>>& f) const {
+    if (!at[j]) {
+      f.fill(missing);
+      return;
+    }
+#pragma unroll
+    for (int h = 0; h < kM; ++h) unpack16<MT>(slot[((j * kM + h) * P + p) * team], f.q + h * kVec<MT> / 2);
+    if (j == 0)
+#pragma unroll
+      for (int i = 0; i < Vals<kVec<T>>::kPairs; ++i) f.q[i] = add2(f.q[i], pair(offset, offset));
+  }
+};
+template <typename T, typename MT, int P, bool kRow, bool kRes>
+using ForwardVectors = std::conditional_t<kRes, RowVectors<T, MT, P, kRow, kScaleVector, kShiftVector, kGateVector>,
+                                          RowVectors<T, MT, P, kRow, kScaleVector, kShiftVector>>;
+template <typename T, typename MT, int P, bool kRow, bool kRes>
+using BackwardVectors = std::conditional_t<kRes, RowVectors<T, MT, P, kRow, kScaleVector, kGateVector>,
+                                           RowVectors<T, MT, P, kRow, kScaleVector>>;
+
 // Long groups of wide rows that share their vectors: CTAs that stay on their SM walk
 // runs of rows with the vectors in registers, P 16-byte vectors a thread.  Each
 // thread copies its own vectors of the next kStages - 1 rows into shared memory:
 // the copies need no barrier and stay in flight across the one that joins a row's
-// statistics.  kFull: every thread has all of its P vectors.
-template <typename T, typename MT, int P, bool kRes, bool kFull, int kThreads, int kMin, int kStages>
+// statistics.  kFull: every thread has all of its P vectors.  kRow: each row has
+// vectors of its own, which are streamed as the rows are.
+template <typename T, typename MT, int P, bool kRes, bool kFull, bool kRow, int kThreads, int kMin, int kStages>
 __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(const SprAdaln op, const Groups gp) {
   constexpr int V = kVec<T>, kIn = kRes ? 2 : 1, e = sizeof(T);
+  constexpr int kM = kRow ? row_pieces<T, MT> : 0, kAll = kIn + kM * (kRes ? 3 : 2);
   __shared__ float2 red[2][16];
   extern __shared__ uint4 ring[];  // [stage][operand][P][thread]
   const int c = op.channels, nvec = c / V, team = blockDim.x, lane = threadIdx.x, warps = team / 32;
@@ -395,10 +459,11 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
   const char* x = run.at(op.x, op.x_sb, op.x_st, e);
   const char* y = kRes ? run.at(op.y, op.y_sb, op.y_st, e) : nullptr;
   const int64_t x_step = (run.step == 1 ? op.x_st : op.x_sb) * e, y_step = (run.step == 1 ? op.y_st : op.y_sb) * e;
+  ForwardVectors<T, MT, P, kRow, kRes> vec(op, run);
   int fetched = 0;
   auto fetch = [&](int stage) {
     if (fetched++ < run.rows) {
-      uint4* to = ring + stage * (kIn * P) * team + lane;
+      uint4* to = ring + stage * (kAll * P) * team + lane;
 #pragma unroll
       for (int p = 0; p < P; ++p)
         if (mine(p)) {
@@ -407,14 +472,16 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
         }
       x += x_step;
       if constexpr (kRes) y += y_step;
+      if constexpr (kRow) vec.copy(to + kIn * P * team, team, [&](int p) { return mine(p); });
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
-  Vals<V> w[P], b[P], gate[P];
+  constexpr int kHeld = kRow ? 1 : P;
+  Vals<V> w[kHeld], b[kHeld], gate[kHeld];
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
+  for (int p = 0; p < (kRow ? 0 : P); ++p) {
     const int v = lane + p * team;
     if (!mine(p)) continue;
     load_factor<MT, V>(op, run.group, v, w[p]);
@@ -429,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
   const int64_t out_step = run.step * c * e;
   for (int r = 0; r < run.rows; ++r) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    const uint4* slot = ring + stage * (kIn * P) * team + lane;
+    const uint4* slot = ring + stage * (kAll * P) * team + lane;
     Vals<V> z[P];
     uint64_t acc[2] = {0, 0};
 #pragma unroll
@@ -439,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
       if constexpr (kRes) {
         Vals<V> yv;
         unpack16<T>(slot[(P + p) * team], yv.q);
-        residual<T, V>(z[p], yv, gate[p]);
+        if constexpr (kRow) vec.read(slot + kIn * P * team, team, p, 2, 0.f, 1.f, gate[0]);
+        residual<T, V>(z[p], yv, gate[kRow ? 0 : p]);
         *reinterpret_cast<uint4*>(z_out + p * team * 16) = pack16<T>(z[p].q);
       }
 #pragma unroll
@@ -471,9 +539,14 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       if (!mine(p)) continue;
+      constexpr int kHold = kRow ? 0 : 1;
+      if constexpr (kRow) {
+        vec.read(slot + kIn * P * team, team, p, 0, op.scale_offset, 1.f, w[0]);
+        vec.read(slot + kIn * P * team, team, p, 1, 0.f, 0.f, b[0]);
+      }
 #pragma unroll
       for (int i = 0; i < V / 2; ++i)
-        z[p].q[i] = fma2(mul2(add2(z[p].q[i], pair(-mean, -mean)), pair(rstd, rstd)), w[p].q[i], b[p].q[i]);
+        z[p].q[i] = fma2(mul2(add2(z[p].q[i], pair(-mean, -mean)), pair(rstd, rstd)), w[p * kHold].q[i], b[p * kHold].q[i]);
       *reinterpret_cast<uint4*>(h_out + p * team * 16) = pack16<T>(z[p].q);
     }
     if (lane == 0 && op.mean) {
@@ -657,12 +730,14 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
 // so the copies need no barrier and stay in flight across the one that joins a
 // round's sums.  A round is R rows, which share the latency of shuffles and barrier.
 // kAgain: n and u are formed again after the barrier instead of held across it
-// (512 threads have 128 registers each; held, they spill).
+// (512 threads have 128 registers each; held, they spill).  kRow: each row has vectors
+// of its own; they are streamed as the rows are, and so are their gradients.
 constexpr int kStatRows = 256;  // rows whose statistics are in shared memory at a time
-template <typename T, typename MT, int P, bool kRes, bool kFull, bool kAgain, int R, int kThreads, int kStages>
+template <typename T, typename MT, int P, bool kRes, bool kFull, bool kRow, bool kAgain, int R, int kThreads, int kStages>
 __global__ void __launch_bounds__(kThreads, 1)
 adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups gp, float* partial) {
   constexpr int V = kVec<T>, kIn = kRes ? 4 : 2, e = sizeof(T);
+  constexpr int kM = kRow ? row_pieces<T, MT> : 0, kAll = kIn + kM * (kRes ? 2 : 1);
   __shared__ uint64_t red[2][R][16];
   __shared__ float stats[2][kStatRows];
   extern __shared__ uint4 ring[];  // [stage][row][operand][P][thread]
@@ -671,12 +746,12 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
   auto mine = [&](int p) { return kFull || lane + p * team < nvec; };
   const float inv_c = 1.f / c;
   for (int i = lane; i < 32 * R; i += team) (&red[0][0][0])[i] = 0;
-  Sums<V, P> st;
+  Sums<V, kRow ? 1 : P> st;
   st.clear();
-  constexpr int kHeld = kAgain ? 1 : P;
-  Vals<V> n[R][kHeld], u[R][kHeld], w[P], gate[P];
+  constexpr int kHeld = kAgain ? 1 : P, kOwn = kRow ? 1 : P;
+  Vals<V> n[R][kHeld], u[R][kHeld], w[kOwn], gate[kOwn];
 #pragma unroll
-  for (int p = 0; p < P; ++p)
+  for (int p = 0; p < (kRow ? 0 : P); ++p)
     if (mine(p)) {
       load_factor<MT, V>(op, run.group, lane + p * team, w[p]);
       if constexpr (kRes) load_gate<MT, V>(op, run.group, lane + p * team, gate[p]);
@@ -688,12 +763,14 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
   const bool along = run.step == 1;
   const int64_t step[4] = {(along ? op.x_st : op.x_sb) * e, (along ? gr.dh_st : gr.dh_sb) * e,
                            (along ? op.y_st : op.y_sb) * e, (along ? gr.dz_st : gr.dz_sb) * e};
+  BackwardVectors<T, MT, P, kRow, kRes> vec(op, run);
   int fetched = 0;
   auto fetch = [&](int stage) {
 #pragma unroll
     for (int q = 0; q < R; ++q)
       if (fetched++ < run.rows) {
-        uint4* to = ring + (stage * R + q) * (kIn * P) * team + lane;
+        uint4* to = ring + (stage * R + q) * (kAll * P) * team + lane;
+        if constexpr (kRow) vec.copy(to + kIn * P * team, team, [&](int p) { return mine(p); });
 #pragma unroll
         for (int k = 0; k < kIn; ++k) {
           if (k == 3 && !has_dz) continue;
@@ -722,7 +799,7 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
       __syncthreads();
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    const uint4* slot = ring + stage * R * (kIn * P) * team + lane;
+    const uint4* slot = ring + stage * R * (kAll * P) * team + lane;
     uint64_t sums[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -733,9 +810,18 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
         for (int p = 0; p < P; ++p) {
           if (!mine(p)) continue;
           Vals<V> z, dh;
-          unpack16<T>(slot[((q * kIn + 0) * P + p) * team], z.q);
-          unpack16<T>(slot[((q * kIn + 1) * P + p) * team], dh.q);
-          st.first(p, z, dh, w[p], minus, rs, n[q][kAgain ? 0 : p], u[q][kAgain ? 0 : p], s0, s1);
+          unpack16<T>(slot[((q * kAll + 0) * P + p) * team], z.q);
+          unpack16<T>(slot[((q * kAll + 1) * P + p) * team], dh.q);
+          if constexpr (kRow) {
+            vec.read(slot + (q * kAll + kIn) * P * team, team, p, 0, op.scale_offset, 1.f, w[0]);
+            st.clear();  // a row's own: written below, not added up
+          }
+          st.first(kRow ? 0 : p, z, dh, w[kRow ? 0 : p], minus, rs, n[q][kAgain ? 0 : p], u[q][kAgain ? 0 : p], s0, s1);
+          if constexpr (kRow) {
+            const int64_t at_c = (run.row0 + r + q) * c + (lane + p * team) * V;
+            if (gr.dshift) store_row<MT, V>((MT*)gr.dshift + at_c, st.shift[0]);
+            if (gr.dscale) store_row<MT, V>((MT*)gr.dscale + at_c, st.scale[0]);
+          }
         }
       }
       const float2 a = halves(s0), b = halves(s1);
@@ -766,24 +852,31 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
       for (int p = 0; p < P; ++p) {
         if (!mine(p)) continue;
         Vals<V> gx, dz;
-        if (has_dz) unpack16<T>(slot[((q * kIn + 3) * P + p) * team], dz.q);
+        if (has_dz) unpack16<T>(slot[((q * kAll + 3) * P + p) * team], dz.q);
         else dz.fill(0.f);
         if constexpr (kAgain) {
           Vals<V> z, dh;
-          unpack16<T>(slot[((q * kIn + 0) * P + p) * team], z.q);
-          unpack16<T>(slot[((q * kIn + 1) * P + p) * team], dh.q);
+          unpack16<T>(slot[((q * kAll + 0) * P + p) * team], z.q);
+          unpack16<T>(slot[((q * kAll + 1) * P + p) * team], dh.q);
           const uint64_t minus = both<V>(stats[0][at + q]);
+          if constexpr (kRow) vec.read(slot + (q * kAll + kIn) * P * team, team, p, 0, op.scale_offset, 1.f, w[0]);
 #pragma unroll
           for (int i = 0; i < V / 2; ++i) {
             n[q][0].q[i] = mul2(add2(z.q[i], minus), rs);
-            u[q][0].q[i] = mul2(dh.q[i], w[p].q[i]);
+            u[q][0].q[i] = mul2(dh.q[i], w[kRow ? 0 : p].q[i]);
           }
         }
         second<V>(n[q][kAgain ? 0 : p], u[q][kAgain ? 0 : p], m0, m1, rs, dz, gx);
         if constexpr (kRes) {
-          Vals<V> y, gy = gate[p];
-          unpack16<T>(slot[((q * kIn + 2) * P + p) * team], y.q);
-          st.branch(p, gx, y, gy);
+          Vals<V> y, gy = gate[kRow ? 0 : p];
+          unpack16<T>(slot[((q * kAll + 2) * P + p) * team], y.q);
+          if constexpr (kRow) {
+            vec.read(slot + (q * kAll + kIn) * P * team, team, p, 1, 0.f, 1.f, gy);
+            st.gate[0].fill(0.f);
+          }
+          st.branch(kRow ? 0 : p, gx, y, gy);
+          if constexpr (kRow)
+            if (gr.dgate) store_row<MT, V>((MT*)gr.dgate + (run.row0 + r + q) * c + (lane + p * team) * V, st.gate[0]);
           *reinterpret_cast<uint4*>(dy + p * team * 16) = pack16<T>(gy.q);
         }
         *reinterpret_cast<uint4*>(dx + p * team * 16) = pack16<T>(gx.q);
@@ -794,11 +887,12 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (!kRow)
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int v = lane + p * team;
-    if (mine(p)) store_sums<MT, V>(gr, gp, blockIdx.x, c, v, partial, st.shift[p], st.scale[p], st.gate[p]);
-  }
+    for (int p = 0; p < P; ++p) {
+      const int v = lane + p * team;
+      if (mine(p)) store_sums<MT, V>(gr, gp, blockIdx.x, c, v, partial, st.shift[p], st.scale[p], st.gate[p]);
+    }
 }
 
 // Joins the runs' column sums in their order: 32 columns by 32 threads each.
@@ -889,13 +983,17 @@ int by_type(const SprAdaln* op, F f) {
 // Rows without gaps between the samples are one sample of batch*tokens rows.
 bool dense_batch(int64_t sb, int64_t st, int64_t tokens) { return sb == tokens * st; }
 void merge_batch(SprAdaln& op, SprAdalnGrad* g) {
-  if (op.batch == 1 || op.shift_sb || op.scale_sb || op.gate_sb || op.shift_st || op.scale_st || op.gate_st) return;
+  if (op.batch == 1) return;
+  for (auto [p, sb, st] : {std::tuple(op.shift, op.shift_sb, op.shift_st), std::tuple(op.scale, op.scale_sb, op.scale_st),
+                           std::tuple(op.gate, op.gate_sb, op.gate_st)})
+    if (p && !dense_batch(sb, st, op.tokens)) return;  // one vector (0, 0), or one for each row
   if (!dense_batch(op.x_sb, op.x_st, op.tokens) || (op.y && !dense_batch(op.y_sb, op.y_st, op.tokens))) return;
-  if (g && (g->mod_batch || g->mod_tokens || !dense_batch(g->dh_sb, g->dh_st, op.tokens) ||
+  if (g && (g->mod_batch != g->mod_tokens || !dense_batch(g->dh_sb, g->dh_st, op.tokens) ||
             (g->dz && !dense_batch(g->dz_sb, g->dz_st, op.tokens))))
     return;
   op.tokens *= op.batch;
   op.batch = 1;
+  if (g) g->mod_batch = 0;
 }
 
 template <int N>
@@ -974,10 +1072,13 @@ constexpr int ring_stages(int bytes) {
   return 4 * bytes <= 200 * 1024 ? 4 : 3 * bytes <= 200 * 1024 ? 3 : 2 * bytes <= 200 * 1024 ? 2 : 0;
 }
 
-template <typename T, typename MT, bool kRes, int P, bool kFull, int kThreads, int kMin>
+template <typename T, typename MT, bool kRes, int P, bool kFull, bool kRow, int kThreads, int kMin>
 int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
-  constexpr int kIn = kRes ? 2 : 1, kStages = ring_stages(kIn * P * kThreads * 16);
-  auto kern = adaln_forward_stream_kernel<T, MT, P, kRes, kFull, kThreads, kMin, kStages>;
+  static_assert(kThreads <= 512, "sums of at most 16 warps are joined");
+  constexpr int kIn = (kRes ? 2 : 1) + (kRow ? row_pieces<T, MT> * (kRes ? 3 : 2) : 0);
+  constexpr int kStages = ring_stages(kIn * P * kThreads * 16);
+  static_assert(kStages >= 2, "no ring fits");
+  auto kern = adaln_forward_stream_kernel<T, MT, P, kRes, kFull, kRow, kThreads, kMin, kStages>;
   const int team = cta_for(op->channels / kVec<T>, P);
   const int smem = kStages * kIn * P * team * 16;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * kIn * P * kThreads * 16) !=
@@ -1002,6 +1103,18 @@ int launch_forward(const SprAdaln* op, cudaStream_t st) {
   auto kept = [&](int64_t scale, int64_t shift, int64_t gate) { return scale || shift || gate; };
   const Groups g = make_groups(op->batch, op->tokens, kept(op->scale_sb, op->shift_sb, op->gate_sb),
                                kept(op->scale_st, op->shift_st, op->gate_st));
+  // Vectors for every token: 8 values a thread, so that a stage of them and the rows is
+  // small enough for several CTAs an SM (of measured bandwidth, 40,000 gated rows of 1536
+  // bf16: 95%, with a CTA a row 69%).  Wider rows keep a CTA a row: one CTA an SM with two
+  // or three stages is slower (20,000 x 5120 gated, fp32 vectors: 67%, with a CTA a row 89%).
+  if (vec && nvec > 32 && kept(op->scale_st, op->shift_st, op->gate_st) && op->tokens >= 8) {
+    constexpr int Q = 8 / kVec<T>;
+    const Groups rows = make_groups(op->batch, op->tokens, 1, 0);  // the samples' rows, one after the other
+    if (nvec <= 512 * Q) {
+      if (nvec % (32 * Q) == 0) return launch_forward_stream<T, MT, kRes, Q, true, true, 512, 1>(op, rows, st);
+      return launch_forward_stream<T, MT, kRes, Q, false, true, 512, 1>(op, rows, st);
+    }
+  }
   constexpr int P = 16 / kVec<T>;  // 16 values a thread, or 8 where that leaves fewer threads idle
   if (vec && nvec > 32 && nvec <= 512 * P && g.rows >= 8 && even_rows(g, op->batch)) {
     // 32 values a thread from 128 threads on: fewer warps pay a row's fixed instructions,
@@ -1010,12 +1123,12 @@ int launch_forward(const SprAdaln* op, cudaStream_t st) {
     // (490 and 513 us).
     if constexpr (!kRes)
       if (nvec % (64 * P) == 0 && nvec >= 256 * P && nvec <= 320 * P)
-        return launch_forward_stream<T, MT, false, 2 * P, true, 160, 3>(op, g, st);
+        return launch_forward_stream<T, MT, false, 2 * P, true, false, 160, 3>(op, g, st);
     if (nvec % (32 * P) == 0)
-      return nvec <= 320 * P ? launch_forward_stream<T, MT, kRes, P, true, 320, 2>(op, g, st)
-                             : launch_forward_stream<T, MT, kRes, P, true, 512, 1>(op, g, st);
-    if (half_fits_better(nvec, P)) return launch_forward_stream<T, MT, kRes, P / 2, false, 512, 1>(op, g, st);
-    return launch_forward_stream<T, MT, kRes, P, false, 512, 1>(op, g, st);
+      return nvec <= 320 * P ? launch_forward_stream<T, MT, kRes, P, true, false, 320, 2>(op, g, st)
+                             : launch_forward_stream<T, MT, kRes, P, true, false, 512, 1>(op, g, st);
+    if (half_fits_better(nvec, P)) return launch_forward_stream<T, MT, kRes, P / 2, false, false, 512, 1>(op, g, st);
+    return launch_forward_stream<T, MT, kRes, P, false, false, 512, 1>(op, g, st);
   }
   return by_shape<T>(vec, forward_per_thread<T>(vec, nvec), [&](auto v, auto p) {
     constexpr int V = decltype(v)::value, P = decltype(p)::value;
@@ -1042,18 +1155,22 @@ int join(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, const floa
   return check_launch("adaln backward");
 }
 
-template <typename T, typename MT, bool kRes, int P, bool kFull, bool kAgain, int R, int kThreads>
+template <typename T, typename MT, bool kRes, int P, bool kFull, bool kRow, bool kAgain, int R, int kThreads>
 int launch_backward_stream(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, float* partial, cudaStream_t st) {
-  constexpr int kIn = kRes ? 4 : 2, kStages = std::min(kRes ? 4 : 3, ring_stages(R * kIn * P * kThreads * 16));
-  auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kFull, kAgain, R, kThreads, kStages>;
+  static_assert(kThreads <= 512, "sums of at most 16 warps are joined");
+  constexpr int kIn = (kRes ? 4 : 2) + (kRow ? row_pieces<T, MT> * (kRes ? 2 : 1) : 0);
+  constexpr int kStages = std::min(kRes ? 4 : 3, ring_stages(R * kIn * P * kThreads * 16));
+  static_assert(kStages >= 2, "no ring fits");
+  auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kFull, kRow, kAgain, R, kThreads, kStages>;
   const int team = cta_for(op->channels / kVec<T>, P);
   const int smem = kStages * R * kIn * P * team * 16;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * R * kIn * P * kThreads * 16) !=
       cudaSuccess)
     return check_launch("adaln backward");
   cut_stream(g, (int64_t)sm_count() * resident(kern, team, smem), (int64_t)kIn * op->channels * sizeof(T),
-             kRes ? 6 : 1, 3 << 19, most_runs(op->channels));
+             kRow || kRes ? 6 : 1, kRow ? 65536 : 3 << 19, kRow ? INT64_MAX : most_runs(op->channels));
   kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, *gr, g, partial);
+  if constexpr (kRow) return check_launch("adaln backward");
   return join<MT>(op, gr, g, partial, st);
 }
 
@@ -1062,17 +1179,29 @@ int launch_backward(const SprAdaln* op, const SprAdalnGrad* gr, float* partial, 
   const bool vec = vectors_fit(op, gr);
   const int nvec = op->channels / (vec ? kVec<T> : 1);
   Groups g = make_groups(op->batch, op->tokens, gr->mod_batch, gr->mod_tokens);
+  if (vec && nvec > 32 && gr->mod_tokens && op->tokens >= 8 && (gr->mod_batch || op->batch == 1)) {
+    constexpr int Q = 8 / kVec<T>;
+    const Groups rows = make_groups(op->batch, op->tokens, 1, 0);
+    if (nvec <= 512 * Q) {
+      if (nvec % (32 * Q) == 0)
+        return launch_backward_stream<T, MT, kRes, Q, true, true, false, 1, 512>(op, gr, rows, partial, st);
+      return launch_backward_stream<T, MT, kRes, Q, false, true, false, 1, 512>(op, gr, rows, partial, st);
+    }
+    if constexpr (!kRes || sizeof(T) == 2)  // six fp32 operands of that width leave no room for two stages
+      if (nvec <= 640 * Q)
+        return launch_backward_stream<T, MT, kRes, 2 * Q, false, true, false, 1, 320>(op, gr, rows, partial, st);
+  }
   constexpr int kPer = 16 / kVec<T>;  // 16 values a thread, or 8 where that leaves fewer threads idle
   constexpr int kWide = kRes && sizeof(T) == 4 ? 320 : 512;  // threads whose ring fits
   if (vec && nvec > 32 && nvec <= kWide * kPer && g.rows >= 8 && even_rows(g, op->batch)) {
     if (nvec % (32 * kPer) == 0) {
       if (nvec <= 320 * kPer)
-        return launch_backward_stream<T, MT, kRes, kPer, true, false, kRes ? 1 : 2, 320>(op, gr, g, partial, st);
-      return launch_backward_stream<T, MT, kRes, kPer, true, kRes, 1, kWide>(op, gr, g, partial, st);
+        return launch_backward_stream<T, MT, kRes, kPer, true, false, false, kRes ? 1 : 2, 320>(op, gr, g, partial, st);
+      return launch_backward_stream<T, MT, kRes, kPer, true, false, kRes, 1, kWide>(op, gr, g, partial, st);
     }
     if (half_fits_better(nvec, kPer))
-      return launch_backward_stream<T, MT, kRes, kPer / 2, false, false, 1, 512>(op, gr, g, partial, st);
-    return launch_backward_stream<T, MT, kRes, kPer, false, kRes, 1, kWide>(op, gr, g, partial, st);
+      return launch_backward_stream<T, MT, kRes, kPer / 2, false, false, false, 1, 512>(op, gr, g, partial, st);
+    return launch_backward_stream<T, MT, kRes, kPer, false, false, kRes, 1, kWide>(op, gr, g, partial, st);
   }
   const int per = nvec <= 32 ? 1 : vec ? (nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : 4) : nvec <= 4096 ? 4 : 16;
   return by_shape<T>(vec, per, [&](auto v, auto p) {

@@ -1032,7 +1032,7 @@ ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype, int scale) {
       // round's end (with a wait for the tile's other warps), the join.
       const int64_t rounds = (work + team_tiles * sms - 1) / (team_tiles * sms);
       const double chunk = (p.ints ? 0.7 : 0.9) * (1 + 0.25 * (p.nt - 1)) * std::max(1.0, along * team_tiles / 12.0);
-      const double time = rounds * (warp_chunks * chunk + (along > 1 ? 1.5 : 0.3)) +
+      const double time = rounds * (warp_chunks * chunk + (along > 1 ? 0.7 : 0.3)) +
                           (slices > 1 ? 3 + slices * (double)rows * (double)w.n * 8 / 5e6 : 0);
       if (time >= best * 0.98) continue;
       best = time;

@@ -71,7 +71,8 @@ def _backward(ctx, dy):
     if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
         dy = dy.contiguous()
     if ctx.needs_input_grad[0]:
-        dx = K.int4_linear_grad(dy, packed, scales, zeros, ctx.in_features)
+        n, groups = scales.shape
+        dx = K.int4_linear_grad_checked(dy, packed, scales, zeros, ctx.in_features, n, 2 * packed.shape[1] // groups)
     if ctx.needs_input_grad[4]:
         dbias = dy.sum(0)  # 16-bit sums are fp32 inside and rounded once
     return dx, None, None, None, dbias

@@ -717,13 +717,19 @@ def int4_linear_grad(dy, packed, scales, zeros, in_features: int) -> torch.Tenso
     """Gradient of :func:`int4_linear` with respect to its rows: ``dy`` [R,N] -> [R, in_features]."""
     _cuda(dy, packed, scales, zeros)
     n, group = _int4_checks("int4_linear_grad", dy, in_features, packed, scales, zeros)
-    r = dy.shape[0]
     if dy.shape[1] != n:
         raise RuntimeError(f"int4_linear_grad: dy {tuple(dy.shape)} does not match {n} weight rows")
+    return int4_linear_grad_checked(dy, packed, scales, zeros, in_features, n, group)
+
+
+def int4_linear_grad_checked(dy, packed, scales, zeros, in_features: int, n: int, group: int) -> torch.Tensor:
+    """:func:`int4_linear_grad` of operands that the forward pass has checked."""
+    r = dy.shape[0]
     dx = dy.new_empty((r, in_features))
-    nbytes = _lib.query("spr_int4_linear_grad_workspace_bytes", r, n, in_features, group, _DT[dy.dtype])
+    dt = _DT[dy.dtype]
+    nbytes = _lib.query("spr_int4_linear_grad_workspace_bytes", r, n, in_features, group, dt)
     ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _count(2)
-    _launch(dy.get_device(), "spr_int4_linear_grad", _p(dy), dy.stride(0), _DT[dy.dtype], r, n, in_features, group, _p(packed),
-            _p(scales), _DT[scales.dtype], _p(zeros), _p(dx), _p(ws), nbytes)
+    _launch(dy.get_device(), "spr_int4_linear_grad", dy.data_ptr(), dy.stride(0), dt, r, n, in_features, group,
+            packed.data_ptr(), scales.data_ptr(), _DT[scales.dtype], _p(zeros), dx.data_ptr(), _p(ws), nbytes)
     return dx

@@ -217,6 +217,15 @@ BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
     (1, 20, 5128, FP, FP, "vector"),
     (1, 77, 8192, HF, FP, "vector"),
     (3, 41, 8200, BF, BF, "vector"),
+    (1, 70, 1536, BF, BF, "token"),
+    (2, 60, 1536, BF, FP, "token"),
+    (3, 50, 328, HF, HF, "token"),
+    (1, 90, 256, FP, FP, "token"),
+    (2, 37, 5120, BF, FP, "token"),
+    (1, 40, 4104, HF, HF, "token"),
+    (3, 33, 640, BF, FP, "shared"),
+    (2, 30, 5120, FP, FP, "token"),
+    (1, 25, 5200, BF, BF, "token"),
     (1, 5, 16384, BF, BF, "vector"),
     (1, 3, 16383, FP, FP, "sample"),
     (2, 4, 16384, FP, FP, "shared"),
@@ -281,6 +290,15 @@ def test_strides_offsets_and_expanded_gradients(cuda):
                  dz=torch.randn(1, n, 1, device=cuda, generator=g).to(BF).expand(b, n, c))
         _check(v, True)
         v.update(shift=shift[0, 0], scale=scale[0, 0], gate=gate[0, 0])  # one vector, strided rows
+        _check(v, False)
+    # A vector for every token, each kind a part of one wider tensor, rows with gaps.
+    wide_mods = torch.randn(b, n, 3 * c, device=cuda, generator=g).to(BF) * 0.3
+    for batch in (slice(0, b), slice(0, 1)):
+        v = dict(x=wide[batch, 2:2 + n, 8:8 + c], y=wide[batch, :n, 8 + c:8 + 2 * c],
+                 dh=torch.randn(b, n, c, device=cuda, generator=g).to(BF)[batch],
+                 dz=torch.randn(b, n, c, device=cuda, generator=g).to(BF)[batch])
+        v.update(zip(("gate", "shift", "scale"), wide_mods[batch].chunk(3, dim=-1)))
+        _check(v, True)
         _check(v, False)
     # A transposed leading order: [n, b, c] seen as [b, n, c], each sample with its vector.
     x = torch.randn(n, b, c, device=cuda, generator=g).to(BF).transpose(0, 1)
@@ -454,3 +472,30 @@ def test_two_captured_graphs_replayed_together(cuda):
     for _g, got, want, _s, _in in runs:
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_captured_autograd_step(cuda):
+    """Forward and backward pass captured as a training step captures them: warmed up on a side
+    stream, no eager graph of the leaves left alive."""
+    v = _inputs(cuda, 1, 1000, 640, BF, FP, "vector", seed=9)
+    leaves = [v[k].detach().requires_grad_() for k in ("x", "y", "gate", "shift", "scale")]
+
+    def step():
+        z, h = spr.gated_residual_layer_norm(*leaves)
+        return torch.autograd.grad((z, h), leaves, (v["dz"], v["dh"]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in got:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
