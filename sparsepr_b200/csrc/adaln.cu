@@ -1043,9 +1043,10 @@ int forward_per_thread(bool vec, int nvec) {
   return nvec <= 4096 ? 4 : 16;
 }
 
-// CTAs of a kernel that an SM holds, asked once for each number of warps.
-template <typename K>
-int resident(K kern, int threads, int smem) {
+// CTAs of a kernel that an SM holds, asked once for each number of warps (a kernel's
+// shared memory follows from them).
+template <auto kern>
+int resident(int threads, int smem) {
   static std::atomic<int> known[33] = {};
   std::atomic<int>& n = known[threads / 32];
   if (n.load(std::memory_order_relaxed) == 0) {
@@ -1078,13 +1079,13 @@ int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
   constexpr int kIn = (kRes ? 2 : 1) + (kRow ? row_pieces<T, MT> * (kRes ? 3 : 2) : 0);
   constexpr int kStages = ring_stages(kIn * P * kThreads * 16);
   static_assert(kStages >= 2, "no ring fits");
-  auto kern = adaln_forward_stream_kernel<T, MT, P, kRes, kFull, kRow, kThreads, kMin, kStages>;
+  constexpr auto kern = adaln_forward_stream_kernel<T, MT, P, kRes, kFull, kRow, kThreads, kMin, kStages>;
   const int team = cta_for(op->channels / kVec<T>, P);
   const int smem = kStages * kIn * P * team * 16;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * kIn * P * kThreads * 16) !=
       cudaSuccess)
     return check_launch("adaln forward");
-  cut_stream(g, (int64_t)sm_count() * resident(kern, team, smem), (int64_t)kIn * op->channels * sizeof(T), 6, 65536,
+  cut_stream(g, (int64_t)sm_count() * resident<kern>(team, smem), (int64_t)kIn * op->channels * sizeof(T), 6, 65536,
              INT64_MAX);
   kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, g);
   return check_launch("adaln forward");
@@ -1161,13 +1162,13 @@ int launch_backward_stream(const SprAdaln* op, const SprAdalnGrad* gr, Groups g,
   constexpr int kIn = (kRes ? 4 : 2) + (kRow ? row_pieces<T, MT> * (kRes ? 2 : 1) : 0);
   constexpr int kStages = std::min(kRes ? 4 : 3, ring_stages(R * kIn * P * kThreads * 16));
   static_assert(kStages >= 2, "no ring fits");
-  auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kFull, kRow, kAgain, R, kThreads, kStages>;
+  constexpr auto kern = adaln_backward_stream_kernel<T, MT, P, kRes, kFull, kRow, kAgain, R, kThreads, kStages>;
   const int team = cta_for(op->channels / kVec<T>, P);
   const int smem = kStages * R * kIn * P * team * 16;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * R * kIn * P * kThreads * 16) !=
       cudaSuccess)
     return check_launch("adaln backward");
-  cut_stream(g, (int64_t)sm_count() * resident(kern, team, smem), (int64_t)kIn * op->channels * sizeof(T),
+  cut_stream(g, (int64_t)sm_count() * resident<kern>(team, smem), (int64_t)kIn * op->channels * sizeof(T),
              kRow || kRes ? 6 : 1, kRow ? 65536 : 3 << 19, kRow ? INT64_MAX : most_runs(op->channels));
   kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, *gr, g, partial);
   if constexpr (kRow) return check_launch("adaln backward");

@@ -499,3 +499,37 @@ def test_captured_autograd_step(cuda):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_the_calls_before(cuda):
+    """The order of a vector gradient's sum is that of a fresh process, whatever other passes over CTAs
+    of the same size ran first."""
+    import subprocess
+    import sys
+
+    script = """
+import sys, torch, sparsepr_b200 as spr
+g = torch.Generator(device="cuda").manual_seed(3)
+def run(c, gated, n, dtype):
+    x, y, dh = torch.randn(3, 1, n, c, device="cuda", generator=g).to(dtype)
+    v = [torch.randn(c, device="cuda", generator=g).to(dtype).requires_grad_() for _ in range(3)]
+    if gated:
+        z, h = spr.gated_residual_layer_norm(x, y, *v)
+        return torch.autograd.grad((z, h), v, (dh, dh))
+    return torch.autograd.grad(spr.modulated_layer_norm(x, *v[:2]), v[:2], dh)
+state = g.get_state()
+if len(sys.argv) > 1:
+    for dtype in (torch.float32, torch.float16):
+        for c in (640, 1280, 2560):
+            run(c, True, 4096, dtype), run(c, False, 4096, dtype), run(c + 8, True, 4096, dtype)
+g.set_state(state)
+for c in (1280, 2560):
+    for gated in (False, True):
+        for t in run(c, gated, 20000, torch.bfloat16):
+            print(t.double().sum().item(), t.double().square().sum().item())
+"""
+    out = [subprocess.run([sys.executable, "-c", script, *args], capture_output=True, text=True, timeout=300)
+           for args in ((), ("first",))]
+    assert out[0].returncode == 0, out[0].stderr
+    assert out[0].stdout and out[0].stdout == out[1].stdout
