@@ -123,6 +123,9 @@ def operands(x, y, gate, shift, scale, scale_offset: float = 1.0):
     return op, (mb, mn)
 
 
+_SAVED = ("x", "y", "gate", "scale")
+
+
 def _backward(ctx, *grads):
     x, y, gate, scale, stats = ctx.saved_tensors
     dz, dh = grads if y is not None else (None, grads[0])
@@ -141,6 +144,12 @@ def _backward(ctx, *grads):
         s.y, s.x_sb, s.x_st = y.data_ptr(), s.tokens * s.channels, s.channels
     s.gate = None if gate is None else gate.data_ptr()
     s.scale = None if scale is None else scale.data_ptr()
+    for name, t, strides in zip(_SAVED, (x, y, gate, scale), ctx.strides):
+        if t is not None and t.stride() != strides:  # a saved-tensor hook gave back another layout
+            b, n = (s.batch, s.tokens) if name in ("x", "y") else mod_shape
+            sb, st = _strides(t, b, n, name)
+            setattr(s, name + "_sb", sb)
+            setattr(s, name + "_st", st)
     mean = stats.data_ptr()
     s.mean, s.rstd = mean, mean + 4 * stats.shape[1]
     return *K.adaln_backward_struct(s, y is not None, dh, dz, ctx.needs_input_grad[2:5], mod_shape, vector_shape, mod_dtype), None, None
@@ -154,7 +163,9 @@ class _AdaLN(torch.autograd.Function):
     def forward(ctx, x, y, gate, shift, scale, eps, scale_offset):
         op, mod_shape = operands(x, y, gate, shift, scale, scale_offset)
         z, h, stats, struct = K.adaln_forward_struct(op, eps, True)
-        ctx.save_for_backward(x if z is None else z, y, gate, scale, stats)
+        saved = x if z is None else z, y, gate, scale
+        ctx.save_for_backward(*saved, stats)
+        ctx.strides = [None if t is None else t.stride() for t in saved]
         ctx.set_materialize_grads(False)
         vector = gate if gate is not None else shift if shift is not None else scale
         ctx.operands = struct, mod_shape, None if vector is None else vector.shape, op.mod_dtype

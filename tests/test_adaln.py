@@ -407,6 +407,29 @@ def test_saved_operands_may_be_moved(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_saved_operands_may_come_back_in_another_layout(cuda, gated):
+    """Such hooks give back dense copies of strided operands."""
+    g = torch.Generator(device=cuda).manual_seed(12)
+    wide = torch.randn(3, 40, 2 * 64, device=cuda, generator=g)
+    x, y = wide[..., :64].requires_grad_(), wide.transpose(0, 1).contiguous().transpose(0, 1)[..., 64:].requires_grad_()
+    gate, shift, scale = (t.requires_grad_() for t in torch.randn(3, 1, 3 * 64, device=cuda, generator=g).chunk(3, -1))
+    dh = torch.randn(3, 40, 64, device=cuda, generator=g)
+
+    def grads():
+        if gated:
+            z, h = spr.gated_residual_layer_norm(x, y, gate, shift, scale)
+            return torch.autograd.grad((z, h), (x, y, gate, shift, scale), (dh, dh))
+        return torch.autograd.grad(spr.modulated_layer_norm(x, shift, scale), (x, shift, scale), dh)
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_refusals(cuda):
     x, v = torch.zeros(2, 4, 16, device=cuda), torch.zeros(16, device=cuda)
     with pytest.raises(RuntimeError, match="fp32/bf16/fp16"):
