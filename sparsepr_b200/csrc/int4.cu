@@ -5,11 +5,14 @@
 // What bounds both is the codes' bytes: HBM gives an SM 23 bytes, 46 codes, a cycle,
 // so a 16 x 32 block of codes has 44 instruction slots of the SM's four schedulers
 // for everything.  Hence tensor-core products whose operand is a few instructions
-// from the packed codes, and no rounding of x:
+// from the packed codes:
 // * 16-bit x: integer products (m16n8k32).  The codes are the bytes w & 0x0f0f0f0f and
-//   (w >> 4) & 0x0f0f0f0f; x is a 23-bit integer relative to its row's largest
-//   magnitude, in three signed bytes, each a column of the product.  An inner sum is
-//   an exact integer.
+//   (w >> 4) & 0x0f0f0f0f; x is a 31-bit integer relative to its row's largest
+//   magnitude (of the CTA's columns), in four signed bytes, each a column of the
+//   product.  An inner sum is an exact integer.  A value far below the largest is
+//   rounded at 2^-30 of it: beside the largest's own term less than an fp32 sum
+//   rounds, and where that term is 0 small values still have bf16's 8 bits down to
+//   2^-22 of it.
 // * fp32 x, and more rows than the integer columns hold: bf16 products (m16n8k16).  A
 //   code is the exact integer code - zero, and x is cut into as many bf16 parts as
 //   its significand needs (bf16 1, fp16 2, fp32 3; exact), each a column.
@@ -28,7 +31,7 @@ constexpr int kTile = 16;  // weight rows of a product
 constexpr int kBlocks = 8;  // blocks of 32 codes in one stage of a warp's ring: 128 bytes of a row
 constexpr int kStages = 4;
 constexpr int kStageBytes = kTile * kBlocks * 16;
-constexpr int kLimbs = 3;
+constexpr int kLimbs = 4;
 
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
   if (dtype == SPR_F32) return __ldg((const float*)p + i);
@@ -53,11 +56,6 @@ __device__ __forceinline__ uint32_t bf16_part(float v, int part) {
   return part == 1 ? __float_as_uint(b) : __float_as_uint(rest - b) & 0xffff0000u;
 }
 __device__ __forceinline__ uint32_t bf16_pair(uint32_t low, uint32_t high) { return __byte_perm(low, high, 0x7632); }
-
-__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -256,9 +254,9 @@ __device__ __forceinline__ void scan_x(const Weights& w, const Rows& in, int row
   __syncthreads();
 }
 
-// Integers q = round(x * 2^power[r]) below 2^22 in magnitude, as signed bytes d0 + 256 d1
-// + 65536 d2: the bytes of q + 0x808080 less 128 each.  sums[segment's first block]
-// [column]: the bytes of a segment added up.  What is not finite counts as 0 and sets
+// Integers q = round(x * 2^power[r]) of at most 2^30 in magnitude, as signed bytes d0 +
+// 256 d1 + 65536 d2 + 2^24 d3: the bytes of q + 0x80808080 less 128 each.  sums[segment's
+// first block][column]: the bytes of a segment added up.  What is not finite counts as 0 and sets
 // bad[r].
 template <int U, int GB>
 __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, bool wide,
@@ -266,7 +264,7 @@ __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int 
                                           const int* bad) {
   const int cols = rows * kLimbs, words = nb * 4;
   for (int r = 0; r < rows; ++r) {
-    const int p = 21 - ((int)(largest[r] >> 23) - 127), half = p / 2;  // -106 .. 148: two factors, each exact
+    const int p = 29 - ((int)(largest[r] >> 23) - 127), half = p / 2;  // -98 .. 156: two factors, each exact
     if (threadIdx.x == 0) power[r] = p;
     const float f0 = __int_as_float((127 + half) << 23), f1 = __int_as_float((127 + p - half) << 23);
     const bool check = bad[r];
@@ -279,15 +277,15 @@ __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (check && !finite(v[e])) v[e] = 0.f;
-          u[e] = 0x808080 + __float2int_rn(v[e] * f0 * f1);
+          u[e] = 0x80808080u + (uint32_t)__float2int_rn(v[e] * f0 * f1);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = 0x808080;
+        for (int e = 0; e < 8; ++e) u[e] = 0x80808080u;
       }
 #pragma unroll
       for (int l = 0; l < kLimbs; ++l) {
-        constexpr uint32_t pick[kLimbs] = {0x40, 0x51, 0x62};
+        constexpr uint32_t pick[kLimbs] = {0x40, 0x51, 0x62, 0x73};
         const uint32_t d0 = __byte_perm(__byte_perm(u[0], u[2], pick[l]), __byte_perm(u[4], u[6], pick[l]), 0x5410) ^
                             0x80808080u;
         const uint32_t d1 = __byte_perm(__byte_perm(u[1], u[3], pick[l]), __byte_perm(u[5], u[7], pick[l]), 0x5410) ^

@@ -198,6 +198,26 @@ def test_unused_codes_are_ignored_and_bad_values_stay_in_their_row(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows", [1, 8])
+def test_values_far_below_the_largest_of_their_row(cuda, dtype, rows):
+    """Where the codes opposite a row's largest value are zero, the small values keep their bits."""
+    n, k = 100, 640
+    w = _weights(cuda, n, k, 64, FP, False)
+    w.packed[:, 50] = w.packed[:, 50] & 0xF0 | 8  # column 100
+    x = torch.randn(rows, k, device=cuda, generator=torch.Generator(device=cuda).manual_seed(2)) * 2.0 ** -6
+    x = x.to(dtype)
+    x[:, 100] = 2.0 ** 12
+    dense = _dense64(w, k)
+    ref = x.double() @ dense.t()
+    terms = x.double().abs() @ dense.abs().t()  # the largest value's are 0
+    err = (spr.int4_linear(x, *w).double() - ref).abs()
+    # One rounding, the fp32 sums, and each small value within half of 2^(12 - 29).
+    tol = torch.finfo(dtype).eps / 2 * ref.abs() + (64 + k) * 2.0 ** -23 * terms + 2.0 ** -18 * dense.abs().sum(1)
+    assert not (err > tol).any(), (err / tol).max().item()
+
+
+@pytest.mark.gpu
 def test_empty_rows_and_outputs(cuda):
     w = _weights(cuda, 8, 64, 32, FP, False)
     x = torch.zeros(0, 64, device=cuda, requires_grad=True)
