@@ -432,8 +432,9 @@ int spr_adaln_forward(const SprAdaln* op, void* stream);
  * of the vectors summed over the rows that share one, dense
  * [groups][channels] in mod_dtype, where groups = the product of the axes that
  * shift/scale/gate are not broadcast along; mod_batch and mod_tokens say which
- * axes those are (1: kept, 0: summed).  dshift, dscale and dgate are nullable
- * (not formed).  The sums run in a fixed order.  workspace:
+ * axes those are (1: kept, 0: summed; scale and gate may not have a stride along
+ * an axis that is summed).  dshift, dscale and dgate are nullable (not formed).
+ * The sums run in a fixed order.  Without rows nothing is written.  workspace:
  * spr_adaln_backward_workspace_bytes(op's sizes).
  */
 typedef struct SprAdalnGrad {
@@ -453,7 +454,7 @@ int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, void* works
  * y[r][n] = sum_k x[r][k] * (code[n][k] - zero[n][k/group]) * scale[n][k/group] + bias[n]
  * for a few rows r (a conditioning vector per sample).  packed [n][groups*group/2]
  * u8: two codes (0..15) per byte, the even column in the low half; scales
- * [n][groups] (scale_dtype); zeros [n][groups] u8 (nullable: 8); bias [n]
+ * [n][groups] (scale_dtype); zeros [n][groups] u8 (0..15; nullable: 8); bias [n]
  * (dtype, nullable).  groups = ceil(k/group), group a multiple of 32; codes of
  * columns >= k are ignored.  x [rows][k] (row stride x_stride elements), y
  * [rows][n] dense, both `dtype`; sums in fp32, one rounding.  packed must be

@@ -1258,6 +1258,9 @@ extern "C" int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, 
   if (op->batch * op->tokens == 0) return SPR_OK;
   if (!op->x || !op->mean || !op->rstd || !grad->dh || !grad->dx || (op->y && !grad->dy) || (grad->dgate && !op->y))
     return fail(SPR_ERR_ARG, "adaln backward: null operand");
+  for (auto [p, sb, st] : {std::tuple(op->scale, op->scale_sb, op->scale_st), std::tuple(op->gate, op->gate_sb, op->gate_st)})
+    if (p && ((sb && op->batch > 1 && !grad->mod_batch) || (st && op->tokens > 1 && !grad->mod_tokens)))
+      return fail(SPR_ERR_ARG, "adaln backward: a vector has a stride along an axis that its gradient is summed over");
   const size_t need =
       spr_adaln_backward_workspace_bytes(op->batch, op->tokens, op->channels, grad->mod_batch, grad->mod_tokens);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))

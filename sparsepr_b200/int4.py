@@ -21,7 +21,7 @@ __all__ = ["Int4Weight", "quantize_int4", "dequantize_int4", "int4_linear"]
 
 class Int4Weight(NamedTuple):
     """``packed`` uint8 [N, groups*group/2] (two codes a byte, the even column in the low
-    half), ``scales`` [N, groups], ``zeros`` uint8 [N, groups] or None (8)."""
+    half), ``scales`` [N, groups], ``zeros`` uint8 [N, groups], 0 to 15, or None (8)."""
 
     packed: torch.Tensor
     scales: torch.Tensor

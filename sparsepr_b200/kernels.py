@@ -697,13 +697,15 @@ def int4_linear(x, packed, scales, zeros=None, bias=None) -> torch.Tensor:
     for a few rows ``x`` [R,K] (row stride free) -> [R,N] in x's type.
 
     ``packed`` uint8 [N, groups*group/2]: two 4-bit codes a byte, the even column in
-    the low half; ``scales`` [N, groups]; ``zeros`` uint8 [N, groups] (None: 8).  The
+    the low half; ``scales`` [N, groups]; ``zeros`` uint8 [N, groups], 0 to 15 (None: 8).  The
     group size is a multiple of 32; codes of columns >= K are ignored."""
     _cuda(x, packed, scales, zeros, bias)
     r, k = x.shape
     n, group = _int4_checks("int4_linear", x, k, packed, scales, zeros)
-    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or (n > 1 and bias.stride(0) != 1)):
-        raise RuntimeError(f"int4_linear: bias must be contiguous {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
+    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,) or (n > 1 and bias.stride(0) != 1)
+                             or bias.get_device() != x.get_device()):
+        raise RuntimeError(f"int4_linear: bias must be contiguous {x.dtype} [{n}] on {x.device}, got {bias.dtype} "
+                           f"{tuple(bias.shape)} on {bias.device}")
     y = x.new_empty((r, n))
     nbytes = _lib.query("spr_int4_linear_workspace_bytes", r, n, k, group, _DT[x.dtype])
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None

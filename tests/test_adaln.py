@@ -76,6 +76,11 @@ def test_c_entries_refuse_before_any_launch():
     with pytest.raises(RuntimeError, match="SPR_ERR_ARG"):
         o = op()  # no statistics
         _lib.call("spr_adaln_backward", ctypes.addressof(o), ctypes.addressof(gr), 256, 1 << 20, None)
+    for kw in (dict(scale=256, scale_st=8), dict(y=256, gate=256, gate_st=8), dict(batch=2, scale=256, scale_sb=8)):
+        gr = _lib.SprAdalnGrad(dh=256, dx=256, dy=256, dscale=256)  # the strides say that the vectors differ
+        o = op(mean=256, rstd=256, **kw)
+        with pytest.raises(RuntimeError, match="summed over"):
+            _lib.call("spr_adaln_backward", ctypes.addressof(o), ctypes.addressof(gr), 256, 1 << 30, None)
 
 
 # ---------------------------------------------------------------- 64-bit reference
