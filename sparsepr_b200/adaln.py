@@ -15,8 +15,9 @@ adjacent: one vector, one per sample ([B, 1, C]), one per token ([B, N, C] or
 normalised, so the norm reads what the residual stream holds.  Statistics and
 sums are fp32, and the gradients of shared vectors are summed in a fixed order.
 
-The gradients are of first order.  A call captured into a CUDA graph needs what
-any captured autograd call needs; :func:`operands` with
+The gradients are of first order.  A backward pass captured into a CUDA graph needs
+what any captured autograd call needs: warm-up passes on a side stream, and no graph
+of an uncaptured forward pass over the same leaves still alive.  :func:`operands` with
 :func:`sparsepr_b200.kernels.adaln_forward` and ``adaln_backward`` are the same passes
 without autograd.
 """
@@ -152,7 +153,9 @@ def _backward(ctx, *grads):
             setattr(s, name + "_st", st)
     mean = stats.data_ptr()
     s.mean, s.rstd = mean, mean + 4 * stats.shape[1]
-    return *K.adaln_backward_struct(s, y is not None, dh, dz, ctx.needs_input_grad[2:5], mod_shape, vector_shape, mod_dtype), None, None
+    grads = K.adaln_backward_struct(s, y is not None, dh, dz, ctx.needs_input_grad[2:5], mod_shape, vector_shape,
+                                    mod_dtype)
+    return *grads, None, None
 
 
 _backward_once = once_differentiable(_backward)

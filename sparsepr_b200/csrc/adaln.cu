@@ -3,7 +3,10 @@
 //   z = x + gate*y,  n = (z - mean z) * rstd,  h = n*w + shift,  w = offset + scale
 //   u = dh*w,  g = dz + rstd*(u - mean u - n*mean(u*n)),  dx = g,  dy = g*gate
 //   dshift = sum dh,  dscale = sum dh*n,  dgate = sum g*y   over the rows of a group
-// Statistics and sums are fp32.
+// Statistics and sums are fp32, and each result is rounded once.  A row is read once
+// and written once a pass, 2 to 4 fp32 operations a byte, so HBM bounds every pass of
+// more than a few hundred rows; below that the launch does.  Bandwidths in this
+// file are of B200's measured copy, 6.56 TB/s, under a sustained load.
 #include <atomic>
 #include <tuple>
 #include <type_traits>
@@ -281,7 +284,10 @@ __device__ __forceinline__ float2 row_stats(const Vals<V> (&z)[P], int lane, int
   return make_float2(mean, rsqrtf(m2 * inv_c + eps));
 }
 
-// One row per team, kept in registers: any width, and a vector for every row.
+// One row per team, kept in registers: few rows, any width and alignment, and the
+// widest rows with a vector each.  A row of four tokens of 5120 takes 3 us, all of
+// it latency.  Single elements (odd widths) are bound by their instructions, one load
+// an element: 30,000 x 1537 bf16 202 us, 14%.
 template <typename T, typename MT, int V, int P, bool kRes>
 __global__ void __launch_bounds__(1024) adaln_forward_kernel(const SprAdaln op, int team) {
   __shared__ float4 red[32];
@@ -434,6 +440,8 @@ using BackwardVectors = std::conditional_t<kRes, RowVectors<T, MT, P, kRow, kSca
 // the copies need no barrier and stay in flight across the one that joins a row's
 // statistics.  kFull: every thread has all of its P vectors.  kRow: each row has
 // vectors of its own, which are streamed as the rows are.
+// 75,600 x 5120 bf16: 249 us (95%), gated with fp32 vectors 490 us (96%); 60,000 x 2048
+// fp32 gated 317 us (94%); 40,000 x 1536 bf16 gated with vectors for every row 136 us (97%).
 template <typename T, typename MT, int P, bool kRes, bool kFull, bool kRow, int kThreads, int kMin, int kStages>
 __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(const SprAdaln op, const Groups gp) {
   constexpr int V = kVec<T>, kIn = kRes ? 2 : 1, e = sizeof(T);
@@ -623,7 +631,8 @@ __device__ __forceinline__ void store_sums(const SprAdalnGrad& gr, const Groups&
 
 // Any width: a CTA takes one run of a group, its teams every other row of it, and
 // joins the teams' column sums at the end; with `own` each team takes a run by
-// itself (groups of few rows, such as a vector for every token).
+// itself (groups of few rows, such as a vector for every token).  75,600 x 64 bf16 17 us
+// (26%); single elements are bound by their instructions (30,000 x 1537 bf16 428 us, 10%).
 template <typename T, typename MT, int V, int P, bool kRes>
 __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op, const SprAdalnGrad gr,
                                                               const Groups gp, int team, int own, float* partial) {
@@ -732,6 +741,8 @@ __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op,
 // kAgain: n and u are formed again after the barrier instead of held across it
 // (512 threads have 128 registers each; held, they spill).  kRow: each row has vectors
 // of its own; they are streamed as the rows are, and so are their gradients.
+// 75,600 x 5120 bf16: 372 us (95%), gated with fp32 vectors 740 us (96%), both with the join;
+// 40,000 x 1536 bf16 gated with vectors for every row 210 us (98%).
 constexpr int kStatRows = 256;  // rows whose statistics are in shared memory at a time
 template <typename T, typename MT, int P, bool kRes, bool kFull, bool kRow, bool kAgain, int R, int kThreads, int kStages>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -895,7 +906,8 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
     }
 }
 
-// Joins the runs' column sums in their order: 32 columns by 32 threads each.
+// Joins the runs' column sums in their order: 32 columns by 32 threads each, each thread
+// every 32nd run.  The sums mostly still lie in L2: 6 to 27 MB in 8 to 13 us.
 template <typename MT>
 __global__ void __launch_bounds__(1024) adaln_join_kernel(const SprAdalnGrad gr, int c, int chunks,
                                                           const float* partial) {

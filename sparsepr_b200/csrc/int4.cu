@@ -16,6 +16,12 @@
 // * fp32 x, and more rows than the integer columns hold: bf16 products (m16n8k16).  A
 //   code is the exact integer code - zero, and x is cut into as many bf16 parts as
 //   its significand needs (bf16 1, fp16 2, fp32 3; exact), each a column.
+// Measured on B200 (copy bandwidth 6.56 TB/s), 245,760 x 5120 codes: two bf16 rows,
+// groups of 128 137 us (73% of the copy's bytes a second), one row, groups of 64 151 us;
+// the schedulers issue in 55% to 60% of all cycles, waiting for one another's
+// products.  fp32 rows (three parts) 122,880 x 5120, groups of 64: 113 us.  The gradient
+// has more to do a code (pairs of weight rows are formed, and the other operand for each
+// group): 122,880 x 5120 two rows, groups of 128 198 us; 30,720 x 5120 four rows 72 us.
 // The 5th-generation tensor instructions work on 128 rows: with so few, they would
 // idle, and their operands would pass through shared memory again once unpacked.
 #include <math.h>
@@ -303,7 +309,9 @@ __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int 
 }
 
 // y for up to NT*8 columns (a row's parts or bytes each one): warp products of 16 weight
-// rows by 32 columns of the weight a step.
+// rows by 32 columns of the weight a step.  Each warp copies its own codes three
+// chunks (6 KB) ahead and needs no other warp until its tile ends, so that an SM has
+// about 100 KB in flight; the CTA's slice of x is laid out in shared memory once.
 template <int NT, int GB, bool kInt, int kScale>
 __global__ void __launch_bounds__(most_warps(NT) * 32, 1)
 int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, float up, const void* bias, void* y,

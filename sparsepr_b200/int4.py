@@ -100,7 +100,9 @@ def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zer
 
     ``x`` [..., K] in fp32, bf16 or fp16 and ``bias`` [N] in x's type; the result [..., N]
     is rounded once from fp32 sums.  Any number of rows is computed, but the
-    weights are read once for each block of rows: the call is for a few rows."""
+    weights are read once for each block of rows: the call is for a few rows.  A backward
+    pass captured into a CUDA graph needs what any captured autograd call needs: no graph
+    of an uncaptured forward pass over the same leaves still alive."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"int4_linear: x must be [..., K], got {tuple(x.shape)}")
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
