@@ -568,6 +568,199 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
+// Rows that 16-byte vectors do not fit (odd widths, odd strides or offsets), in long
+// groups: a CTA that stays on its SM copies the aligned 16-byte pieces which hold a
+// row into shared memory, some rows ahead, and its threads take every team-th
+// element from there, so that a thread's columns, and its part of the vectors, are
+// the same in every row.  The first piece may begin before the row (inside the
+// allocation: these begin on multiples of 16 bytes); the last is cut at its end.
+// One barrier a row: it joins the row's sums, shows every thread the next row, and
+// lets the row before be overwritten.
+struct Window {
+  const char* at;  // the next row to copy; null: none is
+  int64_t step;
+  int row_bytes, off;
+  uint32_t phase;  // where the row at work begins in its first piece
+  __device__ __forceinline__ Window() : at(nullptr), step(0), row_bytes(0), off(0), phase(0) {}
+  __device__ __forceinline__ Window(const Run& run, const void* base, int64_t sb, int64_t st, int e, int c, int off)
+      : at(base ? (const char*)base + (run.first.b * sb + run.first.t * st) * e : nullptr),
+        step((run.step == 1 ? st : sb) * e), row_bytes(c * e), off(off), phase((uint32_t)(uintptr_t)at & 15) {}
+  __device__ __forceinline__ void copy(char* slot) {
+    if (!at) return;
+    const int shift = (int)((uintptr_t)at & 15), bytes = shift + row_bytes;
+    for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       (uint32_t)__cvta_generic_to_shared(slot + off + i)),
+                   "l"(at - shift + i), "r"(min(16, bytes - i))
+                   : "memory");
+    at += step;
+  }
+  __device__ __forceinline__ void advance() { phase = (phase + (uint32_t)step) & 15; }
+  // The thread's elements of the row in a slot, zeros past the end.
+  template <typename U, int P>
+  __device__ __forceinline__ void read(const char* slot, int c, Vals<P>& f) const {
+    const U* p = reinterpret_cast<const U*>(slot + off + phase) + threadIdx.x;
+    const int team = blockDim.x;
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      const int col = threadIdx.x + 2 * i * team;
+      f.q[i] = pair(col < c ? to_f32(p[2 * i * team]) : 0.f, col + team < c ? to_f32(p[(2 * i + 1) * team]) : 0.f);
+    }
+  }
+};
+// Bytes that a row of at most `c` elements takes in a slot.
+constexpr int window_bytes(int c, int e) { return (c * e + 15 + 15) / 16 * 16; }
+
+// The thread's elements of a vector or a row in memory.
+template <typename U, int P>
+__device__ __forceinline__ void load_columns(const U* p, int c, Vals<P>& f) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) {
+    const int a = threadIdx.x + 2 * i * blockDim.x, b = a + blockDim.x;
+    f.q[i] = pair(a < c ? to_f32(__ldg(p + a)) : 0.f, b < c ? to_f32(__ldg(p + b)) : 0.f);
+  }
+}
+template <typename U, int P>
+__device__ __forceinline__ void store_columns(U* p, int c, const Vals<P>& f) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) {
+    const int a = threadIdx.x + 2 * i * blockDim.x, b = a + blockDim.x;
+    const float2 v = halves(f.q[i]);
+    if (a < c) p[a] = from_f32<U>(v.x);
+    if (b < c) p[b] = from_f32<U>(v.y);
+  }
+}
+template <int P>
+__device__ __forceinline__ void add_offset(Vals<P>& w, float offset) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) w.q[i] = add2(w.q[i], pair(offset, offset));
+}
+__device__ __forceinline__ void wait_for_next_row(int stages) {
+  if (stages == 4) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T, typename MT, int P, bool kRes, bool kRow>
+__global__ void __launch_bounds__(512, 1)
+adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slot_bytes) {
+  __shared__ float2 red[2][16];
+  extern __shared__ uint4 ring[];
+  const int c = op.channels, team = blockDim.x, lane = threadIdx.x, warps = team / 32, e = sizeof(T), me = sizeof(MT);
+  const Run run(op, gp, blockIdx.x);
+  const int row_place = window_bytes(team * P, e), vec_place = window_bytes(team * P, me);
+  Window x(run, op.x, op.x_sb, op.x_st, e, c, 0), y, scale, shift, gate;
+  if constexpr (kRes) y = Window(run, op.y, op.y_sb, op.y_st, e, c, row_place);
+  if constexpr (kRow) {
+    constexpr int rows = kRes ? 2 : 1;
+    scale = Window(run, op.scale, op.scale_sb, op.scale_st, me, c, rows * row_place);
+    shift = Window(run, op.shift, op.shift_sb, op.shift_st, me, c, rows * row_place + vec_place);
+    if constexpr (kRes) gate = Window(run, op.gate, op.gate_sb, op.gate_st, me, c, rows * row_place + 2 * vec_place);
+  }
+  auto elements = [&](int w) {
+    int n = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) n += min(max(c - 32 * w - p * team, 0), 32);
+    return (float)n;
+  };
+  const int who = lane & 15;
+  const float n_who = who < warps ? elements(who) : 0.f;
+  const float inv_who = n_who > 0.f ? __frcp_rn(n_who) : 0.f;
+  const float inv_n = __frcp_rn(elements(lane >> 5)), inv_c = __frcp_rn((float)c);
+  if (lane < 32) red[lane >> 4][lane & 15] = make_float2(0.f, 0.f);
+  int fetched = 0;
+  auto fetch = [&](int stage) {
+    if (fetched++ < run.rows) {
+      char* slot = reinterpret_cast<char*>(ring) + stage * slot_bytes;
+      x.copy(slot);
+      if constexpr (kRes) y.copy(slot);
+      if constexpr (kRow) {
+        scale.copy(slot);
+        shift.copy(slot);
+        if constexpr (kRes) gate.copy(slot);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int i = 0; i < stages - 1; ++i) fetch(i);
+  Vals<P> w, b, g;
+  w.fill(1.f);
+  b.fill(0.f);
+  g.fill(1.f);
+  if constexpr (!kRow) {
+    const RowId& id = run.group;
+    if (op.scale) {
+      load_columns<MT, P>((const MT*)op.scale + id.b * op.scale_sb + id.t * op.scale_st, c, w);
+      add_offset<P>(w, op.scale_offset);
+    }
+    if (op.shift) load_columns<MT, P>((const MT*)op.shift + id.b * op.shift_sb + id.t * op.shift_st, c, b);
+    if (kRes && op.gate) load_columns<MT, P>((const MT*)op.gate + id.b * op.gate_sb + id.t * op.gate_st, c, g);
+  }
+  if (stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncthreads();
+  int stage = 0;
+  for (int r = 0; r < run.rows; ++r) {
+    const char* slot = reinterpret_cast<const char*>(ring) + stage * slot_bytes;
+    const int64_t row = run.row0 + r * run.step;
+    Vals<P> z;
+    x.read<T, P>(slot, c, z);
+    if constexpr (kRes) {
+      Vals<P> yv;
+      y.read<T, P>(slot, c, yv);
+      if (kRow && gate.at) gate.read<MT, P>(slot, c, g);
+      residual<T, P>(z, yv, g);
+      store_columns<T, P>((T*)op.z + row * c, c, z);
+    }
+    uint64_t acc[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) acc[i & 1] = add2(acc[i & 1], z.q[i]);
+    float2 h = halves(add2(acc[0], acc[1]));
+    const float sum = warp_sum(h.x + h.y);
+    const float near = -sum * inv_n;
+    acc[0] = acc[1] = 0;
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      const float2 d = halves(add2(z.q[i], pair(near, near)));
+      const int col = lane + 2 * i * team;
+      const uint64_t in = pair(col < c ? d.x : 0.f, col + team < c ? d.y : 0.f);
+      acc[i & 1] = fma2(in, in, acc[i & 1]);
+    }
+    h = halves(add2(acc[0], acc[1]));
+    const float m2 = warp_sum(h.x + h.y);
+    if ((lane & 31) == 0) red[r & 1][lane >> 5] = make_float2(sum, m2);
+    wait_for_next_row(stages);
+    __syncthreads();
+    fetch(stage == 0 ? stages - 1 : stage - 1);
+    // M2 = sum_w M2_w + n_w (mean_w - mean)^2, a warp's values in each of 16 lanes.
+    const float2 part = red[r & 1][who];
+    const float mean = sum16(part.x) * inv_c;
+    const float off = fmaf(part.x, inv_who, -mean);
+    const float rstd = rsqrtf(sum16(fmaf(off * off, n_who, part.y)) * inv_c + op.eps);
+    if constexpr (kRow) {
+      if (scale.at) {
+        scale.read<MT, P>(slot, c, w);
+        add_offset<P>(w, op.scale_offset);
+      }
+      if (shift.at) shift.read<MT, P>(slot, c, b);
+    }
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i)
+      z.q[i] = fma2(mul2(add2(z.q[i], pair(-mean, -mean)), pair(rstd, rstd)), w.q[i], b.q[i]);
+    store_columns<T, P>((T*)op.h + row * c, c, z);
+    if (lane == 0 && op.mean) {
+      op.mean[row] = mean;
+      op.rstd[row] = rstd;
+    }
+    x.advance();
+    y.advance();
+    scale.advance();
+    shift.advance();
+    gate.advance();
+    stage = stage + 1 == stages ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // The row arithmetic that both backward kernels share: n = (z - mean)*rstd, u = dh*w
 // and a lane's sums before the reduction, the gradients after it.
 template <int V, int P>
@@ -906,6 +1099,134 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
     }
 }
 
+// The backward pass of rows that 16-byte vectors do not fit, as the forward pass takes them.
+template <typename T, typename MT, int P, bool kRes, bool kRow>
+__global__ void __launch_bounds__(512, 1)
+adaln_backward_any_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups gp, int stages, int slot_bytes,
+                          float* partial) {
+  __shared__ uint64_t red[2][16];
+  extern __shared__ uint4 ring[];
+  const int c = op.channels, team = blockDim.x, lane = threadIdx.x, e = sizeof(T), me = sizeof(MT);
+  const Run run(op, gp, blockIdx.x);
+  const int row_place = window_bytes(team * P, e), vec_place = window_bytes(team * P, me);
+  Window x(run, op.x, op.x_sb, op.x_st, e, c, 0), dh(run, gr.dh, gr.dh_sb, gr.dh_st, e, c, row_place), y, dz, scale,
+      gate;
+  if constexpr (kRes) {
+    y = Window(run, op.y, op.y_sb, op.y_st, e, c, 2 * row_place);
+    dz = Window(run, gr.dz, gr.dz_sb, gr.dz_st, e, c, 3 * row_place);
+  }
+  if constexpr (kRow) {
+    constexpr int rows = kRes ? 4 : 2;
+    scale = Window(run, op.scale, op.scale_sb, op.scale_st, me, c, rows * row_place);
+    if constexpr (kRes) gate = Window(run, op.gate, op.gate_sb, op.gate_st, me, c, rows * row_place + vec_place);
+  }
+  const float inv_c = 1.f / c;
+  if (lane < 32) (&red[0][0])[lane] = 0;
+  int fetched = 0;
+  auto fetch = [&](int stage) {
+    if (fetched++ < run.rows) {
+      char* slot = reinterpret_cast<char*>(ring) + stage * slot_bytes;
+      x.copy(slot);
+      dh.copy(slot);
+      if constexpr (kRes) {
+        y.copy(slot);
+        dz.copy(slot);
+      }
+      if constexpr (kRow) {
+        scale.copy(slot);
+        if constexpr (kRes) gate.copy(slot);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int i = 0; i < stages - 1; ++i) fetch(i);
+  Vals<P> w, gv;
+  w.fill(1.f);
+  gv.fill(1.f);
+  if constexpr (!kRow) {
+    const RowId& id = run.group;
+    if (op.scale) {
+      load_columns<MT, P>((const MT*)op.scale + id.b * op.scale_sb + id.t * op.scale_st, c, w);
+      add_offset<P>(w, op.scale_offset);
+    }
+    if (kRes && op.gate) load_columns<MT, P>((const MT*)op.gate + id.b * op.gate_sb + id.t * op.gate_st, c, gv);
+  }
+  Sums<P, 1> st;
+  st.clear();
+  float next_mean = op.mean[run.row0], next_rstd = op.rstd[run.row0];
+  if (stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncthreads();
+  int stage = 0;
+  for (int r = 0; r < run.rows; ++r) {
+    const char* slot = reinterpret_cast<const char*>(ring) + stage * slot_bytes;
+    const int64_t row = run.row0 + r * run.step;
+    const uint64_t minus = pair(-next_mean, -next_mean), rs = pair(next_rstd, next_rstd);
+    if (r + 1 < run.rows) {
+      next_mean = op.mean[row + run.step];
+      next_rstd = op.rstd[row + run.step];
+    }
+    Vals<P> z, d, n, u;
+    x.read<T, P>(slot, c, z);
+    dh.read<T, P>(slot, c, d);
+    if (kRow && scale.at) {
+      scale.read<MT, P>(slot, c, w);
+      add_offset<P>(w, op.scale_offset);
+    }
+    if constexpr (kRow) st.clear();  // a row's own: written below, not added up
+    uint64_t s0 = 0, s1 = 0;
+    st.first(0, z, d, w, minus, rs, n, u, s0, s1);
+    if constexpr (kRow) {
+      if (gr.dshift) store_columns<MT, P>((MT*)gr.dshift + row * c, c, st.shift[0]);
+      if (gr.dscale) store_columns<MT, P>((MT*)gr.dscale + row * c, c, st.scale[0]);
+    }
+    const float2 a = halves(s0), b = halves(s1);
+    uint64_t sums = team_sum2(pair(a.x + a.y, b.x + b.y), 32);
+    if ((lane & 31) == 0) red[r & 1][lane >> 5] = sums;
+    wait_for_next_row(stages);
+    __syncthreads();
+    fetch(stage == 0 ? stages - 1 : stage - 1);
+    sums = red[r & 1][lane & 15];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sums = add2(sums, __shfl_xor_sync(0xffffffffu, sums, o, 16));
+    const float2 m = halves(sums);
+    Vals<P> g, dzv;
+    dzv.fill(0.f);
+    if (kRes && dz.at) dz.read<T, P>(slot, c, dzv);
+    second<P>(n, u, pair(-m.x * inv_c, -m.x * inv_c), pair(-m.y * inv_c, -m.y * inv_c), rs, dzv, g);
+    if constexpr (kRes) {
+      Vals<P> yv, dy = gv;
+      y.read<T, P>(slot, c, yv);
+      if (kRow && gate.at) gate.read<MT, P>(slot, c, dy);
+      st.branch(0, g, yv, dy);
+      if (kRow && gr.dgate) store_columns<MT, P>((MT*)gr.dgate + row * c, c, st.gate[0]);
+      store_columns<T, P>((T*)gr.dy + row * c, c, dy);
+    }
+    store_columns<T, P>((T*)gr.dx + row * c, c, g);
+    x.advance();
+    dh.advance();
+    y.advance();
+    dz.advance();
+    scale.advance();
+    gate.advance();
+    stage = stage + 1 == stages ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (!kRow) {
+    if (gp.chunks == 1) {
+      const int64_t at = (int64_t)blockIdx.x * c;
+      if (gr.dshift) store_columns<MT, P>((MT*)gr.dshift + at, c, st.shift[0]);
+      if (gr.dscale) store_columns<MT, P>((MT*)gr.dscale + at, c, st.scale[0]);
+      if (gr.dgate) store_columns<MT, P>((MT*)gr.dgate + at, c, st.gate[0]);
+    } else {
+      float* p = partial + (int64_t)blockIdx.x * 3 * c;
+      if (gr.dshift) store_columns<float, P>(p, c, st.shift[0]);
+      if (gr.dscale) store_columns<float, P>(p + c, c, st.scale[0]);
+      if (gr.dgate) store_columns<float, P>(p + 2 * c, c, st.gate[0]);
+    }
+  }
+}
+
 // Joins the runs' column sums in their order: 32 columns by 32 threads each, each thread
 // every 32nd run.  The sums mostly still lie in L2: 6 to 27 MB in 8 to 13 us.
 template <typename MT>
@@ -1026,6 +1347,7 @@ int by_shape(bool vec, int per, F f) {
   return f(Int<1>{}, Int<16>{});
 }
 
+constexpr int kAnySmem = 200 * 1024;
 constexpr int kCtaThreads = 256;  // of a CTA whose teams are at most a warp
 
 // Whether a run's rows are equally spaced in every operand: within one sample, or
@@ -1103,6 +1425,63 @@ int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
   return check_launch("adaln forward");
 }
 
+// Slots of a row's operands that a CTA holds: 4, or 3, or 0 where they do not fit.
+int any_stages(int slot_bytes) { return 4 * slot_bytes <= kAnySmem ? 4 : 3 * slot_bytes <= kAnySmem ? 3 : 0; }
+template <typename T, typename MT, bool kRes, bool kRow, bool kBackward>
+int any_slot(int columns) {
+  const int rows = kBackward ? (kRes ? 4 : 2) : kRes ? 2 : 1;
+  const int vecs = kRow ? (kBackward ? (kRes ? 2 : 1) : kRes ? 3 : 2) : 0;
+  return rows * window_bytes(columns, sizeof(T)) + vecs * window_bytes(columns, sizeof(MT));
+}
+// Columns a thread: 8, which keeps the vectors and sums of a wide row in registers,
+// or 16 where 512 threads need them.
+constexpr int any_per(int channels) { return channels <= 512 * 8 ? 8 : 16; }
+template <typename T, typename MT, bool kRes, bool kRow, bool kBackward>
+bool any_fits(int channels) {
+  const int per = any_per(channels), team = cta_for(channels, per);
+  return channels >= 64 && team <= 512 && any_stages(any_slot<T, MT, kRes, kRow, kBackward>(team * per)) > 0;
+}
+
+template <typename T, typename MT, bool kRes, bool kRow, int P>
+int launch_forward_any(const SprAdaln* op, Groups g, cudaStream_t st) {
+  constexpr auto kern = adaln_forward_any_kernel<T, MT, P, kRes, kRow>;
+  const int team = cta_for(op->channels, P), slot = any_slot<T, MT, kRes, kRow, false>(team * P);
+  const int stages = any_stages(slot), smem = stages * slot;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kAnySmem) != cudaSuccess)
+    return check_launch("adaln forward");
+  cut_stream(g, (int64_t)sm_count() * resident<kern>(team, smem), slot, 6, 65536, INT64_MAX);
+  kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, g, stages, slot);
+  return check_launch("adaln forward");
+}
+template <typename T, typename MT, bool kRes, bool kRow>
+int launch_forward_any(const SprAdaln* op, const Groups& g, cudaStream_t st) {
+  return any_per(op->channels) == 8 ? launch_forward_any<T, MT, kRes, kRow, 8>(op, g, st)
+                                    : launch_forward_any<T, MT, kRes, kRow, 16>(op, g, st);
+}
+
+template <typename MT>
+int join(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, const float* partial, cudaStream_t st);
+int64_t most_runs(int channels);
+
+template <typename T, typename MT, bool kRes, bool kRow, int P>
+int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, float* partial, cudaStream_t st) {
+  constexpr auto kern = adaln_backward_any_kernel<T, MT, P, kRes, kRow>;
+  const int team = cta_for(op->channels, P), slot = any_slot<T, MT, kRes, kRow, true>(team * P);
+  const int stages = any_stages(slot), smem = stages * slot;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kAnySmem) != cudaSuccess)
+    return check_launch("adaln backward");
+  cut_stream(g, (int64_t)sm_count() * resident<kern>(team, smem), slot, kRow || kRes ? 6 : 1, kRow ? 65536 : 3 << 19,
+             kRow ? INT64_MAX : most_runs(op->channels));
+  kern<<<(unsigned)(g.count * g.chunks), team, smem, st>>>(*op, *gr, g, stages, slot, partial);
+  if constexpr (kRow) return check_launch("adaln backward");
+  return join<MT>(op, gr, g, partial, st);
+}
+template <typename T, typename MT, bool kRes, bool kRow>
+int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, float* partial, cudaStream_t st) {
+  return any_per(op->channels) == 8 ? launch_backward_any<T, MT, kRes, kRow, 8>(op, gr, g, partial, st)
+                                    : launch_backward_any<T, MT, kRes, kRow, 16>(op, gr, g, partial, st);
+}
+
 // Whether P/2 vectors a thread leave fewer idle places in a CTA of at most 512.
 bool half_fits_better(int nvec, int P) {
   const int half = cta_for(nvec, P / 2);
@@ -1142,6 +1521,13 @@ int launch_forward(const SprAdaln* op, cudaStream_t st) {
                              : launch_forward_stream<T, MT, kRes, P, true, false, 512, 1>(op, g, st);
     if (half_fits_better(nvec, P)) return launch_forward_stream<T, MT, kRes, P / 2, false, false, 512, 1>(op, g, st);
     return launch_forward_stream<T, MT, kRes, P, false, false, 512, 1>(op, g, st);
+  }
+  if (!vec) {
+    const bool own = kept(op->scale_st, op->shift_st, op->gate_st);
+    if (own && op->tokens >= 8 && any_fits<T, MT, kRes, true, false>(op->channels))
+      return launch_forward_any<T, MT, kRes, true>(op, make_groups(op->batch, op->tokens, 1, 0), st);
+    if (!own && g.rows >= 8 && even_rows(g, op->batch) && any_fits<T, MT, kRes, false, false>(op->channels))
+      return launch_forward_any<T, MT, kRes, false>(op, g, st);
   }
   return by_shape<T>(vec, forward_per_thread<T>(vec, nvec), [&](auto v, auto p) {
     constexpr int V = decltype(v)::value, P = decltype(p)::value;
@@ -1215,6 +1601,13 @@ int launch_backward(const SprAdaln* op, const SprAdalnGrad* gr, float* partial, 
     if (half_fits_better(nvec, kPer))
       return launch_backward_stream<T, MT, kRes, kPer / 2, false, false, false, 1, 512>(op, gr, g, partial, st);
     return launch_backward_stream<T, MT, kRes, kPer, false, false, kRes, 1, kWide>(op, gr, g, partial, st);
+  }
+  if (!vec) {
+    if (gr->mod_tokens && op->tokens >= 8 && (gr->mod_batch || op->batch == 1) &&
+        any_fits<T, MT, kRes, true, true>(op->channels))
+      return launch_backward_any<T, MT, kRes, true>(op, gr, make_groups(op->batch, op->tokens, 1, 0), partial, st);
+    if (!gr->mod_tokens && g.rows >= 8 && even_rows(g, op->batch) && any_fits<T, MT, kRes, false, true>(op->channels))
+      return launch_backward_any<T, MT, kRes, false>(op, gr, g, partial, st);
   }
   const int per = nvec <= 32 ? 1 : vec ? (nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : 4) : nvec <= 4096 ? 4 : 16;
   return by_shape<T>(vec, per, [&](auto v, auto p) {

@@ -240,6 +240,31 @@ def test_values_and_gradients(cuda, gated, b, n, c, dtype, mod_dtype, mods):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("b,n,c,dtype,mod_dtype,mods,pad", [
+    (1, 70, 1537, BF, BF, "vector", 0),
+    (1, 2000, 1537, BF, FP, "vector", 0),  # several runs of rows
+    (2, 40, 1003, FP, FP, "sample", 0),
+    (1, 33, 65, HF, HF, "token", 0),
+    (2, 20, 4099, BF, FP, "token", 0),     # three slots of gated rows; the gradient's do not fit
+    (1, 30, 8191, HF, HF, "vector", 0),
+    (3, 17, 2049, FP, FP, "token", 0),
+    (1, 24, 5001, FP, FP, "vector", 0),
+    (3, 21, 777, BF, BF, "shared", 0),
+    (2, 45, 512, BF, BF, "vector", 1),     # rows of whole vectors at odd addresses and strides
+    (3, 19, 1024, FP, FP, "sample", 3),
+    (2, 23, 640, HF, FP, "token", 5),
+])
+def test_rows_that_no_vectors_fit(cuda, gated, b, n, c, dtype, mod_dtype, mods, pad):
+    v = _inputs(cuda, b, n, c, dtype, mod_dtype, mods, seed=c + n)
+    for name in ("x", "y") if pad else ():
+        wide = v[name].new_full((b, n, c + pad), float("nan"))
+        wide[..., pad:] = v[name]
+        v[name] = wide[..., pad:]
+    _check(v, gated)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_affine_layer_norm(cuda, dtype):
     v = _inputs(cuda, 1, 77, 1003, dtype, FP, "vector", seed=5)
