@@ -285,9 +285,7 @@ __device__ __forceinline__ float2 row_stats(const Vals<V> (&z)[P], int lane, int
 }
 
 // One row per team, kept in registers: few rows, any width and alignment, and the
-// widest rows with a vector each.  A row of four tokens of 5120 takes 3 us, all of
-// it latency.  Single elements (odd widths) are bound by their instructions, one load
-// an element: 30,000 x 1537 bf16 202 us, 14%.
+// widest rows with a vector each.  Four rows of 5120 take 3 us, all of it latency.
 template <typename T, typename MT, int V, int P, bool kRes>
 __global__ void __launch_bounds__(1024) adaln_forward_kernel(const SprAdaln op, int team) {
   __shared__ float4 red[32];
@@ -570,65 +568,79 @@ __global__ void __launch_bounds__(kThreads, kMin) adaln_forward_stream_kernel(co
 
 // Rows that 16-byte vectors do not fit (odd widths, odd strides or offsets), in long
 // groups: a CTA that stays on its SM copies the aligned 16-byte pieces which hold a
-// row into shared memory, some rows ahead, and its threads take every team-th
-// element from there, so that a thread's columns, and its part of the vectors, are
-// the same in every row.  The first piece may begin before the row (inside the
-// allocation: these begin on multiples of 16 bytes); the last is cut at its end.
-// One barrier a row: it joins the row's sums, shows every thread the next row, and
-// lets the row before be overwritten.
+// row into shared memory, some rows ahead.  A warp takes 32*P neighbouring columns, a
+// thread every 32nd of them: its columns, and its part of the vectors, are the same
+// in every row, at constant distances.  The first piece may begin before the row
+// (inside the allocation: these begin on multiples of 16 bytes); the last is cut at its
+// end and zeros fill the place up, so that only stores and the variance look at the
+// width, in the last warp.  One barrier a row: it joins the row's sums, shows every
+// thread the next row, and lets the row before be overwritten.
+// Bound by instructions, a load, a conversion and a store for every element: 30,000 x 1003
+// fp32 47 us (78% of bandwidth), gated 92 us (80%); 16-bit elements are twice as many
+// for the bytes: 30,000 x 1537 bf16 66 us (43%), gated 117 us (48%).
+template <int P>
+__device__ __forceinline__ int first_column() { return (threadIdx.x & ~31) * P + (threadIdx.x & 31); }
+// Bytes that a row of at most `c` elements takes in a slot.
+__host__ __device__ constexpr int window_bytes(int c, int e) { return (c * e + 15 + 15) / 16 * 16; }
 struct Window {
   const char* at;  // the next row to copy; null: none is
   int64_t step;
-  int row_bytes, off;
+  int row_bytes, place_bytes, off;
   uint32_t phase;  // where the row at work begins in its first piece
-  __device__ __forceinline__ Window() : at(nullptr), step(0), row_bytes(0), off(0), phase(0) {}
+  __device__ __forceinline__ Window() : at(nullptr), step(0), row_bytes(0), place_bytes(0), off(0), phase(0) {}
   __device__ __forceinline__ Window(const Run& run, const void* base, int64_t sb, int64_t st, int e, int c, int off)
       : at(base ? (const char*)base + (run.first.b * sb + run.first.t * st) * e : nullptr),
-        step((run.step == 1 ? st : sb) * e), row_bytes(c * e), off(off), phase((uint32_t)(uintptr_t)at & 15) {}
+        step((run.step == 1 ? st : sb) * e), row_bytes(c * e), place_bytes(window_bytes(c, e)), off(off), phase((uint32_t)(uintptr_t)at & 15) {}
   __device__ __forceinline__ void copy(char* slot) {
     if (!at) return;
     const int shift = (int)((uintptr_t)at & 15), bytes = shift + row_bytes;
-    for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+    for (int i = threadIdx.x * 16; i < place_bytes; i += blockDim.x * 16) {
+      const int some = min(max(bytes - i, 0), 16);  // the rest of the 16 is zeros
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                        (uint32_t)__cvta_generic_to_shared(slot + off + i)),
-                   "l"(at - shift + i), "r"(min(16, bytes - i))
+                   "l"(at - shift + (some ? i : 0)), "r"(some)
                    : "memory");
+    }
     at += step;
   }
   __device__ __forceinline__ void advance() { phase = (phase + (uint32_t)step) & 15; }
   // The thread's elements of the row in a slot, zeros past the end.
   template <typename U, int P>
-  __device__ __forceinline__ void read(const char* slot, int c, Vals<P>& f) const {
-    const U* p = reinterpret_cast<const U*>(slot + off + phase) + threadIdx.x;
-    const int team = blockDim.x;
+  __device__ __forceinline__ void read(const char* slot, Vals<P>& f) const {
+    const U* p = reinterpret_cast<const U*>(slot + off + phase) + first_column<P>();
 #pragma unroll
-    for (int i = 0; i < P / 2; ++i) {
-      const int col = threadIdx.x + 2 * i * team;
-      f.q[i] = pair(col < c ? to_f32(p[2 * i * team]) : 0.f, col + team < c ? to_f32(p[(2 * i + 1) * team]) : 0.f);
-    }
+    for (int i = 0; i < P / 2; ++i) f.q[i] = pair(to_f32(p[64 * i]), to_f32(p[64 * i + 32]));
   }
 };
-// Bytes that a row of at most `c` elements takes in a slot.
-constexpr int window_bytes(int c, int e) { return (c * e + 15 + 15) / 16 * 16; }
 
+template <int P>
+__device__ __forceinline__ bool whole_warp(int c) { return ((threadIdx.x & ~31) + 32) * P <= c; }
 // The thread's elements of a vector or a row in memory.
 template <typename U, int P>
 __device__ __forceinline__ void load_columns(const U* p, int c, Vals<P>& f) {
+  const int first = first_column<P>();
+  p += first;
 #pragma unroll
-  for (int i = 0; i < P / 2; ++i) {
-    const int a = threadIdx.x + 2 * i * blockDim.x, b = a + blockDim.x;
-    f.q[i] = pair(a < c ? to_f32(__ldg(p + a)) : 0.f, b < c ? to_f32(__ldg(p + b)) : 0.f);
-  }
+  for (int i = 0; i < P / 2; ++i)
+    f.q[i] = pair(first + 64 * i < c ? to_f32(__ldg(p + 64 * i)) : 0.f,
+                  first + 64 * i + 32 < c ? to_f32(__ldg(p + 64 * i + 32)) : 0.f);
 }
 template <typename U, int P>
 __device__ __forceinline__ void store_columns(U* p, int c, const Vals<P>& f) {
+  const int first = first_column<P>();
+  p += first;
+  const bool all = whole_warp<P>(c);
 #pragma unroll
   for (int i = 0; i < P / 2; ++i) {
-    const int a = threadIdx.x + 2 * i * blockDim.x, b = a + blockDim.x;
     const float2 v = halves(f.q[i]);
-    if (a < c) p[a] = from_f32<U>(v.x);
-    if (b < c) p[b] = from_f32<U>(v.y);
+    if (all || first + 64 * i < c) p[64 * i] = from_f32<U>(v.x);
+    if (all || first + 64 * i + 32 < c) p[64 * i + 32] = from_f32<U>(v.y);
   }
+}
+// Zeros in the whole ring, for the places behind the rows.
+__device__ __forceinline__ void clear_ring(uint4* ring, int bytes) {
+  for (int i = threadIdx.x; i < bytes / 16; i += blockDim.x) ring[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
 }
 template <int P>
 __device__ __forceinline__ void add_offset(Vals<P>& w, float offset) {
@@ -640,8 +652,8 @@ __device__ __forceinline__ void wait_for_next_row(int stages) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename T, typename MT, int P, bool kRes, bool kRow>
-__global__ void __launch_bounds__(512, 1)
+template <typename T, typename MT, int P, bool kRes, bool kRow, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1)
 adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slot_bytes) {
   __shared__ float2 red[2][16];
   extern __shared__ uint4 ring[];
@@ -656,13 +668,9 @@ adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slo
     shift = Window(run, op.shift, op.shift_sb, op.shift_st, me, c, rows * row_place + vec_place);
     if constexpr (kRes) gate = Window(run, op.gate, op.gate_sb, op.gate_st, me, c, rows * row_place + 2 * vec_place);
   }
-  auto elements = [&](int w) {
-    int n = 0;
-#pragma unroll
-    for (int p = 0; p < P; ++p) n += min(max(c - 32 * w - p * team, 0), 32);
-    return (float)n;
-  };
-  const int who = lane & 15;
+  auto elements = [&](int w) { return (float)min(max(c - 32 * P * w, 0), 32 * P); };
+  const int who = lane & 15, first = first_column<P>();
+  const bool whole = whole_warp<P>(c);
   const float n_who = who < warps ? elements(who) : 0.f;
   const float inv_who = n_who > 0.f ? __frcp_rn(n_who) : 0.f;
   const float inv_n = __frcp_rn(elements(lane >> 5)), inv_c = __frcp_rn((float)c);
@@ -681,6 +689,7 @@ adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slo
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  clear_ring(ring, stages * slot_bytes);
   for (int i = 0; i < stages - 1; ++i) fetch(i);
   Vals<P> w, b, g;
   w.fill(1.f);
@@ -703,11 +712,11 @@ adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slo
     const char* slot = reinterpret_cast<const char*>(ring) + stage * slot_bytes;
     const int64_t row = run.row0 + r * run.step;
     Vals<P> z;
-    x.read<T, P>(slot, c, z);
+    x.read<T, P>(slot, z);
     if constexpr (kRes) {
       Vals<P> yv;
-      y.read<T, P>(slot, c, yv);
-      if (kRow && gate.at) gate.read<MT, P>(slot, c, g);
+      y.read<T, P>(slot, yv);
+      if (kRow && gate.at) gate.read<MT, P>(slot, g);
       residual<T, P>(z, yv, g);
       store_columns<T, P>((T*)op.z + row * c, c, z);
     }
@@ -720,10 +729,12 @@ adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slo
     acc[0] = acc[1] = 0;
 #pragma unroll
     for (int i = 0; i < P / 2; ++i) {
-      const float2 d = halves(add2(z.q[i], pair(near, near)));
-      const int col = lane + 2 * i * team;
-      const uint64_t in = pair(col < c ? d.x : 0.f, col + team < c ? d.y : 0.f);
-      acc[i & 1] = fma2(in, in, acc[i & 1]);
+      uint64_t d = add2(z.q[i], pair(near, near));
+      if (!whole) {
+        const float2 f = halves(d);
+        d = pair(first + 64 * i < c ? f.x : 0.f, first + 64 * i + 32 < c ? f.y : 0.f);
+      }
+      acc[i & 1] = fma2(d, d, acc[i & 1]);
     }
     h = halves(add2(acc[0], acc[1]));
     const float m2 = warp_sum(h.x + h.y);
@@ -738,10 +749,10 @@ adaln_forward_any_kernel(const SprAdaln op, const Groups gp, int stages, int slo
     const float rstd = rsqrtf(sum16(fmaf(off * off, n_who, part.y)) * inv_c + op.eps);
     if constexpr (kRow) {
       if (scale.at) {
-        scale.read<MT, P>(slot, c, w);
+        scale.read<MT, P>(slot, w);
         add_offset<P>(w, op.scale_offset);
       }
-      if (shift.at) shift.read<MT, P>(slot, c, b);
+      if (shift.at) shift.read<MT, P>(slot, b);
     }
 #pragma unroll
     for (int i = 0; i < P / 2; ++i)
@@ -825,7 +836,7 @@ __device__ __forceinline__ void store_sums(const SprAdalnGrad& gr, const Groups&
 // Any width: a CTA takes one run of a group, its teams every other row of it, and
 // joins the teams' column sums at the end; with `own` each team takes a run by
 // itself (groups of few rows, such as a vector for every token).  75,600 x 64 bf16 17 us
-// (26%); single elements are bound by their instructions (30,000 x 1537 bf16 428 us, 10%).
+// (26% of bandwidth).
 template <typename T, typename MT, int V, int P, bool kRes>
 __global__ void __launch_bounds__(1024) adaln_backward_kernel(const SprAdaln op, const SprAdalnGrad gr,
                                                               const Groups gp, int team, int own, float* partial) {
@@ -1099,9 +1110,11 @@ adaln_backward_stream_kernel(const SprAdaln op, const SprAdalnGrad gr, const Gro
     }
 }
 
-// The backward pass of rows that 16-byte vectors do not fit, as the forward pass takes them.
-template <typename T, typename MT, int P, bool kRes, bool kRow>
-__global__ void __launch_bounds__(512, 1)
+// The backward pass of rows that 16-byte vectors do not fit, as the forward pass takes
+// them: 30,000 x 1537 bf16 84 us (50% of bandwidth), gated 171 us (49%), 30,000 x 1003 fp32
+// gated 142 us (77%).
+template <typename T, typename MT, int P, bool kRes, bool kRow, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1)
 adaln_backward_any_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups gp, int stages, int slot_bytes,
                           float* partial) {
   __shared__ uint64_t red[2][16];
@@ -1139,6 +1152,7 @@ adaln_backward_any_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  clear_ring(ring, stages * slot_bytes);
   for (int i = 0; i < stages - 1; ++i) fetch(i);
   Vals<P> w, gv;
   w.fill(1.f);
@@ -1167,10 +1181,10 @@ adaln_backward_any_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups
       next_rstd = op.rstd[row + run.step];
     }
     Vals<P> z, d, n, u;
-    x.read<T, P>(slot, c, z);
-    dh.read<T, P>(slot, c, d);
+    x.read<T, P>(slot, z);
+    dh.read<T, P>(slot, d);
     if (kRow && scale.at) {
-      scale.read<MT, P>(slot, c, w);
+      scale.read<MT, P>(slot, w);
       add_offset<P>(w, op.scale_offset);
     }
     if constexpr (kRow) st.clear();  // a row's own: written below, not added up
@@ -1192,12 +1206,12 @@ adaln_backward_any_kernel(const SprAdaln op, const SprAdalnGrad gr, const Groups
     const float2 m = halves(sums);
     Vals<P> g, dzv;
     dzv.fill(0.f);
-    if (kRes && dz.at) dz.read<T, P>(slot, c, dzv);
+    if (kRes && dz.at) dz.read<T, P>(slot, dzv);
     second<P>(n, u, pair(-m.x * inv_c, -m.x * inv_c), pair(-m.y * inv_c, -m.y * inv_c), rs, dzv, g);
     if constexpr (kRes) {
       Vals<P> yv, dy = gv;
-      y.read<T, P>(slot, c, yv);
-      if (kRow && gate.at) gate.read<MT, P>(slot, c, dy);
+      y.read<T, P>(slot, yv);
+      if (kRow && gate.at) gate.read<MT, P>(slot, dy);
       st.branch(0, g, yv, dy);
       if (kRow && gr.dgate) store_columns<MT, P>((MT*)gr.dgate + row * c, c, st.gate[0]);
       store_columns<T, P>((T*)gr.dy + row * c, c, dy);
@@ -1433,18 +1447,20 @@ int any_slot(int columns) {
   const int vecs = kRow ? (kBackward ? (kRes ? 2 : 1) : kRes ? 3 : 2) : 0;
   return rows * window_bytes(columns, sizeof(T)) + vecs * window_bytes(columns, sizeof(MT));
 }
-// Columns a thread: 8, which keeps the vectors and sums of a wide row in registers,
-// or 16 where 512 threads need them.
-constexpr int any_per(int channels) { return channels <= 512 * 8 ? 8 : 16; }
+// Columns a thread: 16, so that a row's fixed instructions serve more columns (30,000 x 1537
+// bf16 forward 66 us, with 8 96 us; gated 117 and 126; only with vectors for every row 8
+// are a little faster, 72 against 77 us at 10,000 rows), and 8 where one warp of those holds
+// the row (75,600 x 131 bf16 gated 37 us, with 16 54 us).
+constexpr int any_per(int channels) { return channels <= 256 ? 8 : 16; }
 template <typename T, typename MT, bool kRes, bool kRow, bool kBackward>
 bool any_fits(int channels) {
   const int per = any_per(channels), team = cta_for(channels, per);
   return channels >= 64 && team <= 512 && any_stages(any_slot<T, MT, kRes, kRow, kBackward>(team * per)) > 0;
 }
 
-template <typename T, typename MT, bool kRes, bool kRow, int P>
+template <typename T, typename MT, bool kRes, bool kRow, int P, int kThreads>
 int launch_forward_any(const SprAdaln* op, Groups g, cudaStream_t st) {
-  constexpr auto kern = adaln_forward_any_kernel<T, MT, P, kRes, kRow>;
+  constexpr auto kern = adaln_forward_any_kernel<T, MT, P, kRes, kRow, kThreads>;
   const int team = cta_for(op->channels, P), slot = any_slot<T, MT, kRes, kRow, false>(team * P);
   const int stages = any_stages(slot), smem = stages * slot;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kAnySmem) != cudaSuccess)
@@ -1455,17 +1471,18 @@ int launch_forward_any(const SprAdaln* op, Groups g, cudaStream_t st) {
 }
 template <typename T, typename MT, bool kRes, bool kRow>
 int launch_forward_any(const SprAdaln* op, const Groups& g, cudaStream_t st) {
-  return any_per(op->channels) == 8 ? launch_forward_any<T, MT, kRes, kRow, 8>(op, g, st)
-                                    : launch_forward_any<T, MT, kRes, kRow, 16>(op, g, st);
+  if (any_per(op->channels) == 8) return launch_forward_any<T, MT, kRes, kRow, 8, 32>(op, g, st);
+  return op->channels <= 16 * 256 ? launch_forward_any<T, MT, kRes, kRow, 16, 256>(op, g, st)
+                                  : launch_forward_any<T, MT, kRes, kRow, 16, 512>(op, g, st);
 }
 
 template <typename MT>
 int join(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, const float* partial, cudaStream_t st);
 int64_t most_runs(int channels);
 
-template <typename T, typename MT, bool kRes, bool kRow, int P>
+template <typename T, typename MT, bool kRes, bool kRow, int P, int kThreads>
 int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, float* partial, cudaStream_t st) {
-  constexpr auto kern = adaln_backward_any_kernel<T, MT, P, kRes, kRow>;
+  constexpr auto kern = adaln_backward_any_kernel<T, MT, P, kRes, kRow, kThreads>;
   const int team = cta_for(op->channels, P), slot = any_slot<T, MT, kRes, kRow, true>(team * P);
   const int stages = any_stages(slot), smem = stages * slot;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kAnySmem) != cudaSuccess)
@@ -1478,8 +1495,9 @@ int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, fl
 }
 template <typename T, typename MT, bool kRes, bool kRow>
 int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, float* partial, cudaStream_t st) {
-  return any_per(op->channels) == 8 ? launch_backward_any<T, MT, kRes, kRow, 8>(op, gr, g, partial, st)
-                                    : launch_backward_any<T, MT, kRes, kRow, 16>(op, gr, g, partial, st);
+  if (any_per(op->channels) == 8) return launch_backward_any<T, MT, kRes, kRow, 8, 32>(op, gr, g, partial, st);
+  return op->channels <= 16 * 256 ? launch_backward_any<T, MT, kRes, kRow, 16, 256>(op, gr, g, partial, st)
+                                  : launch_backward_any<T, MT, kRes, kRow, 16, 512>(op, gr, g, partial, st);
 }
 
 // Whether P/2 vectors a thread leave fewer idle places in a CTA of at most 512.
