@@ -1440,9 +1440,9 @@ int launch_forward_stream(const SprAdaln* op, Groups g, cudaStream_t st) {
 }
 
 // Slots of a row's operands that a CTA holds: 4, or 3, or 0 where they do not fit.
-int any_stages(int slot_bytes) { return 4 * slot_bytes <= kAnySmem ? 4 : 3 * slot_bytes <= kAnySmem ? 3 : 0; }
+constexpr int any_stages(int slot_bytes) { return 4 * slot_bytes <= kAnySmem ? 4 : 3 * slot_bytes <= kAnySmem ? 3 : 0; }
 template <typename T, typename MT, bool kRes, bool kRow, bool kBackward>
-int any_slot(int columns) {
+constexpr int any_slot(int columns) {
   const int rows = kBackward ? (kRes ? 4 : 2) : kRes ? 2 : 1;
   const int vecs = kRow ? (kBackward ? (kRes ? 2 : 1) : kRes ? 3 : 2) : 0;
   return rows * window_bytes(columns, sizeof(T)) + vecs * window_bytes(columns, sizeof(MT));
@@ -1452,6 +1452,9 @@ int any_slot(int columns) {
 // are a little faster, 72 against 77 us at 10,000 rows), and 8 where one warp of those holds
 // the row (75,600 x 131 bf16 gated 37 us, with 16 54 us).
 constexpr int any_per(int channels) { return channels <= 256 ? 8 : 16; }
+// Whether slots of the narrowest rows that need more than 256 threads fit.
+template <typename T, typename MT, bool kRes, bool kRow, bool kBackward>
+constexpr bool any_wide = any_stages(any_slot<T, MT, kRes, kRow, kBackward>(16 * 288)) > 0;
 // From 64 columns on a CTA of one warp a row is faster than several rows to a warp (75,600 x
 // 65 bf16: forward 26 and 33 us, backward 38 and 54 us; x 193: 27 and 79, 42 and 357 us).
 template <typename T, typename MT, bool kRes, bool kRow, bool kBackward>
@@ -1474,8 +1477,9 @@ int launch_forward_any(const SprAdaln* op, Groups g, cudaStream_t st) {
 template <typename T, typename MT, bool kRes, bool kRow>
 int launch_forward_any(const SprAdaln* op, const Groups& g, cudaStream_t st) {
   if (any_per(op->channels) == 8) return launch_forward_any<T, MT, kRes, kRow, 8, 32>(op, g, st);
-  return op->channels <= 16 * 256 ? launch_forward_any<T, MT, kRes, kRow, 16, 256>(op, g, st)
-                                  : launch_forward_any<T, MT, kRes, kRow, 16, 512>(op, g, st);
+  if constexpr (any_wide<T, MT, kRes, kRow, false>)
+    if (op->channels > 16 * 256) return launch_forward_any<T, MT, kRes, kRow, 16, 512>(op, g, st);
+  return launch_forward_any<T, MT, kRes, kRow, 16, 256>(op, g, st);
 }
 
 template <typename MT>
@@ -1498,8 +1502,9 @@ int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, Groups g, fl
 template <typename T, typename MT, bool kRes, bool kRow>
 int launch_backward_any(const SprAdaln* op, const SprAdalnGrad* gr, const Groups& g, float* partial, cudaStream_t st) {
   if (any_per(op->channels) == 8) return launch_backward_any<T, MT, kRes, kRow, 8, 32>(op, gr, g, partial, st);
-  return op->channels <= 16 * 256 ? launch_backward_any<T, MT, kRes, kRow, 16, 256>(op, gr, g, partial, st)
-                                  : launch_backward_any<T, MT, kRes, kRow, 16, 512>(op, gr, g, partial, st);
+  if constexpr (any_wide<T, MT, kRes, kRow, true>)
+    if (op->channels > 16 * 256) return launch_backward_any<T, MT, kRes, kRow, 16, 512>(op, gr, g, partial, st);
+  return launch_backward_any<T, MT, kRes, kRow, 16, 256>(op, gr, g, partial, st);
 }
 
 // Whether P/2 vectors a thread leave fewer idle places in a CTA of at most 512.
