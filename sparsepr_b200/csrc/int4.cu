@@ -27,17 +27,13 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "int4_plan.h"
 
 namespace spr {
 
-namespace {
+using namespace int4;
 
-constexpr int most_warps(int nt) { return nt == 1 ? 16 : nt == 2 ? 12 : 8; }  // of a CTA: what shared memory holds
-constexpr int kTile = 16;  // weight rows of a product
-constexpr int kBlocks = 8;  // blocks of 32 codes in one stage of a warp's ring: 128 bytes of a row
-constexpr int kStages = 4;
-constexpr int kStageBytes = kTile * kBlocks * 16;
-constexpr int kLimbs = 4;
+namespace {
 
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
   if (dtype == SPR_F32) return __ldg((const float*)p + i);
@@ -90,15 +86,7 @@ __device__ __forceinline__ uint32_t codes(uint32_t word, uint32_t zero) {
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// The operands as the kernels take them.
-struct Weights {
-  const uint8_t* packed;
-  const void* scales;
-  const uint8_t* zeros;
-  int scale_dtype;
-  int64_t n;
-  int k, groups, group_blocks, blocks;  // blocks of 32 codes a row, the unused ones of the last group too
-};
+// The rows as the kernels take them.
 struct Rows {
   const void* x;
   int64_t stride;
@@ -131,8 +119,6 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[U]) {
 // chunk's segments (GB blocks, within one group) are loaded one chunk ahead into
 // registers.  A slot holds a span; a row's pieces take an odd number of places, which
 // keeps the rows in different banks.
-constexpr int piece_bytes(int scale) { return 8 * (scale ? scale : 4) + 8; }
-
 template <int GB>
 struct Values {
   static constexpr int kSegments = kBlocks / GB, kRegs = kSegments > 1 ? kSegments / 2 : 1;
@@ -155,16 +141,6 @@ struct Values {
       reinterpret_cast<uint8_t*>(slot + kTile * 32)[at] = zero[i];
     }
   }
-};
-
-// Where a launch's warps work: `along` warps of a CTA share a tile, each with
-// `warp_chunks` neighbouring chunks of the CTA's slice of the columns; `tiles` such
-// teams to a CTA.
-struct Shape {
-  int along, tiles, warp_chunks;
-  int slice_chunks, slices;
-  int span, pieces, places;  // chunks of a span, its pieces a row, the places they take
-  int slots, slot_bytes;     // a warp's slots of scales and zeros
 };
 
 // Eight values of x from column k, zeros past the end.
@@ -968,92 +944,11 @@ int sm_count() {
   return sms[dev];
 }
 
-int parts_of(int dtype) { return dtype == SPR_BF16 ? 1 : dtype == SPR_F16 ? 2 : 3; }
-
-Weights make_weights(const uint8_t* packed, const void* scales, int scale_dtype, const uint8_t* zeros, int64_t n,
-                     int64_t k, int group) {
-  Weights w{packed, scales, zeros, scale_dtype, n, (int)k, (int)((k + group - 1) / group), group / 32, 0};
-  w.blocks = w.groups * w.group_blocks;
-  return w;
-}
-
-constexpr int kSmem = 225 * 1024;  // of a CTA at most, less what a kernel declares itself
-
-struct ForwardPlan {
-  Shape sh;
-  bool ints;
-  int scale;  // bytes of a scale that is copied ahead, 0: none is
-  int parts, pass_rows, passes, nt, gb, grid, smem;
-};
-
 // Bytes of a scale that can be copied ahead: pieces of eight, whole and aligned, and
 // groups that a chunk does not straddle; else 0.
 int scale_ahead(const Weights& w) {
   const bool whole = w.groups % 8 == 0 && (kBlocks % w.group_blocks == 0 || w.group_blocks % kBlocks == 0);
   return whole && aligned(w.scales, 16) && aligned(w.zeros, 8) ? dtype_bytes(w.scale_dtype) : 0;
-}
-
-// Rows a pass: what 32 columns of a product hold.  16-bit rows go to the integer
-// products while one pass holds them; more of them take fewer columns as bf16 parts.
-// The rest weighs, by estimates of the time: slices of the weight's columns (each CTA
-// then stages less of x, which leaves room for more warps, but the slices' sums have to
-// be joined) against warps on a tile (idle warps at the last round, and sums to join).
-ForwardPlan plan_forward(int64_t rows, const Weights& w, int dtype, int scale) {
-  ForwardPlan p{};
-  p.ints = dtype != SPR_F32 && rows <= 32 / kLimbs;
-  p.parts = p.ints ? kLimbs : parts_of(dtype);
-  p.pass_rows = (int)std::min<int64_t>(rows, 32 / p.parts);
-  p.passes = (int)((rows + p.pass_rows - 1) / p.pass_rows);
-  const int cols = p.pass_rows * p.parts;
-  p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  p.gb = w.group_blocks % 8 == 0 ? 8 : w.group_blocks % 4 == 0 ? 4 : w.group_blocks % 2 == 0 ? 2 : 1;
-  p.scale = scale;
-  Shape& sh = p.sh;
-  sh.span = w.group_blocks * ((3 + w.group_blocks) / w.group_blocks);
-  sh.pieces = sh.span / w.group_blocks;
-  sh.places = p.scale ? sh.pieces | 1 : 1;
-  sh.slot_bytes = kTile * sh.places * piece_bytes(p.scale);
-
-  const int chunks = (w.blocks + kBlocks - 1) / kBlocks;
-  const int64_t tiles = (w.n + kTile - 1) / kTile, sms = sm_count();
-  const int chunk_bytes = kBlocks * (p.ints ? cols * 32 + p.nt * 32 : cols * 64);
-  const int warp_most = kStages * kStageBytes + 4 * sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
-  const int least = std::max(1, (int)(((int64_t)chunks * chunk_bytes + kSmem - 8 * warp_most - 1) /
-                                      (kSmem - 8 * warp_most)));  // slices that leave room for eight warps
-  double best = 1e30;
-  for (int slices = least; slices <= std::min(chunks, 2 * least + 3); ++slices) {
-    const int slice_chunks = (chunks + slices - 1) / slices;
-    if ((chunks + slice_chunks - 1) / slice_chunks != slices) continue;
-    const int64_t work = tiles * p.passes * slices;
-    for (int along = 1; along <= 8 && along <= slice_chunks; along *= 2) {
-      const int warp_chunks = (slice_chunks + along - 1) / along;
-      // The span at work and those that the copies, three chunks ahead, may have reached;
-      // a tile's first and last span may be short.
-      const int slots = !p.scale || (warp_chunks % sh.span == 0 && slice_chunks % sh.span == 0) ? 2 : 4;
-      const int warp_bytes = kStages * kStageBytes + slots * sh.slot_bytes + 2 * kTile * p.nt * 8 * 4;
-      const int fit = std::min(most_warps(p.nt), (kSmem - slice_chunks * chunk_bytes) / warp_bytes);
-      const int64_t team_tiles = std::min<int64_t>(fit / along, (work + sms - 1) / sms);
-      if (team_tiles < 1) continue;
-      // Microseconds: a chunk of a warp (more where many warps share the schedulers), a
-      // round's end (with a wait for the tile's other warps), the join.
-      const int64_t rounds = (work + team_tiles * sms - 1) / (team_tiles * sms);
-      const double chunk = (p.ints ? 0.7 : 0.9) * (1 + 0.25 * (p.nt - 1)) * std::max(1.0, along * team_tiles / 12.0);
-      const double time = rounds * (warp_chunks * chunk + (along > 1 ? 0.7 : 0.3)) +
-                          (slices > 1 ? 3 + slices * (double)rows * (double)w.n * 8 / 5e6 : 0);
-      if (time >= best * 0.98) continue;
-      best = time;
-      sh.along = along;
-      sh.tiles = (int)team_tiles;
-      sh.warp_chunks = warp_chunks;
-      sh.slice_chunks = slice_chunks;
-      sh.slices = slices;
-      sh.slots = slots;
-      p.smem = along * (int)team_tiles * warp_bytes + slice_chunks * chunk_bytes;
-    }
-  }
-  const int64_t teams = (tiles + sh.tiles - 1) / sh.tiles;
-  p.grid = (int)std::min(teams, std::max<int64_t>(1, sms / (p.passes * sh.slices)));
-  return p;
 }
 
 template <int NT, int GB, bool kInt, int kScale>
@@ -1154,7 +1049,7 @@ extern "C" size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64
   const Weights w = make_weights(nullptr, nullptr, 0, nullptr, n, k, group);
   size_t most = 0;
   for (int scale : {0, 2, 4}) {  // whatever the scales' type and alignment will be
-    const ForwardPlan p = plan_forward(rows, w, dtype, scale);
+    const ForwardPlan p = plan_forward(rows, w, dtype, scale, sm_count());
     if (p.sh.slices > 1) most = std::max(most, (size_t)p.sh.slices * rows * n * sizeof(float));
   }
   return most;
@@ -1168,7 +1063,7 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
   if (rows == 0 || n == 0) return SPR_OK;
   if (!x || !packed || !scales || !y) return fail(SPR_ERR_ARG, "int4 linear: null operand");
   const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
-  const ForwardPlan p = plan_forward(rows, w, dtype, scale_ahead(w));
+  const ForwardPlan p = plan_forward(rows, w, dtype, scale_ahead(w), sm_count());
   const size_t need = p.sh.slices > 1 ? (size_t)p.sh.slices * rows * n * sizeof(float) : 0;
   if (need && (!workspace || workspace_bytes < need))
     return fail(SPR_ERR_WORKSPACE, "int4 linear: workspace %zu < %zu bytes", workspace_bytes, need);

@@ -1,0 +1,72 @@
+"""The 4-bit product where its sums are exact: rows of small integers and scales that are
+powers of two give sums that fp32 holds without a rounding, so that results are
+compared bit for bit and one wrong scale, zero code or column is an error.  On the
+CPU, the plans that spread the product over a GPU are enumerated and walked."""
+
+import os
+import subprocess
+
+import pytest
+import torch
+
+import sparsepr_b200 as spr
+from sparsepr_b200 import Int4Weight
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def test_plans_give_out_all_work_and_keep_scales_until_read(tmp_path):
+    walk = str(tmp_path / "walk")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", os.path.join(HERE, "..", "sparsepr_b200", "csrc"),
+                    os.path.join(HERE, "int4_plan_walk.cpp"), "-o", walk], check=True)
+    out = subprocess.run([walk], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.endswith(" 0 wrong\n"), out.stdout
+
+
+def _integers(dev, rows, n, k, group, dtype, sdt, zeros, seed):
+    """Rows and gradients in -1, 0, 1 (and rows of 2), scales 1/2 and 1: the sums' absolute
+    values, in units of 1/2, stay below 2^24 for the sizes here (asserted)."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    groups = -(-k // group)
+    packed = torch.randint(0, 256, (n, groups * group // 2), device=dev, generator=g).to(torch.uint8)
+    scales = (0.5 * torch.randint(1, 3, (n, groups), device=dev, generator=g)).to(sdt)
+    z = torch.randint(0, 16, (n, groups), device=dev, generator=g).to(torch.uint8) if zeros else None
+    x = torch.randint(-2, 3, (rows, k), device=dev, generator=g).to(dtype)
+    dy = torch.randint(-1, 2, (rows, n), device=dev, generator=g).to(dtype)
+    return Int4Weight(packed, scales, z), x, dy
+
+
+def _dense(w, k):
+    n, groups = w.scales.shape
+    codes = torch.stack((w.packed & 15, w.packed >> 4), -1).view(n, groups, -1).double()
+    codes -= 8.0 if w.zeros is None else w.zeros.double()[..., None]
+    return codes.mul_(w.scales.double()[..., None]).view(n, -1)[:, :k]
+
+
+def _check_exact(dev, rows, n, k, group, dtype, sdt, zeros):
+    w, x, dy = _integers(dev, rows, n, k, group, dtype, sdt, zeros, seed=n + k)
+    dense = _dense(w, k)
+    x64, d64 = x.double(), dy.double()
+    assert 2 * max((x64.abs() @ dense.abs().t()).max().item(), (d64.abs() @ dense.abs()).max().item()) < 2 ** 24
+    x.requires_grad_()
+    y = spr.int4_linear(x, *w)
+    dx, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(y, (x64 @ dense.t()).to(dtype))
+    assert torch.equal(dx, (d64 @ dense).to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,dtype,sdt,zeros", [
+    (1, 30720, 3328, BF, FP, True),    # thirteen chunks of 256 columns: a last slice of one
+    (4, 19968, 4352, BF, BF, True),
+    (3, 19968, 7424, BF, BF, False),
+    (23, 32636, 3328, BF, BF, True),
+    (2, 30720, 4352, HF, FP, True),
+    (8, 61440, 7424, BF, BF, True),
+    (1, 15360, 13824, FP, FP, True),   # fifty-four: a rest of two
+    (5, 15360, 3584, HF, HF, True),
+    (2, 15360, 3840, FP, BF, False),   # fifteen: a rest of three
+])
+def test_groups_of_32_in_several_slices(cuda, rows, n, k, dtype, sdt, zeros):
+    _check_exact(cuda, rows, n, k, 32, dtype, sdt, zeros)
