@@ -405,7 +405,7 @@ int spr_repair_apply(const void* base, const float* x_mean, const float* x_scale
  * *_st are the element strides of the batch and token axes.  The strides of
  * shift, scale and gate may be 0 (broadcast along that axis), the same axes for
  * all three.  z and h are dense.  mean and rstd [batch*tokens] fp32 (nullable)
- * are what the backward pass needs.  1 <= channels <= 16384.
+ * are what the backward pass needs.  1 <= channels <= 16384, batch*tokens < 2^31.
  */
 typedef struct SprAdaln {
   int dtype, mod_dtype;
@@ -435,7 +435,7 @@ int spr_adaln_forward(const SprAdaln* op, void* stream);
  * axes those are (1: kept, 0: summed; scale and gate may not have a stride along
  * an axis that is summed).  dshift, dscale and dgate are nullable (not formed).
  * The sums run in a fixed order.  Without rows nothing is written.  workspace:
- * spr_adaln_backward_workspace_bytes(op's sizes).
+ * spr_adaln_backward_workspace_bytes(op's sizes; 0 for sizes that the pass refuses).
  */
 typedef struct SprAdalnGrad {
   const void *dh, *dz;
@@ -458,7 +458,9 @@ int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, void* works
  * (dtype, nullable).  groups = ceil(k/group), group a multiple of 32; codes of
  * columns >= k are ignored.  x [rows][k] (row stride x_stride elements), y
  * [rows][n] dense, both `dtype`; sums in fp32, one rounding.  packed must be
- * 16-byte aligned.  workspace: spr_int4_linear_workspace_bytes (0 is possible).
+ * 16-byte aligned.  workspace: spr_int4_linear_workspace_bytes (0 is possible, and the
+ * answer for sizes that the call refuses).  At most 65,535 rows, 2^31 - 1 outputs,
+ * 2^27 columns and groups of 2^20.
  * No counterpart in the reference.
  */
 size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype);

@@ -1283,12 +1283,14 @@ int team_for(int vectors) {
   return t;
 }
 
+bool rows_fit(int64_t batch, int64_t tokens) { return tokens == 0 || batch <= 0x7fffffffLL / tokens; }
+
 int check_adaln(const SprAdaln* op) {
   if (!op) return fail(SPR_ERR_ARG, "adaln: no operands");
   if (op->batch < 0 || op->tokens < 0 || op->channels < 1 || op->channels > kMaxChannels)
     return fail(SPR_ERR_SHAPE, "adaln: batch=%lld tokens=%lld channels=%d (channels must be 1..%d)",
                 (long long)op->batch, (long long)op->tokens, op->channels, kMaxChannels);
-  if (op->tokens && op->batch > 0x7fffffffLL / op->tokens) return fail(SPR_ERR_SHAPE, "adaln: batch*tokens too large");
+  if (!rows_fit(op->batch, op->tokens)) return fail(SPR_ERR_SHAPE, "adaln: batch*tokens too large");
   if (op->dtype != SPR_F32 && op->dtype != SPR_BF16 && op->dtype != SPR_F16)
     return fail(SPR_ERR_DTYPE, "adaln: unsupported dtype %d", op->dtype);
   if (op->mod_dtype != op->dtype && op->mod_dtype != SPR_F32)
@@ -1675,7 +1677,7 @@ extern "C" int spr_adaln_forward(const SprAdaln* op, void* stream) {
 
 extern "C" size_t spr_adaln_backward_workspace_bytes(int64_t batch, int64_t tokens, int channels, int mod_batch,
                                                      int mod_tokens) {
-  if (batch <= 0 || tokens <= 0 || channels <= 0) return 0;
+  if (batch <= 0 || tokens <= 0 || channels <= 0 || channels > kMaxChannels || !rows_fit(batch, tokens)) return 0;
   Groups g = make_groups(batch, tokens, mod_batch, mod_tokens);
   cut_groups(g, most_runs(channels), 4);  // as many runs as any launch takes
   return g.chunks == 1 ? 0 : (size_t)g.count * g.chunks * 3 * channels * sizeof(float);

@@ -920,14 +920,22 @@ int4_linear_grad_kernel(const Weights w, const GradShape sh, const void* dy, int
   }
 }
 
+// Sizes that the kernels' indices hold, as check_int4 names them.
+constexpr int64_t kMostOut = 0x7fffffffLL, kMostRows = 65535, kMostIn = 1 << 27;
+constexpr int kMostGroup = 1 << 20;
+bool sizes_fit(int64_t rows, int64_t n, int64_t k, int group) {
+  return rows > 0 && rows <= kMostRows && n > 0 && n <= kMostOut && k > 0 && k <= kMostIn && group >= 32 &&
+         group % 32 == 0 && group <= kMostGroup;
+}
+
 int check_int4(const char* what, int64_t stride, int dtype, int64_t rows, int64_t n, int64_t k, int64_t row_len,
                int group, const void* packed, int scale_dtype) {
   if (rows < 0 || n < 0 || k < 1)
     return fail(SPR_ERR_SHAPE, "%s: rows=%lld n=%lld k=%lld", what, (long long)rows, (long long)n, (long long)k);
-  if (rows > 65535 || n > 0x7fffffffLL || k > (1 << 27))
+  if (rows > kMostRows || n > kMostOut || k > kMostIn)
     return fail(SPR_ERR_SHAPE, "%s: rows=%lld n=%lld k=%lld too large", what, (long long)rows, (long long)n,
                 (long long)k);
-  if (group < 32 || group % 32 || group > (1 << 20))
+  if (group < 32 || group % 32 || group > kMostGroup)
     return fail(SPR_ERR_SHAPE, "%s: group=%d must be a multiple of 32", what, group);
   if (rows > 1 && stride < row_len) return fail(SPR_ERR_SHAPE, "%s: row stride %lld", what, (long long)stride);
   for (int d : {dtype, scale_dtype})
@@ -1045,7 +1053,7 @@ int launch_grad(const GradPlan& p, const Weights& w, const void* dy, int64_t dy_
 using namespace spr;
 
 extern "C" size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype) {
-  if (rows <= 0 || n <= 0 || k <= 0 || group < 32) return 0;
+  if (!sizes_fit(rows, n, k, group)) return 0;
   const Weights w = make_weights(nullptr, nullptr, 0, nullptr, n, k, group);
   size_t most = 0;
   for (int scale : {0, 2, 4}) {  // whatever the scales' type and alignment will be
@@ -1077,7 +1085,7 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
 }
 
 extern "C" size_t spr_int4_linear_grad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype) {
-  if (rows <= 0 || n <= 0 || k <= 0 || group < 32) return 0;
+  if (!sizes_fit(rows, n, k, group)) return 0;
   size_t most = 0;
   for (int scale_dtype : {SPR_F32, SPR_BF16}) {
     const GradPlan p = plan_grad(rows, make_weights(nullptr, nullptr, scale_dtype, nullptr, n, k, group), dtype);
