@@ -404,8 +404,9 @@ int spr_repair_apply(const void* base, const float* x_mean, const float* x_scale
  * have `mod_dtype` (`dtype` or SPR_F32).  Channels are contiguous; *_sb and
  * *_st are the element strides of the batch and token axes.  The strides of
  * shift, scale and gate may be 0 (broadcast along that axis), the same axes for
- * all three.  z and h are dense.  mean and rstd [batch*tokens] fp32 (nullable)
- * are what the backward pass needs.  1 <= channels <= 16384, batch*tokens < 2^31.
+ * all three.  z and h are dense.  mean and rstd [batch*tokens] fp32 (both or
+ * neither) are what the backward pass needs.  Operands begin on their elements.
+ * 1 <= channels <= 16384, batch*tokens < 2^31.
  */
 typedef struct SprAdaln {
   int dtype, mod_dtype;
@@ -427,7 +428,7 @@ int spr_adaln_forward(const SprAdaln* op, void* stream);
 /*
  * The backward pass: op->x holds the stored z of the forward pass when
  * op->y != NULL (op->z, op->h are not read), op->mean and op->rstd its
- * statistics.  dh and dz (nullable: no gradient) with their strides; outputs
+ * statistics.  dh and dz (only with y; nullable: no gradient) with their strides; outputs
  * dx and dy dense [batch][tokens][channels] (dy only with y), and the gradients
  * of the vectors summed over the rows that share one, dense
  * [groups][channels] in mod_dtype, where groups = the product of the axes that
@@ -458,9 +459,10 @@ int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, void* works
  * (dtype, nullable).  groups = ceil(k/group), group a multiple of 32; codes of
  * columns >= k are ignored.  x [rows][k] (row stride x_stride elements), y
  * [rows][n] dense, both `dtype`; sums in fp32, one rounding.  packed must be
- * 16-byte aligned.  workspace: spr_int4_linear_workspace_bytes (0 is possible, and the
- * answer for sizes that the call refuses).  At most 65,535 rows, 2^31 - 1 outputs,
- * 2^27 columns and groups of 2^20.
+ * 16-byte aligned, the other operands begin on their elements.  workspace:
+ * spr_int4_linear_workspace_bytes (0 is possible, and the answer for sizes that the
+ * call refuses).  At most 65,535 rows, 2^31 - 1 outputs, 2^27 columns and groups of
+ * 2^20.
  * No counterpart in the reference.
  */
 size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype);

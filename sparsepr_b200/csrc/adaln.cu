@@ -1300,6 +1300,21 @@ int check_adaln(const SprAdaln* op) {
   return SPR_OK;
 }
 
+// Whether every operand begins on one of its elements, and the statistics come together.
+int check_pointers(const SprAdaln* op, const SprAdalnGrad* g) {
+  const size_t e = dtype_bytes(op->dtype), m = dtype_bytes(op->mod_dtype);
+  bool ok = aligned(op->mean, 4) && aligned(op->rstd, 4);
+  for (const void* p : {op->x, op->y, (const void*)op->z, (const void*)op->h}) ok &= aligned(p, e);
+  for (const void* p : {op->shift, op->scale, op->gate}) ok &= aligned(p, m);
+  if (g) {
+    for (const void* p : {g->dh, g->dz, (const void*)g->dx, (const void*)g->dy}) ok &= aligned(p, e);
+    for (const void* p : {g->dshift, g->dscale, g->dgate}) ok &= aligned(p, m);
+  }
+  if (!ok) return fail(SPR_ERR_ALIGN, "adaln: an operand is not aligned to its elements");
+  if (!op->mean != !op->rstd) return fail(SPR_ERR_ARG, "adaln: mean without rstd, or rstd without mean");
+  return SPR_OK;
+}
+
 // Whether 16-byte vectors fit the width, a pointer and its strides.
 bool vectors_fit(const void* p, int64_t sb, int64_t st, int dtype) {
   const int e = dtype_bytes(dtype);
@@ -1665,6 +1680,7 @@ extern "C" int spr_adaln_forward(const SprAdaln* op, void* stream) {
   if (int rc = check_adaln(op)) return rc;
   if (op->batch * op->tokens == 0) return SPR_OK;
   if (!op->x || !op->h || (op->y && !op->z)) return fail(SPR_ERR_ARG, "adaln forward: null operand");
+  if (int rc = check_pointers(op, nullptr)) return rc;
   SprAdaln o = *op;
   merge_batch(o, nullptr);
   return by_type(op, [&](auto t, auto m) {
@@ -1690,6 +1706,8 @@ extern "C" int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, 
   if (op->batch * op->tokens == 0) return SPR_OK;
   if (!op->x || !op->mean || !op->rstd || !grad->dh || !grad->dx || (op->y && !grad->dy) || (grad->dgate && !op->y))
     return fail(SPR_ERR_ARG, "adaln backward: null operand");
+  if (grad->dz && !op->y) return fail(SPR_ERR_ARG, "adaln backward: a gradient of z without a branch");
+  if (int rc = check_pointers(op, grad)) return rc;
   for (auto [p, sb, st] : {std::tuple(op->scale, op->scale_sb, op->scale_st), std::tuple(op->gate, op->gate_sb, op->gate_st)})
     if (p && ((sb && op->batch > 1 && !grad->mod_batch) || (st && op->tokens > 1 && !grad->mod_tokens)))
       return fail(SPR_ERR_ARG, "adaln backward: a vector has a stride along an axis that its gradient is summed over");

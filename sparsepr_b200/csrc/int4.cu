@@ -26,6 +26,8 @@
 // idle, and their operands would pass through shared memory again once unpacked.
 #include <math.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "int4_plan.h"
 
@@ -952,6 +954,14 @@ int sm_count() {
   return sms[dev];
 }
 
+// Whether the rows, results, scales and the workspace begin on their elements.
+int check_pointers(const char* what, int dtype, std::initializer_list<const void*> of_dtype, const void* scales,
+                   int scale_dtype, const void* workspace) {
+  bool ok = aligned(scales, dtype_bytes(scale_dtype)) && aligned(workspace, 4);
+  for (const void* p : of_dtype) ok &= aligned(p, dtype_bytes(dtype));
+  return ok ? SPR_OK : fail(SPR_ERR_ALIGN, "%s: an operand is not aligned to its elements", what);
+}
+
 // Bytes of a scale that can be copied ahead: pieces of eight, whole and aligned, and
 // groups that a chunk does not straddle; else 0.
 int scale_ahead(const Weights& w) {
@@ -1070,6 +1080,7 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
   if (int rc = check_int4("int4 linear", x_stride, dtype, rows, n, k, k, group, packed, scale_dtype)) return rc;
   if (rows == 0 || n == 0) return SPR_OK;
   if (!x || !packed || !scales || !y) return fail(SPR_ERR_ARG, "int4 linear: null operand");
+  if (int rc = check_pointers("int4 linear", dtype, {x, bias, y}, scales, scale_dtype, workspace)) return rc;
   const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
   const ForwardPlan p = plan_forward(rows, w, dtype, scale_ahead(w), sm_count());
   const size_t need = p.sh.slices > 1 ? (size_t)p.sh.slices * rows * n * sizeof(float) : 0;
@@ -1101,6 +1112,7 @@ extern "C" int spr_int4_linear_grad(const void* dy, int64_t dy_stride, int dtype
   if (int rc = check_int4("int4 linear grad", dy_stride, dtype, rows, n, k, n, group, packed, scale_dtype)) return rc;
   if (rows == 0) return SPR_OK;
   if (!dx || (n && (!dy || !packed || !scales))) return fail(SPR_ERR_ARG, "int4 linear grad: null operand");
+  if (int rc = check_pointers("int4 linear grad", dtype, {dy, dx}, scales, scale_dtype, workspace)) return rc;
   const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
   cudaStream_t st = (cudaStream_t)stream;
   int walks = 0;
