@@ -238,18 +238,18 @@ __device__ __forceinline__ void scan_x(const Weights& w, const Rows& in, int row
   __syncthreads();
 }
 
-// Integers q = round(x * 2^power[r]) of at most 2^30 in magnitude, as signed bytes d0 +
+// Integers q = round(x * 2^p) of at most 2^30 in magnitude, as signed bytes d0 +
 // 256 d1 + 65536 d2 + 2^24 d3: the bytes of q + 0x80808080 less 128 each.  sums[segment's
-// first block][column]: the bytes of a segment added up.  What is not finite counts as 0 and sets
-// bad[r].
+// first block][column]: the bytes of a segment added up.  What is not finite (bad[r]) counts
+// as 0.  back[r]: 2^-p as two factors.
 template <int U, int GB>
 __device__ __forceinline__ void stage_int(const Weights& w, const Rows& in, int row0, int rows, int b0, int nb, bool wide,
-                                          uint2* xs, int* sums, int sum_cols, const uint32_t* largest, int* power,
+                                          uint2* xs, int* sums, int sum_cols, const uint32_t* largest, float2* back,
                                           const int* bad) {
   const int cols = rows * kLimbs, words = nb * 4;
   for (int r = 0; r < rows; ++r) {
     const int p = 29 - ((int)(largest[r] >> 23) - 127), half = p / 2;  // -98 .. 156: two factors, each exact
-    if (threadIdx.x == 0) power[r] = p;
+    if (threadIdx.x == 0) back[r] = make_float2(__int_as_float((127 - half) << 23), __int_as_float((127 - p + half) << 23));
     const float f0 = __int_as_float((127 + half) << 23), f1 = __int_as_float((127 + p - half) << 23);
     const bool check = bad[r];
     for (int first = 0; first < words; first += blockDim.x) {
@@ -297,7 +297,8 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   constexpr int U = GB < 4 ? GB : 4, kUnits = GB / U;  // a unit's blocks, a segment's units
   extern __shared__ __align__(128) char smem[];
   __shared__ uint32_t largest[32];
-  __shared__ int power[32], bad[32];
+  __shared__ int bad[32];
+  __shared__ float2 back[32];  // two powers of two: from a row's integers to its values
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: the same in all lanes
   const int warps = sh.along * sh.tiles;
   const int row0 = blockIdx.y * in.pass, rows = min(in.pass, in.all - row0), cols = rows * in.parts;
@@ -409,7 +410,7 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
   }
 
   if constexpr (kInt)
-    stage_int<U, GB>(w, in, row0, rows, b0, nb, wide, reinterpret_cast<uint2*>(xs), sums, NT * 8, largest, power, bad);
+    stage_int<U, GB>(w, in, row0, rows, b0, nb, wide, reinterpret_cast<uint2*>(xs), sums, NT * 8, largest, back, bad);
   __syncthreads();
 
   uint64_t acc[NT][2] = {};  // pairs of neighbouring columns, rows r8 and r8 + 8
@@ -545,15 +546,19 @@ int4_linear_kernel(const Weights w, const Shape sh, const Rows in, float down, f
       const int row = i % kTile, r = i / kTile;
       const int64_t n = (int64_t)tile * kTile + row;
       if (n >= w.n) continue;
+      // A row's parts, or its bytes' sums: each of these is brought to its place by powers of
+      // two before they meet, since 2^30 times the result may leave fp32.
       float v = 0.f, unit = 1.f;
       for (int p = 0; p < in.parts; ++p) {
         float a = 0.f;
         for (int q = 0; q < sh.along; ++q) a += part[(q * kTile + row) * NT * 8 + r * in.parts + p];
-        v = fmaf(a, unit, v);
-        if (kInt) unit *= 256.f;
+        if constexpr (kInt) {
+          a = a * back[r].x * unit * back[r].y;
+          unit *= 256.f;
+        }
+        v += a;
       }
       if constexpr (kInt) {
-        v = scalbnf(v, -power[r]);
         if (bad[r])  // infinities and NaN of the row, one by one
           for (int k = b0 * 32; k < min(w.k, (b0 + nb) * 32); ++k) {
             const float xv = load_as_f32(in.x, in.dtype, (int64_t)(row0 + r) * in.stride + k);

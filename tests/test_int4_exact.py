@@ -52,8 +52,8 @@ def _check_exact(dev, rows, n, k, group, dtype, sdt, zeros):
     x.requires_grad_()
     y = spr.int4_linear(x, *w)
     dx, = torch.autograd.grad(y, x, dy)
-    assert torch.equal(y, (x64 @ dense.t()).to(dtype))
-    assert torch.equal(dx, (d64 @ dense).to(dtype))
+    same = torch.equal(y, (x64 @ dense.t()).to(dtype)), torch.equal(dx, (d64 @ dense).to(dtype))
+    assert same == (True, True)
 
 
 @pytest.mark.gpu
@@ -70,3 +70,19 @@ def _check_exact(dev, rows, n, k, group, dtype, sdt, zeros):
 ])
 def test_groups_of_32_in_several_slices(cuda, rows, n, k, dtype, sdt, zeros):
     _check_exact(cuda, rows, n, k, 32, dtype, sdt, zeros)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [100, -100])
+@pytest.mark.parametrize("rows,dtype", [(1, BF), (8, BF), (9, BF), (2, FP)])
+def test_large_scales_and_small_rows_and_the_other_way_round(cuda, rows, dtype, power):
+    """Scales 2^100 larger and rows (or gradients) 2^100 smaller leave the results as they are."""
+    w, x, dy = _integers(cuda, rows, 500, 640, 64, dtype, FP, True, seed=rows)
+    dense = _dense(w, 640)
+    scaled = Int4Weight(w.packed, w.scales * 2.0 ** power, w.zeros)
+    x = (x * 2.0 ** -power).requires_grad_()
+    y = spr.int4_linear(x, *scaled)
+    dx, = torch.autograd.grad(y, x, dy * 2.0 ** -power)
+    same = (torch.equal(y, ((x.detach().double() * 2.0 ** power) @ dense.t()).to(dtype)),
+            torch.equal(dx, (dy.double() @ dense).to(dtype)))
+    assert same == (True, True)
