@@ -461,8 +461,8 @@ int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, void* works
  * [rows][n] dense, both `dtype`; sums in fp32, one rounding.  packed must be
  * 16-byte aligned, the other operands begin on their elements.  workspace:
  * spr_int4_linear_workspace_bytes (0 is possible, and the answer for sizes that the
- * call refuses).  At most 65,535 rows, 2^31 - 1 outputs, 2^27 columns and groups of
- * 2^20.
+ * call refuses).  At most 2^31 - 1 rows and outputs, 2^27 columns and groups of 2^20;
+ * rows are cut into launches of 65,535, which share the workspace.
  * No counterpart in the reference.
  */
 size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype);

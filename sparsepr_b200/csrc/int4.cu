@@ -927,8 +927,9 @@ int4_linear_grad_kernel(const Weights w, const GradShape sh, const void* dy, int
   }
 }
 
-// Sizes that the kernels' indices hold, as check_int4 names them.
-constexpr int64_t kMostOut = 0x7fffffffLL, kMostRows = 65535, kMostIn = 1 << 27;
+// Sizes that the kernels' indices hold, as check_int4 names them.  A launch takes kLaunchRows
+// rows (a grid's passes), more of them are cut into launches that share the workspace.
+constexpr int64_t kMostOut = 0x7fffffffLL, kMostRows = 0x7fffffffLL, kMostIn = 1 << 27, kLaunchRows = 65535;
 constexpr int kMostGroup = 1 << 20;
 bool sizes_fit(int64_t rows, int64_t n, int64_t k, int group) {
   return rows > 0 && rows <= kMostRows && n > 0 && n <= kMostOut && k > 0 && k <= kMostIn && group >= 32 &&
@@ -1061,6 +1062,46 @@ int launch_grad(const GradPlan& p, const Weights& w, const void* dy, int64_t dy_
   return check_launch("int4 linear grad");
 }
 
+int linear_rows(const Weights& w, const void* x, int64_t x_stride, int dtype, int64_t rows, const void* bias, void* y,
+                void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  const ForwardPlan p = plan_forward(rows, w, dtype, scale_ahead(w), sm_count());
+  const size_t need = p.sh.slices > 1 ? (size_t)p.sh.slices * rows * w.n * sizeof(float) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SPR_ERR_WORKSPACE, "int4 linear: workspace %zu < %zu bytes", workspace_bytes, need);
+  float* partial = need ? (float*)workspace : nullptr;
+  return by_plan(p, [&](auto nt, auto gb, auto ints, auto scale) {
+    return launch_forward<decltype(nt)::value, decltype(gb)::value, decltype(ints)::value != 0, decltype(scale)::value>(
+        p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
+  });
+}
+
+int grad_rows(const Weights& w, int group, const void* dy, int64_t dy_stride, int dtype, int64_t rows, void* dx,
+              void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  int walks = 0;
+  if (w.n) {
+    const GradPlan p = plan_grad(rows, w, dtype);
+    const size_t need = spr_int4_linear_grad_workspace_bytes(rows, w.n, w.k, group, dtype);
+    if (!workspace || workspace_bytes < need)
+      return fail(SPR_ERR_WORKSPACE, "int4 linear grad: workspace %zu < %zu bytes", workspace_bytes, need);
+    auto by_group = [&](auto mt, auto halves, auto parts) {
+      constexpr int MT = decltype(mt)::value, H = decltype(halves)::value, PARTS = decltype(parts)::value;
+      float* out = (float*)workspace;
+      return p.g == 4   ? launch_grad<MT, H, 4, PARTS>(p, w, dy, dy_stride, dtype, out, st)
+             : p.g == 2 ? launch_grad<MT, H, 2, PARTS>(p, w, dy, dy_stride, dtype, out, st)
+                        : launch_grad<MT, H, 1, PARTS>(p, w, dy, dy_stride, dtype, out, st);
+    };
+    auto by_rows = [&](auto parts) {
+      return p.halves == 1 ? by_group(Int<1>{}, Int<1>{}, parts)
+             : p.mt == 1   ? by_group(Int<1>{}, Int<2>{}, parts)
+                           : by_group(Int<2>{}, Int<2>{}, parts);
+    };
+    if (int rc = p.parts == 2 ? by_rows(Int<2>{}) : by_rows(Int<3>{})) return rc;
+    walks = p.walks;
+  }
+  join_slices((const float*)workspace, walks, rows * w.k, w.k, nullptr, dx, dtype, st);
+  return check_launch("int4 linear grad");
+}
+
 }  // namespace
 
 }  // namespace spr
@@ -1069,6 +1110,7 @@ using namespace spr;
 
 extern "C" size_t spr_int4_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype) {
   if (!sizes_fit(rows, n, k, group)) return 0;
+  rows = std::min(rows, kLaunchRows);
   const Weights w = make_weights(nullptr, nullptr, 0, nullptr, n, k, group);
   size_t most = 0;
   for (int scale : {0, 2, 4}) {  // whatever the scales' type and alignment will be
@@ -1087,21 +1129,17 @@ extern "C" int spr_int4_linear(const void* x, int64_t x_stride, int dtype, int64
   if (!x || !packed || !scales || !y) return fail(SPR_ERR_ARG, "int4 linear: null operand");
   if (int rc = check_pointers("int4 linear", dtype, {x, bias, y}, scales, scale_dtype, workspace)) return rc;
   const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
-  const ForwardPlan p = plan_forward(rows, w, dtype, scale_ahead(w), sm_count());
-  const size_t need = p.sh.slices > 1 ? (size_t)p.sh.slices * rows * n * sizeof(float) : 0;
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(SPR_ERR_WORKSPACE, "int4 linear: workspace %zu < %zu bytes", workspace_bytes, need);
-  float* partial = need ? (float*)workspace : nullptr;
-  cudaStream_t st = (cudaStream_t)stream;
-  return by_plan(p, [&](auto nt, auto gb, auto ints, auto scale) {
-    return launch_forward<decltype(nt)::value, decltype(gb)::value, decltype(ints)::value != 0,
-                          decltype(scale)::value>(
-        p, w, x, x_stride, dtype, (int)rows, bias, y, partial, st);
-  });
+  const int e = dtype_bytes(dtype);
+  for (int64_t r = 0; r < rows; r += kLaunchRows)
+    if (int rc = linear_rows(w, (const char*)x + r * x_stride * e, x_stride, dtype, std::min(rows - r, kLaunchRows), bias,
+                             (char*)y + r * n * e, workspace, workspace_bytes, (cudaStream_t)stream))
+      return rc;
+  return SPR_OK;
 }
 
 extern "C" size_t spr_int4_linear_grad_workspace_bytes(int64_t rows, int64_t n, int64_t k, int group, int dtype) {
   if (!sizes_fit(rows, n, k, group)) return 0;
+  rows = std::min(rows, kLaunchRows);
   size_t most = 0;
   for (int scale_dtype : {SPR_F32, SPR_BF16}) {
     const GradPlan p = plan_grad(rows, make_weights(nullptr, nullptr, scale_dtype, nullptr, n, k, group), dtype);
@@ -1119,29 +1157,10 @@ extern "C" int spr_int4_linear_grad(const void* dy, int64_t dy_stride, int dtype
   if (!dx || (n && (!dy || !packed || !scales))) return fail(SPR_ERR_ARG, "int4 linear grad: null operand");
   if (int rc = check_pointers("int4 linear grad", dtype, {dy, dx}, scales, scale_dtype, workspace)) return rc;
   const Weights w = make_weights(packed, scales, scale_dtype, zeros, n, k, group);
-  cudaStream_t st = (cudaStream_t)stream;
-  int walks = 0;
-  if (n) {
-    const GradPlan p = plan_grad(rows, w, dtype);
-    const size_t need = spr_int4_linear_grad_workspace_bytes(rows, n, k, group, dtype);
-    if (!workspace || workspace_bytes < need)
-      return fail(SPR_ERR_WORKSPACE, "int4 linear grad: workspace %zu < %zu bytes", workspace_bytes, need);
-    auto by_group = [&](auto mt, auto halves, auto parts) {
-      constexpr int MT = decltype(mt)::value, H = decltype(halves)::value, PARTS = decltype(parts)::value;
-      float* out = (float*)workspace;
-      return p.g == 4   ? launch_grad<MT, H, 4, PARTS>(p, w, dy, dy_stride, dtype, out, st)
-             : p.g == 2 ? launch_grad<MT, H, 2, PARTS>(p, w, dy, dy_stride, dtype, out, st)
-                        : launch_grad<MT, H, 1, PARTS>(p, w, dy, dy_stride, dtype, out, st);
-    };
-    auto by_rows = [&](auto parts) {
-      return p.halves == 1 ? by_group(Int<1>{}, Int<1>{}, parts)
-             : p.mt == 1   ? by_group(Int<1>{}, Int<2>{}, parts)
-                           : by_group(Int<2>{}, Int<2>{}, parts);
-    };
-    if (int rc = p.parts == 2 ? by_rows(Int<2>{}) : by_rows(Int<3>{})) return rc;
-    walks = p.walks;
-  }
-  const int64_t size = rows * k;
-  join_slices((const float*)workspace, walks, size, k, nullptr, dx, dtype, st);
-  return check_launch("int4 linear grad");
+  const int e = dtype_bytes(dtype);
+  for (int64_t r = 0; r < rows; r += kLaunchRows)
+    if (int rc = grad_rows(w, group, (const char*)dy + r * dy_stride * e, dy_stride, dtype, std::min(rows - r, kLaunchRows),
+                           (char*)dx + r * k * e, workspace, workspace_bytes, (cudaStream_t)stream))
+      return rc;
+  return SPR_OK;
 }

@@ -100,7 +100,7 @@ def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zer
 
     ``x`` [..., K] in fp32, bf16 or fp16 and ``bias`` [N] in x's type; the result [..., N]
     is rounded once from fp32 sums.  Any number of rows is computed, but the
-    weights are read once for each block of rows: the call is for a few rows.  A backward
+    weights are read again for every 8 to 32 rows: the call is for a few rows.  A backward
     pass captured into a CUDA graph needs what any captured autograd call needs: no graph
     of an uncaptured forward pass over the same leaves still alive."""
     if x.dim() < 1 or x.shape[-1] < 1:

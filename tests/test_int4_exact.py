@@ -86,3 +86,9 @@ def test_large_scales_and_small_rows_and_the_other_way_round(cuda, rows, dtype, 
     same = (torch.equal(y, ((x.detach().double() * 2.0 ** power) @ dense.t()).to(dtype)),
             torch.equal(dx, (dy.double() @ dense).to(dtype)))
     assert same == (True, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k,group,dtype", [(72, 64, BF), (64, 32, FP)])
+def test_more_rows_than_a_launch_takes(cuda, k, group, dtype):
+    _check_exact(cuda, 65535 + 65535 + 41, 40, k, group, dtype, FP, True)
