@@ -128,7 +128,8 @@ _SAVED = ("x", "y", "gate", "scale")
 
 
 def _backward(ctx, *grads):
-    x, y, gate, scale, stats = ctx.saved_tensors
+    # Saved-tensor hooks may give back another layout, but not other values' places or types.
+    x, y, gate, scale, stats = saved = [K.as_saved(t, meta) for t, meta in zip(ctx.saved_tensors, ctx.saved_meta)]
     dz, dh = grads if y is not None else (None, grads[0])
     if dh is None:
         if dz is None:
@@ -145,8 +146,8 @@ def _backward(ctx, *grads):
         s.y, s.x_sb, s.x_st = y.data_ptr(), s.tokens * s.channels, s.channels
     s.gate = None if gate is None else gate.data_ptr()
     s.scale = None if scale is None else scale.data_ptr()
-    for name, t, strides in zip(_SAVED, (x, y, gate, scale), ctx.strides):
-        if t is not None and t.stride() != strides:  # a saved-tensor hook gave back another layout
+    for name, t, meta in zip(_SAVED, saved, ctx.saved_meta):
+        if t is not None and t.stride() != meta[1]:
             b, n = (s.batch, s.tokens) if name in ("x", "y") else mod_shape
             sb, st = _strides(t, b, n, name)
             setattr(s, name + "_sb", sb)
@@ -166,9 +167,9 @@ class _AdaLN(torch.autograd.Function):
     def forward(ctx, x, y, gate, shift, scale, eps, scale_offset):
         op, mod_shape = operands(x, y, gate, shift, scale, scale_offset)
         z, h, stats, struct = K.adaln_forward_struct(op, eps, True)
-        saved = x if z is None else z, y, gate, scale
-        ctx.save_for_backward(*saved, stats)
-        ctx.strides = [None if t is None else t.stride() for t in saved]
+        saved = x if z is None else z, y, gate, scale, stats
+        ctx.save_for_backward(*saved)
+        ctx.saved_meta = [K.saved_meta(t) for t in saved]
         ctx.set_materialize_grads(False)
         vector = gate if gate is not None else shift if shift is not None else scale
         ctx.operands = struct, mod_shape, None if vector is None else vector.shape, op.mod_dtype

@@ -66,7 +66,7 @@ def dequantize_int4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Ten
 
 
 def _backward(ctx, dy):
-    packed, scales, zeros = ctx.saved_tensors
+    packed, scales, zeros = (K.as_saved(t, meta) for t, meta in zip(ctx.saved_tensors, ctx.saved_meta))
     dx = dbias = None
     if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
         dy = dy.contiguous()
@@ -85,6 +85,7 @@ class _Int4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, packed, scales, zeros, bias):
         ctx.save_for_backward(packed, scales, zeros)
+        ctx.saved_meta = [K.saved_meta(t) for t in (packed, scales, zeros)]
         ctx.in_features = x.shape[1]
         return K.int4_linear(x, packed, scales, zeros, bias)
 

@@ -573,6 +573,23 @@ def _launch(index: int, name: str, *args) -> None:
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def saved_meta(t):
+    """What :func:`as_saved` compares a saved operand with."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def as_saved(t, meta):
+    """A saved operand as a backward pass may read it.  Saved-tensor hooks give back what they
+    like: a layout other than the saved one becomes dense, another shape, type or device is refused."""
+    if t is None:
+        return None
+    shape, strides, dtype, index = meta
+    if t.dtype != dtype or t.shape != shape or t.get_device() != index:
+        raise RuntimeError(f"a saved operand came back as {tuple(t.shape)} {t.dtype} on {t.device}; it was "
+                           f"{tuple(shape)} {dtype} on cuda:{index}")
+    return t if t.stride() == strides else t.contiguous()
+
+
 class AdalnOperands(NamedTuple):
     """Operands of the adaLN passes as the kernels read them: tensors, the rows as [batch][tokens][channels]
     with (batch, token) element strides, and the vectors' strides (0: broadcast along that axis)."""
