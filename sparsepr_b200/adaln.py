@@ -15,9 +15,10 @@ adjacent: one vector, one per sample ([B, 1, C]), one per token ([B, N, C] or
 normalised, so the norm reads what the residual stream holds.  Statistics and
 sums are fp32, and the gradients of shared vectors are summed in a fixed order.
 
-The gradients are of first order.  A backward pass captured into a CUDA graph needs
-what any captured autograd call needs: warm-up passes on a side stream, and no graph
-of an uncaptured forward pass over the same leaves still alive.  :func:`operands` with
+The gradients are of first order, in reverse mode (dual tensors are refused).  A backward
+pass captured into a CUDA graph needs what any captured autograd call needs: warm-up
+passes on a side stream, and no graph of an uncaptured forward pass over the same leaves
+still alive.  :func:`operands` with
 :func:`sparsepr_b200.kernels.adaln_forward` and ``adaln_backward`` are the same passes
 without autograd.
 """
@@ -130,6 +131,7 @@ _SAVED = ("x", "y", "gate", "scale")
 def _backward(ctx, *grads):
     # Saved-tensor hooks may give back another layout, but not other values' places or types.
     x, y, gate, scale, stats = saved = [K.as_saved(t, meta) for t, meta in zip(ctx.saved_tensors, ctx.saved_meta)]
+    K.refuse_tangents("layer norm gradient", x, y, gate, scale, *grads)
     dz, dh = grads if y is not None else (None, grads[0])
     if dh is None:
         if dz is None:
@@ -182,6 +184,7 @@ class _AdaLN(torch.autograd.Function):
 
 
 def _wants_grad(x, y, gate, shift, scale):
+    K.refuse_tangents("layer norm", x, y, gate, shift, scale)
     return torch.is_grad_enabled() and (x.requires_grad or (y is not None and y.requires_grad)
                                         or (gate is not None and gate.requires_grad)
                                         or (shift is not None and shift.requires_grad)

@@ -67,6 +67,7 @@ def dequantize_int4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Ten
 
 def _backward(ctx, dy):
     packed, scales, zeros = (K.as_saved(t, meta) for t, meta in zip(ctx.saved_tensors, ctx.saved_meta))
+    K.refuse_tangents("int4_linear gradient", dy)
     dx = dbias = None
     if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
         dy = dy.contiguous()
@@ -101,11 +102,13 @@ def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zer
 
     ``x`` [..., K] in fp32, bf16 or fp16 and ``bias`` [N] in x's type; the result [..., N]
     is rounded once from fp32 sums.  Any number of rows is computed, but the
-    weights are read again for every 8 to 32 rows: the call is for a few rows.  A backward
-    pass captured into a CUDA graph needs what any captured autograd call needs: no graph
-    of an uncaptured forward pass over the same leaves still alive."""
+    weights are read again for every 8 to 32 rows: the call is for a few rows.  Gradients
+    are of first order, in reverse mode (dual tensors are refused).  A backward pass captured
+    into a CUDA graph needs what any captured autograd call needs: no graph of an uncaptured
+    forward pass over the same leaves still alive."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"int4_linear: x must be [..., K], got {tuple(x.shape)}")
+    K.refuse_tangents("int4_linear", x, scales, bias)
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()

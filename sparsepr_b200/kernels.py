@@ -12,6 +12,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -571,6 +572,14 @@ def _launch(index: int, name: str, *args) -> None:
     else:
         with torch.cuda.device(index):
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raise where a forward-mode derivative would be lost: the kernels read a dual tensor's values alone."""
+    if forward_ad._current_level >= 0:  # within a dual level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}: forward-mode derivatives are not supported")
 
 
 def saved_meta(t):
