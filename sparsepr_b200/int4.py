@@ -105,10 +105,13 @@ def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zer
     weights are read again for every 8 to 32 rows: the call is for a few rows.  Gradients
     are of first order, in reverse mode (dual tensors are refused).  A backward pass captured
     into a CUDA graph needs what any captured autograd call needs: no graph of an uncaptured
-    forward pass over the same leaves still alive."""
+    forward pass over the same leaves still alive.  The weight is frozen: scales that ask for
+    a gradient are refused."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f"int4_linear: x must be [..., K], got {tuple(x.shape)}")
     K.refuse_tangents("int4_linear", x, scales, bias)
+    if scales.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("int4_linear: the weight is frozen, its scales take no gradient; pass scales.detach()")
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()

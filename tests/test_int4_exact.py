@@ -92,3 +92,15 @@ def test_large_scales_and_small_rows_and_the_other_way_round(cuda, rows, dtype, 
 @pytest.mark.parametrize("k,group,dtype", [(72, 64, BF), (64, 32, FP)])
 def test_more_rows_than_a_launch_takes(cuda, k, group, dtype):
     _check_exact(cuda, 65535 + 65535 + 41, 40, k, group, dtype, FP, True)
+
+
+def test_scales_that_ask_for_a_gradient_are_refused():
+    w = spr.quantize_int4(torch.randn(8, 64), 32)
+    scales = w.scales.requires_grad_()
+    for x in (torch.zeros(1, 64), torch.zeros(1, 64, requires_grad=True)):
+        with pytest.raises(RuntimeError, match="frozen"):
+            spr.int4_linear(x, w.packed, scales, w.zeros)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="need CUDA tensors"):
+            spr.int4_linear(x, w.packed, scales, w.zeros)
+    with pytest.raises(RuntimeError, match="need CUDA tensors"):
+        spr.int4_linear(x, w.packed, scales.detach(), w.zeros)
