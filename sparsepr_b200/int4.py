@@ -48,7 +48,9 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 64, symmetric: bool = 
     w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group_size - k)).view(n, groups, group_size)
     lo, hi = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
     step = torch.maximum(-lo, hi) / 7.0 if symmetric else (hi - lo) / 15.0
-    scales = step.clamp(min=torch.finfo(sdt).tiny).to(sdt)  # normal numbers, groups of zeros among them
+    if sdt == torch.float16:  # below 2^-14, multiples of 2^-24: rounded up, so that all codes fit
+        step = torch.where(step < 2.0 ** -14, (step * 2.0 ** 24).ceil().clamp(min=1.0) * 2.0 ** -24, step)
+    scales = step.clamp(min=torch.finfo(torch.float32).tiny).to(sdt)  # positive, of groups of zeros too
     s = scales.float()
     zeros = None if symmetric else (-lo / s).round().clamp(0, 15).to(torch.uint8)
     codes = ((w / s[..., None]).round() + (8.0 if symmetric else zeros.float()[..., None])).clamp(0, 15)

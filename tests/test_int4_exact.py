@@ -104,3 +104,22 @@ def test_scales_that_ask_for_a_gradient_are_refused():
             spr.int4_linear(x, w.packed, scales, w.zeros)
     with pytest.raises(RuntimeError, match="need CUDA tensors"):
         spr.int4_linear(x, w.packed, scales.detach(), w.zeros)
+
+
+@pytest.mark.parametrize("std", [1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("dtype", [HF, FP])
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_small_weights_keep_their_codes_under_fp16_scales(std, dtype, symmetric):
+    """Steps below fp16's normal numbers are rounded up to the next multiple of 2^-24: codes are off by half a
+    step, or a whole one where a zero code was rounded too."""
+    w = (torch.randn(16, 256, generator=torch.Generator().manual_seed(4)) * std).to(dtype)
+    q = spr.quantize_int4(w, 64, symmetric=symmetric, scale_dtype=HF)
+    groups = w.double().view(16, 4, 64)
+    if symmetric:
+        step = groups.abs().amax(-1) / 7
+    else:
+        step = (groups.amax(-1).clamp(min=0) - groups.amin(-1).clamp(max=0)) / 15
+    assert (step < 2.0 ** -14).all()
+    assert (q.scales.double() >= step * (1 - 2.0 ** -22)).all() and (q.scales.double() <= step + 2.0 ** -24).all()
+    err = (spr.dequantize_int4(*q, 256).double() - w.double()).abs().view(16, 4, 64)
+    assert (err <= (0.5 if symmetric else 1.0) * (1 + 2.0 ** -20) * q.scales.double()[..., None]).all()
