@@ -34,7 +34,8 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 64, symmetric: bool = 
 
     Each run of ``group_size`` columns (a multiple of 32; the last may be partly
     used) has a scale in ``scale_dtype`` (default: the weight's type) and, unless
-    ``symmetric``, a zero code; the codes are those nearest under the stored scale."""
+    ``symmetric``, a zero code; the codes are those nearest under the stored scale.  A
+    weight that is not finite, or too large for its scales' type, raises."""
     if weight.dim() != 2 or weight.dtype not in K._DT or weight.numel() == 0:
         raise RuntimeError(f"quantize_int4 expects a non-empty fp32/bf16/fp16 [N, K] weight, got "
                            f"{tuple(weight.shape)} {weight.dtype}")
@@ -52,6 +53,8 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 64, symmetric: bool = 
         step = torch.where(step < 2.0 ** -14, (step * 2.0 ** 24).ceil().clamp(min=1.0) * 2.0 ** -24, step)
     scales = step.clamp(min=torch.finfo(torch.float32).tiny).to(sdt)  # positive, of groups of zeros too
     s = scales.float()
+    if not torch.isfinite(s).all():
+        raise RuntimeError(f"quantize_int4: the weight is not finite, or too large for scales in {sdt}")
     zeros = None if symmetric else (-lo / s).round().clamp(0, 15).to(torch.uint8)
     codes = ((w / s[..., None]).round() + (8.0 if symmetric else zeros.float()[..., None])).clamp(0, 15)
     codes = codes.to(torch.uint8).view(n, groups * group_size)

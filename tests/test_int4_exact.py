@@ -123,3 +123,14 @@ def test_small_weights_keep_their_codes_under_fp16_scales(std, dtype, symmetric)
     assert (q.scales.double() >= step * (1 - 2.0 ** -22)).all() and (q.scales.double() <= step + 2.0 ** -24).all()
     err = (spr.dequantize_int4(*q, 256).double() - w.double()).abs().view(16, 4, 64)
     assert (err <= (0.5 if symmetric else 1.0) * (1 + 2.0 ** -20) * q.scales.double()[..., None]).all()
+
+
+def test_weights_without_a_scale_are_refused():
+    for bad in (float("inf"), float("nan")):
+        w = torch.ones(2, 64)
+        w[1, 5] = bad
+        with pytest.raises(RuntimeError, match="not finite"):
+            spr.quantize_int4(w, 32)
+    with pytest.raises(RuntimeError, match="too large"):
+        spr.quantize_int4(torch.full((2, 64), 1e6), 32, scale_dtype=HF)
+    spr.quantize_int4(torch.full((2, 64), 1e6), 32, scale_dtype=BF)
