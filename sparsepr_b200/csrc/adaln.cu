@@ -1408,18 +1408,21 @@ int forward_per_thread(bool vec, int nvec) {
   return nvec <= 4096 ? 4 : 16;
 }
 
-// CTAs of a kernel that an SM holds, asked once for each number of warps (a kernel's
-// shared memory follows from them).
+// CTAs of a kernel that an SM of the current device holds, asked once for each device and
+// number of warps (a kernel's shared memory follows from them); an answer that failed is
+// not kept.
 template <auto kern>
 int resident(int threads, int smem) {
-  static std::atomic<int> known[33] = {};
-  std::atomic<int>& n = known[threads / 32];
-  if (n.load(std::memory_order_relaxed) == 0) {
-    int got = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kern, threads, smem) != cudaSuccess) got = 1;
-    n.store(std::max(1, got), std::memory_order_relaxed);
-  }
-  return n.load(std::memory_order_relaxed);
+  constexpr int kDevices = 16;
+  static std::atomic<int> known[kDevices][17] = {};
+  int dev = -1, got = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  std::atomic<int>* kept = dev < kDevices && threads <= 512 ? &known[dev][threads / 32] : nullptr;
+  if (kept && (got = kept->load(std::memory_order_relaxed)) != 0) return got;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kern, threads, smem) != cudaSuccess) return 1;
+  got = std::max(1, got);
+  if (kept) kept->store(got, std::memory_order_relaxed);
+  return got;
 }
 
 // How a streaming launch cuts its groups: as many runs as fit on the GPU at once, and

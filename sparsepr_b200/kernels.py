@@ -574,6 +574,19 @@ def _launch(index: int, name: str, *args) -> None:
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _launch_with_workspace(like: torch.Tensor, query: str, sizes, name: str, *args) -> None:
+    """``name`` with a workspace of its own behind ``args``, sized by ``query`` under the device that the launch is
+    planned for: that of ``like``, also where another one is current."""
+    index = like.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _launch_with_workspace(like, query, sizes, name, *args)
+    nbytes = _lib.query(query, *sizes)
+    ws = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _count(2 if nbytes else 1)
+    _lib.call(name, *args, _p(ws), nbytes, torch._C._cuda_getCurrentRawStream(index))
+
+
 def refuse_tangents(what: str, *tensors) -> None:
     """Raise where a forward-mode derivative would be lost: the kernels read a dual tensor's values alone."""
     if forward_ad._current_level >= 0:  # within a dual level
@@ -670,10 +683,8 @@ def adaln_backward_struct(s: _lib.SprAdaln, branch: bool, dh, dz, needs, mod_sha
     keep_b, keep_n = int(mod_shape[0] > 1), int(mod_shape[1] > 1)
     gr = _lib.SprAdalnGrad(dh.data_ptr(), _p(dz), n * c, c, n * c, c, dx.data_ptr(), _p(dy), _p(dshift), _p(dscale),
                            _p(dgate), keep_b, keep_n)
-    nbytes = _lib.query("spr_adaln_backward_workspace_bytes", b, n, c, keep_b, keep_n)
-    ws = new(nbytes, dtype=torch.uint8) if nbytes else None
-    _count(2 if nbytes else 1)
-    _launch(dh.get_device(), "spr_adaln_backward", ctypes.addressof(s), ctypes.addressof(gr), _p(ws), nbytes)
+    _launch_with_workspace(dh, "spr_adaln_backward_workspace_bytes", (b, n, c, keep_b, keep_n), "spr_adaln_backward",
+                           ctypes.addressof(s), ctypes.addressof(gr))
     return dx, dy, dgate, dshift, dscale
 
 
@@ -733,11 +744,10 @@ def int4_linear(x, packed, scales, zeros=None, bias=None) -> torch.Tensor:
         raise RuntimeError(f"int4_linear: bias must be contiguous {x.dtype} [{n}] on {x.device}, got {bias.dtype} "
                            f"{tuple(bias.shape)} on {bias.device}")
     y = x.new_empty((r, n))
-    nbytes = _lib.query("spr_int4_linear_workspace_bytes", r, n, k, group, _DT[x.dtype])
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _count(2 if nbytes else 1)
-    _launch(x.get_device(), "spr_int4_linear", _p(x), x.stride(0), _DT[x.dtype], r, n, k, group, _p(packed), _p(scales),
-            _DT[scales.dtype], _p(zeros), _p(bias), _p(y), _p(ws), nbytes)
+    dt = _DT[x.dtype]
+    _launch_with_workspace(x, "spr_int4_linear_workspace_bytes", (r, n, k, group, dt), "spr_int4_linear", _p(x),
+                           x.stride(0), dt, r, n, k, group, _p(packed), _p(scales), _DT[scales.dtype], _p(zeros),
+                           _p(bias), _p(y))
     return y
 
 
@@ -755,9 +765,7 @@ def int4_linear_grad_checked(dy, packed, scales, zeros, in_features: int, n: int
     r = dy.shape[0]
     dx = dy.new_empty((r, in_features))
     dt = _DT[dy.dtype]
-    nbytes = _lib.query("spr_int4_linear_grad_workspace_bytes", r, n, in_features, group, dt)
-    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _count(2)
-    _launch(dy.get_device(), "spr_int4_linear_grad", dy.data_ptr(), dy.stride(0), dt, r, n, in_features, group,
-            packed.data_ptr(), scales.data_ptr(), _DT[scales.dtype], _p(zeros), dx.data_ptr(), _p(ws), nbytes)
+    _launch_with_workspace(dy, "spr_int4_linear_grad_workspace_bytes", (r, n, in_features, group, dt),
+                           "spr_int4_linear_grad", dy.data_ptr(), dy.stride(0), dt, r, n, in_features, group,
+                           packed.data_ptr(), scales.data_ptr(), _DT[scales.dtype], _p(zeros), dx.data_ptr())
     return dx

@@ -84,3 +84,33 @@ def test_int4_operands(kw):
     if "bias" not in kw:
         _refused("SPR_ERR_ALIGN", "spr_int4_linear_grad", a["x"], 8, 1, 1, 8, 64, 32, 256, a["scales"], 0, None, a["y"],
                  a["workspace"] or 256, 1 << 30, None)
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_workspace_is_sized_under_the_device_of_the_launch(monkeypatch, current):
+    """Tensors on device 1: the size, the allocation and the launch all see device 1 as the current one."""
+    import contextlib
+    import types
+
+    import torch
+
+    from sparsepr_b200 import kernels as K
+
+    state, seen = {"device": current}, []
+
+    @contextlib.contextmanager
+    def device(index):
+        before, state["device"] = state["device"], index
+        yield
+        state["device"] = before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["device"])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7 + index, raising=False)
+    monkeypatch.setattr(K._lib, "query", lambda name, *a: seen.append((name, a, state["device"])) or 64)
+    monkeypatch.setattr(K._lib, "call", lambda name, *a: seen.append((name, a, state["device"])))
+    buffer = torch.empty(64, dtype=torch.uint8)
+    like = types.SimpleNamespace(get_device=lambda: 1, new_empty=lambda n, dtype: buffer)
+    K._launch_with_workspace(like, "query", (1, 2), "entry", 3, 4)
+    assert seen == [("query", (1, 2), 1), ("entry", (3, 4, buffer.data_ptr(), 64, 8), 1)]
+    assert state["device"] == current
