@@ -175,7 +175,7 @@ class HunyuanDiT:
         return x.reshape((t // pt) * (h // ph) * (w // pw), c * pt * ph * pw), (t // pt, h // ph, w // pw)
 
     def _modulation_layers(self):
-        """Every modulation layer's (rows, owner, key) in the order of the blocks: a double
+        """Every modulation layer's (owner, key) in the order of the blocks: a double
         block's video and text ones, the single blocks', the output layer's."""
         for blk in self.double:
             for s in ("img", "txt"):
@@ -256,6 +256,8 @@ class HunyuanDiT:
                 qkv[s] = (q, k, v)
             o_img, o_txt = attention(i, *qkv["img"], *qkv["txt"])
             for s, o in (("img", o_img), ("txt", o_txt)):
+                if s == "txt" and i + 1 == len(self.double) and not self.single:
+                    continue  # the output layer takes the video tokens alone
                 _, _, g1, sh2, sc2, g2 = double[i][s]
                 branch = self._lin(o.reshape(x[s].shape[0], cfg.hidden), blk[s]["proj"])
                 x[s], m = self._residual_norm(x[s], branch, g1, sh2, sc2)
