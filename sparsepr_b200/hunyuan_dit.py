@@ -236,20 +236,20 @@ class HunyuanDiT:
         ns = n // world
         pos = torch.arange(rank * ns, (rank + 1) * ns, device=self.device)
         cos, sin = rope_3d(grid, pos, cfg.rope_axes, cfg.rope_theta, self.device)
-        img = self._lin(tokens[rank * ns:(rank + 1) * ns], self.patch_in)
-        txt = self._lin(text.to(self.dtype), self.txt_in)
+        # The streams and their norms are held by these alone, so that each goes when it is replaced or used.
+        x = {"img": self._lin(tokens[rank * ns:(rank + 1) * ns], self.patch_in),
+             "txt": self._lin(text.to(self.dtype), self.txt_in)}
         vec = (self._mlp2(_timestep_embedding(t.view(1)).to(self.dtype), self.time_in)
                + self._mlp2(_timestep_embedding(guidance.view(1)).to(self.dtype), self.guid_in)
                + self._mlp2(pooled.to(self.dtype).view(1, -1), self.vec_in)).view(-1)
         svec = F.silu(vec)
         double, single, final = self._modulations(svec)
         after = [*double, {"img": single[0], "txt": single[0]} if single else {"img": final, "txt": final}]
-        x = {"img": img, "txt": txt}
         h = {s: self._norm(x[s], *after[0][s][:2]) for s in x}
         for i, blk in enumerate(self.double):
             qkv = {}
             for s in x:
-                q, k, v = self._lin(h[s], blk[s]["qkv"]).view(x[s].shape[0], 3, cfg.heads, cfg.head_dim).unbind(1)
+                q, k, v = self._lin(h.pop(s), blk[s]["qkv"]).view(x[s].shape[0], 3, cfg.heads, cfg.head_dim).unbind(1)
                 q, k = _rms(q, blk[s]["qn"]), _rms(k, blk[s]["kn"])
                 if s == "img":
                     q, k = _apply_rope(q, cos, sin), _apply_rope(k, cos, sin)
