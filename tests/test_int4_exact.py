@@ -134,3 +134,25 @@ def test_weights_without_a_scale_are_refused():
     with pytest.raises(RuntimeError, match="too large"):
         spr.quantize_int4(torch.full((2, 64), 1e6), 32, scale_dtype=HF)
     spr.quantize_int4(torch.full((2, 64), 1e6), 32, scale_dtype=BF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,k,group,dtype,sdt,zeros", [
+    (1, 5120, 256, 32, BF, BF, False),
+    (2, 17, 130, 64, BF, FP, True),
+    (3, 7777, 4999, 64, FP, FP, False),
+    (1, 20000, 5120, 64, BF, BF, True),
+    (2, 40000, 5120, 128, BF, BF, True),
+    (4, 30720, 5120, 64, HF, HF, True),
+    (7, 250, 2049, 96, HF, FP, True),
+    (8, 3333, 4800, 160, BF, HF, True),
+    (2, 3, 16000, 128, FP, FP, True),
+    (6, 12001, 96, 96, BF, BF, False),
+    (1, 64, 30000, 16384, BF, FP, True),
+    (9, 3000, 2560, 256, FP, BF, True),
+    (16, 5000, 4096, 64, HF, HF, False),
+    (17, 2600, 10000, 512, BF, BF, True),
+    (33, 960, 3200, 64, FP, FP, True),
+])
+def test_exact_sums(cuda, rows, n, k, group, dtype, sdt, zeros):
+    _check_exact(cuda, rows, n, k, group, dtype, sdt, zeros)
