@@ -1554,13 +1554,18 @@ int launch_forward(const SprAdaln* op, cudaStream_t st) {
   }
   constexpr int P = 16 / kVec<T>;  // 16 values a thread, or 8 where that leaves fewer threads idle
   if (vec && nvec > 32 && nvec <= 512 * P && g.rows >= 8 && even_rows(g, op->batch)) {
-    // 32 values a thread from 128 threads on: fewer warps pay a row's fixed instructions,
-    // which bound the pass at the clocks of a sustained load (75,600 x 5120 bf16: 271 us
-    // with 16 values, 250 us with 32).  With a branch the vectors leave no room for that
-    // (490 and 513 us).
-    if constexpr (!kRes)
-      if (nvec % (64 * P) == 0 && nvec >= 256 * P && nvec <= 320 * P)
-        return launch_forward_stream<T, MT, false, 2 * P, true, false, 160, 3>(op, g, st);
+    // 16-bit rows of 4,096 channels and more that are whole warps of 32 values a thread take
+    // those: fewer warps pay a row's fixed instructions, which bound the pass at the clocks
+    // of a sustained load.  387 M elements of bf16, us with 16 and 32 values a thread: 1024
+    // channels 246 and 254, 2048 255 and 253, 4096 277 and 256, 5120 268 and 248, 6144 319
+    // and 254, 7168 305 and 254, 8192 303 and 251.  An fp32 row has twice the bytes for its
+    // fixed instructions: 193 M elements, 4096 channels 254 and 265, 6144 257 and 271, 8192
+    // 272 and 277.  With a branch the vectors leave no room for 32 values (75,600 x 5120 bf16:
+    // 490 and 513).
+    if constexpr (!kRes && sizeof(T) == 2)
+      if (nvec % (64 * P) == 0 && nvec >= 256 * P)
+        return nvec <= 320 * P ? launch_forward_stream<T, MT, false, 2 * P, true, false, 160, 3>(op, g, st)
+                               : launch_forward_stream<T, MT, false, 2 * P, true, false, 256, 2>(op, g, st);
     if (nvec % (32 * P) == 0)
       return nvec <= 320 * P ? launch_forward_stream<T, MT, kRes, P, true, false, 320, 2>(op, g, st)
                              : launch_forward_stream<T, MT, kRes, P, true, false, 512, 1>(op, g, st);

@@ -1,0 +1,29 @@
+"""The plain and affine norms at the widths where the rows change hands between kernels,
+against 64 bits: one rounding to the result's type (half a step), and 32 roundings of
+2^-24 on what enters it before."""
+
+import pytest
+import torch
+
+import sparsepr_b200 as spr
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("c", [2048, 4096, 4352, 5120, 5632, 6144, 7168, 8184, 8192, 8200])
+def test_norm_of_wide_rows(cuda, c, dtype):
+    g = torch.Generator(device=cuda).manual_seed(c)
+    x = (torch.randn(2, 700, c, device=cuda, generator=g) * 2 + 0.5).to(dtype)
+    shift, scale = (torch.randn(s, device=cuda, generator=g) for s in ((c,), (c,)))
+    x64 = x.double()
+    mean = x64.mean(-1, keepdim=True)
+    rstd = ((x64 - mean).square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    norm, spread = (x64 - mean) * rstd, (x64.abs() + mean.abs() + x64.abs().mean(-1, keepdim=True)) * rstd
+    for got, w in ((spr.modulated_layer_norm(x, shift, scale), 1 + scale.double()),
+                   (spr.layer_norm(x, scale, shift), scale.double())):
+        ref = norm * w + shift.double()
+        amp = (spread + norm.abs()) * w.abs() + shift.double().abs()
+        tol = torch.finfo(dtype).eps / 2 * ref.abs() + 32 * 2.0 ** -24 * amp + torch.finfo(dtype).tiny
+        assert not ((got.double() - ref).abs() > tol).any()
