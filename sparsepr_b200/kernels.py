@@ -672,7 +672,7 @@ def adaln_backward_struct(s: _lib.SprAdaln, branch: bool, dh, dz, needs, mod_sha
     dx = torch.empty_like(dh)
     dy = torch.empty_like(dh) if branch else None
     new = dh.new_empty
-    dgate = new(vector_shape, dtype=mod_dtype) if needs[0] else None
+    dgate = new(vector_shape, dtype=mod_dtype) if needs[0] and branch else None
     dshift = new(vector_shape, dtype=mod_dtype) if needs[1] else None
     dscale = new(vector_shape, dtype=mod_dtype) if needs[2] else None
     if b * n == 0:
@@ -694,7 +694,7 @@ def adaln_backward(op: AdalnOperands, stats: torch.Tensor, dh, dz=None, needs=(T
 
     ``op.x`` is the forward pass's ``z`` (its ``x`` without a branch); ``dh`` and ``dz`` (None:
     no gradient) are dense in its shape.  ``needs`` says which of (dgate, dshift, dscale) are
-    formed: [*mod_shape, channels] with ``mod_shape`` (batch or 1, tokens or 1), summed over the
+    formed (dgate only with a branch): [*mod_shape, channels] with ``mod_shape`` (batch or 1, tokens or 1), summed over the
     axes of extent 1 in a fixed order.  The workspace belongs to this call alone, so
     that calls on several streams and captured graphs share none."""
     mean = stats.data_ptr()

@@ -27,3 +27,23 @@ def test_norm_of_wide_rows(cuda, c, dtype):
         amp = (spread + norm.abs()) * w.abs() + shift.double().abs()
         tol = torch.finfo(dtype).eps / 2 * ref.abs() + 32 * 2.0 ** -24 * amp + torch.finfo(dtype).tiny
         assert not ((got.double() - ref).abs() > tol).any()
+
+
+@pytest.mark.gpu
+def test_passes_without_autograd_and_without_a_branch(cuda):
+    """The kernels' own backward call with its defaults: no gate, no gradient of one."""
+    from sparsepr_b200 import kernels as K
+    from sparsepr_b200.adaln import operands
+
+    g = torch.Generator(device=cuda).manual_seed(2)
+    x, dh = (torch.randn(2, 30, 256, device=cuda, generator=g) for _ in range(2))
+    shift, scale = (torch.randn(256, device=cuda, generator=g).requires_grad_() for _ in range(2))
+    op, mod_shape = operands(x, None, None, shift.detach(), scale.detach())
+    _z, h, stats = K.adaln_forward(op, 1e-6, True)
+    dx, dy, dgate, dshift, dscale = K.adaln_backward(op, stats, dh, mod_shape=mod_shape)
+    assert dy is None and dgate is None
+    leaf = x.clone().requires_grad_()
+    want = spr.modulated_layer_norm(leaf, shift, scale)
+    assert torch.equal(want, h)
+    for a, b in zip((dx, dshift, dscale), torch.autograd.grad(want, (leaf, shift, scale), dh)):
+        assert torch.equal(a.reshape(b.shape), b)
