@@ -455,10 +455,12 @@ int spr_adaln_backward(const SprAdaln* op, const SprAdalnGrad* grad, void* works
  * y[r][n] = sum_k x[r][k] * (code[n][k] - zero[n][k/group]) * scale[n][k/group] + bias[n]
  * for a few rows r (a conditioning vector per sample).  packed [n][groups*group/2]
  * u8: two codes (0..15) per byte, the even column in the low half; scales
- * [n][groups] (scale_dtype); zeros [n][groups] u8 (0..15; nullable: 8); bias [n]
- * (dtype, nullable).  groups = ceil(k/group), group a multiple of 32; codes of
- * columns >= k are ignored.  x [rows][k] (row stride x_stride elements), y
- * [rows][n] dense, both `dtype`; sums in fp32, one rounding.  packed must be
+ * [n][groups] (scale_dtype); zeros [n][groups] u8 (nullable: 8; 0..15, larger ones
+ * give meaningless sums); bias [n] (dtype, nullable).  groups = ceil(k/group), group
+ * a multiple of 32; codes of columns >= k are ignored.  x [rows][k] (row stride
+ * x_stride elements), y [rows][n] dense, both `dtype`; sums in fp32, one rounding (up
+ * to eight 16-bit rows as integers: an entry below 2^-22 of its row's largest keeps
+ * fewer than 8 bits, below 2^-31 none).  packed must be
  * 16-byte aligned, the other operands begin on their elements.  workspace:
  * spr_int4_linear_workspace_bytes (0 is possible, and the answer for sizes that the
  * call refuses).  At most 2^31 - 1 rows and outputs, 2^27 columns and groups of 2^20;

@@ -5,8 +5,8 @@
 * :func:`gated_residual_layer_norm` — ``z = x + gate * y`` and the modulated norm of
   ``z`` in one pass, returning both.
 
-``x`` and ``y`` are [..., C] CUDA tensors in fp32, bf16 or fp16 (C <= 16384, the
-channels contiguous, the axes before them in any order of strides that
+``x`` and ``y`` are [..., C] CUDA tensors in fp32, bf16 or fp16 (C <= 16384, fewer than
+2^31 rows, the channels contiguous, the axes before them in any order of strides that
 ``Tensor.view`` can merge).  ``weight``, ``bias``, ``shift``, ``scale`` and ``gate`` are of
 one type, x's or fp32, and of one shape: [C], or x's shape with some of the
 leading axes of extent 1, where the axes kept and the axes broadcast are each

@@ -12,18 +12,22 @@
 //   product.  An inner sum is an exact integer.  A value far below the largest is
 //   rounded at 2^-30 of it: beside the largest's own term less than an fp32 sum
 //   rounds, and where that term is 0 small values still have bf16's 8 bits down to
-//   2^-22 of it.
+//   2^-22 of it; below 2^-31 it is lost.
 // * fp32 x, and more rows than the integer columns hold: bf16 products (m16n8k16).  A
 //   code is the exact integer code - zero, and x is cut into as many bf16 parts as
 //   its significand needs (bf16 1, fp16 2, fp32 3; exact), each a column.
-// Measured on B200 (copy bandwidth 6.56 TB/s), 245,760 x 5120 codes: two bf16 rows,
-// groups of 128 137 us (73% of the copy's bytes a second), one row, groups of 64 151 us;
-// the schedulers issue in 55% to 60% of all cycles, waiting for one another's
-// products.  fp32 rows (three parts) 122,880 x 5120, groups of 64: 113 us.  The gradient
-// has more to do a code (pairs of weight rows are formed, and the other operand for each
-// group): 122,880 x 5120 two rows, groups of 128 198 us; 30,720 x 5120 four rows 72 us.
-// The 5th-generation tensor instructions work on 128 rows: with so few, they would
-// idle, and their operands would pass through shared memory again once unpacked.
+// Measured on B200 (copy bandwidth 6.56 TB/s) under a sustained load, 245,760 x 5120
+// codes: two bf16 rows, groups of 128 133 us (75% of the copy's bytes a second), one row,
+// groups of 64 150 us (70%); the schedulers issue in 55% to 60% of all cycles, waiting
+// for one another's products.  122,880 x 5120 codes: 9, 16 and 32 bf16 rows, groups of
+// 128, 129, 145 and 301 us; one, two and three fp32 rows (three parts each), groups of 64,
+// 109, 115 and 149 us.  The gradient has more to do a code (pairs of weight rows are
+// formed, and the other operand for each group): two rows, groups of 128 200 us; 30,720 x
+// 5120 four rows 75 us.
+// The 5th-generation tensor instructions would take 128 weight rows a tile, from shared or
+// tensor memory: the codes, once unpacked, would have to be written there, two to four
+// times the bytes that were copied in.  Whether larger tiles win back those instructions
+// was not measured.
 #include <math.h>
 
 #include <initializer_list>

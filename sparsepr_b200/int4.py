@@ -21,7 +21,8 @@ __all__ = ["Int4Weight", "quantize_int4", "dequantize_int4", "int4_linear"]
 
 class Int4Weight(NamedTuple):
     """``packed`` uint8 [N, groups*group/2] (two codes a byte, the even column in the low
-    half), ``scales`` [N, groups], ``zeros`` uint8 [N, groups], 0 to 15, or None (8)."""
+    half), ``scales`` [N, groups], ``zeros`` uint8 [N, groups], or None (8).  Zero codes are 0
+    to 15; larger ones are not looked for and give meaningless products."""
 
     packed: torch.Tensor
     scales: torch.Tensor
@@ -105,8 +106,12 @@ def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zer
                 bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ W.T + bias`` with the 4-bit weight ``W`` [N, K] of :func:`quantize_int4`.
 
-    ``x`` [..., K] in fp32, bf16 or fp16 and ``bias`` [N] in x's type; the result [..., N]
-    is rounded once from fp32 sums.  Any number of rows is computed, but the
+    ``x`` [..., K] in fp32, bf16 or fp16 and ``bias`` [N] in x's type; ``packed`` begins on 16
+    bytes; the result [..., N] is rounded once from fp32 sums.  Up to eight 16-bit rows are
+    multiplied as integers of 31 bits relative to each row's largest value (of up to all its
+    columns): entries keep bf16's 8 bits down to 2^-22 of that value and are lost below
+    2^-31, which shows only where the codes opposite the larger values are zero; cast ``x``
+    to fp32 to keep every entry whole.  Any number of rows is computed, but the
     weights are read again for every 8 to 32 rows: the call is for a few rows.  Gradients
     are of first order, in reverse mode (dual tensors are refused).  A backward pass captured
     into a CUDA graph needs what any captured autograd call needs: no graph of an uncaptured
