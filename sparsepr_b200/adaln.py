@@ -125,13 +125,25 @@ def operands(x, y, gate, shift, scale, scale_offset: float = 1.0):
     return op, (mb, mn)
 
 
-_SAVED = ("x", "y", "gate", "scale")
+def _saved(s, name, t, dtype, b, n, index):
+    """Point operand ``name`` of ``s`` at a saved tensor, which hooks may have given back in another layout."""
+    K.check_saved(t, dtype, b * n * s.channels, index)
+    if t.is_contiguous():
+        sb, st = (n * s.channels if b > 1 else 0), (s.channels if n > 1 else 0)
+    else:
+        try:
+            sb, st = _strides(t, b, n, name)
+        except RuntimeError:
+            return _saved(s, name, t.contiguous(), dtype, b, n, index)
+    setattr(s, name, t.data_ptr())
+    setattr(s, name + "_sb", sb)
+    setattr(s, name + "_st", st)
+    return t
 
 
 def _backward(ctx, *grads):
-    # Saved-tensor hooks may give back another layout, but not other values' places or types.
-    x, y, gate, scale, stats = saved = [K.as_saved(t, meta) for t, meta in zip(ctx.saved_tensors, ctx.saved_meta)]
-    K.refuse_tangents("layer norm gradient", x, y, gate, scale, *grads)
+    K.refuse_tangents("layer norm gradient", *grads)
+    x, y, gate, scale, stats = ctx.saved_tensors
     dz, dh = grads if y is not None else (None, grads[0])
     if dh is None:
         if dz is None:
@@ -143,19 +155,14 @@ def _backward(ctx, *grads):
         dz = dz.contiguous()
     s, mod_shape, vector_shape, mod_dtype = ctx.operands
     s = type(s).from_buffer_copy(s)
-    s.x = x.data_ptr()
-    if y is not None:  # the norm's input is z, which is dense
-        s.y, s.x_sb, s.x_st = y.data_ptr(), s.tokens * s.channels, s.channels
-    s.gate = None if gate is None else gate.data_ptr()
-    s.scale = None if scale is None else scale.data_ptr()
-    for name, t, meta in zip(_SAVED, saved, ctx.saved_meta):
-        if t is not None and t.stride() != meta[1]:
-            b, n = (s.batch, s.tokens) if name in ("x", "y") else mod_shape
-            sb, st = _strides(t, b, n, name)
-            setattr(s, name + "_sb", sb)
-            setattr(s, name + "_st", st)
+    b, n, index = s.batch, s.tokens, dh.get_device()
+    x = _saved(s, "x", x, dh.dtype, b, n, index)  # z, where there is a branch
+    y = y if y is None else _saved(s, "y", y, dh.dtype, b, n, index)
+    gate = gate if gate is None else _saved(s, "gate", gate, mod_dtype, *mod_shape, index)
+    scale = scale if scale is None else _saved(s, "scale", scale, mod_dtype, *mod_shape, index)
+    stats = K.dense_saved(stats, torch.float32, 2 * b * n, index)
     mean = stats.data_ptr()
-    s.mean, s.rstd = mean, mean + 4 * stats.shape[1]
+    s.mean, s.rstd = mean, mean + 4 * b * n
     grads = K.adaln_backward_struct(s, y is not None, dh, dz, ctx.needs_input_grad[2:5], mod_shape, vector_shape,
                                     mod_dtype)
     return *grads, None, None
@@ -169,9 +176,7 @@ class _AdaLN(torch.autograd.Function):
     def forward(ctx, x, y, gate, shift, scale, eps, scale_offset):
         op, mod_shape = operands(x, y, gate, shift, scale, scale_offset)
         z, h, stats, struct = K.adaln_forward_struct(op, eps, True)
-        saved = x if z is None else z, y, gate, scale, stats
-        ctx.save_for_backward(*saved)
-        ctx.saved_meta = [K.saved_meta(t) for t in saved]
+        ctx.save_for_backward(x if z is None else z, y, gate, scale, stats)
         ctx.set_materialize_grads(False)
         vector = gate if gate is not None else shift if shift is not None else scale
         ctx.operands = struct, mod_shape, None if vector is None else vector.shape, op.mod_dtype

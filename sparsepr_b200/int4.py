@@ -72,14 +72,18 @@ def dequantize_int4(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Ten
 
 
 def _backward(ctx, dy):
-    packed, scales, zeros = (K.as_saved(t, meta) for t, meta in zip(ctx.saved_tensors, ctx.saved_meta))
     K.refuse_tangents("int4_linear gradient", dy)
+    packed, scales, zeros = ctx.saved_tensors
+    (n, half), groups, scale_dtype = ctx.weight
+    index = dy.get_device()
+    packed = K.dense_saved(packed, torch.uint8, n * half, index)
+    scales = K.dense_saved(scales, scale_dtype, n * groups, index)
+    zeros = zeros if zeros is None else K.dense_saved(zeros, torch.uint8, n * groups, index)
     dx = dbias = None
     if dy.stride(1) != 1 or (dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]):
         dy = dy.contiguous()
     if ctx.needs_input_grad[0]:
-        n, groups = scales.shape
-        dx = K.int4_linear_grad_checked(dy, packed, scales, zeros, ctx.in_features, n, 2 * packed.shape[1] // groups)
+        dx = K.int4_linear_grad_checked(dy, packed, scales, zeros, ctx.in_features, n, 2 * half // groups)
     if ctx.needs_input_grad[4]:
         dbias = dy.sum(0)  # 16-bit sums are fp32 inside and rounded once
     return dx, None, None, None, dbias
@@ -92,9 +96,9 @@ class _Int4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, packed, scales, zeros, bias):
         ctx.save_for_backward(packed, scales, zeros)
-        ctx.saved_meta = [K.saved_meta(t) for t in (packed, scales, zeros)]
-        ctx.in_features = x.shape[1]
-        return K.int4_linear(x, packed, scales, zeros, bias)
+        y = K.int4_linear(x, packed, scales, zeros, bias)
+        ctx.in_features, ctx.weight = x.shape[1], (packed.shape, scales.shape[1], scales.dtype)
+        return y
 
     @staticmethod
     def backward(ctx, dy):

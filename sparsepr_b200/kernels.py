@@ -595,21 +595,19 @@ def refuse_tangents(what: str, *tensors) -> None:
                 raise RuntimeError(f"{what}: forward-mode derivatives are not supported")
 
 
-def saved_meta(t):
-    """What :func:`as_saved` compares a saved operand with."""
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+def check_saved(t: torch.Tensor, dtype: torch.dtype, numel: int, index: int) -> torch.Tensor:
+    """A saved operand as a backward pass may read it, by its own layout.  Saved-tensor hooks give back what they
+    like: other sizes, types and devices than those saved are refused."""
+    if t.dtype != dtype or t.numel() != numel or t.get_device() != index:
+        raise RuntimeError(f"a saved operand came back as {tuple(t.shape)} {t.dtype} on {t.device}; it had {numel} "
+                           f"values of {dtype} on cuda:{index}")
+    return t
 
 
-def as_saved(t, meta):
-    """A saved operand as a backward pass may read it.  Saved-tensor hooks give back what they
-    like: a layout other than the saved one becomes dense, another shape, type or device is refused."""
-    if t is None:
-        return None
-    shape, strides, dtype, index = meta
-    if t.dtype != dtype or t.shape != shape or t.get_device() != index:
-        raise RuntimeError(f"a saved operand came back as {tuple(t.shape)} {t.dtype} on {t.device}; it was "
-                           f"{tuple(shape)} {dtype} on cuda:{index}")
-    return t if t.stride() == strides else t.contiguous()
+def dense_saved(t: torch.Tensor, dtype: torch.dtype, numel: int, index: int) -> torch.Tensor:
+    """:func:`check_saved` of an operand that the kernels read densely."""
+    check_saved(t, dtype, numel, index)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class AdalnOperands(NamedTuple):

@@ -41,15 +41,16 @@ def _int4(dev):
     return lambda: torch.autograd.grad(spr.int4_linear(x, *w), x, dy)
 
 
-def test_metadata_of_a_saved_operand():
+def test_checks_of_a_saved_operand():
     t = torch.arange(12.0).view(3, 4)
-    meta = K.saved_meta(t)
-    assert K.as_saved(t, meta) is t and K.as_saved(None, None) is None
-    back = K.as_saved(_turned(t), meta)
+    assert K.check_saved(_turned(t), FP, 12, -1) is not None
+    assert K.dense_saved(t, FP, 12, -1) is t
+    back = K.dense_saved(_turned(t), FP, 12, -1)
     assert back.is_contiguous() and torch.equal(back, t)
-    for other in (t.double(), t.view(4, 3), t[:2], t.view(torch.int32)):
-        with pytest.raises(RuntimeError, match="came back as"):
-            K.as_saved(other, meta)
+    for other, index in ((t.double(), -1), (t[:2], -1), (t.view(torch.int32), -1), (t, 0)):
+        for f in (K.check_saved, K.dense_saved):
+            with pytest.raises(RuntimeError, match="came back as"):
+                f(other, FP, 12, index)
 
 
 @pytest.mark.gpu
