@@ -1568,11 +1568,16 @@ int launch_forward(const SprAdaln* op, cudaStream_t st) {
     // and 254, 7168 305 and 254, 8192 303 and 251.  An fp32 row has twice the bytes for its
     // fixed instructions: 193 M elements, 4096 channels 254 and 265, 6144 257 and 271, 8192
     // 272 and 277.  With a branch the vectors leave no room for 32 values (75,600 x 5120 bf16:
-    // 490 and 513).
-    if constexpr (!kRes && sizeof(T) == 2)
-      if (nvec % (64 * P) == 0 && nvec >= 256 * P)
-        return nvec <= 320 * P ? launch_forward_stream<T, MT, false, 2 * P, true, false, 160, 3>(op, g, st)
-                               : launch_forward_stream<T, MT, false, 2 * P, true, false, 256, 2>(op, g, st);
+    // 490 and 513).  Few rows are bound by the time of one, which more threads shorten: up to
+    // six rows for each CTA of the 16-value form that an SM holds (two, above 5,120 channels
+    // one).  600 rows of 5120 6.4 and 7.0, 1,200 7.5 and 8.0, 2,400 10.9 and 10.4; 740 rows of
+    // 6144 6.3 and 7.3, 900 7.6 and 7.3, 2,400 18.0 and 12.4.
+    if constexpr (!kRes && sizeof(T) == 2) {
+      const bool wide = nvec > 320 * P;
+      if (nvec % (64 * P) == 0 && nvec >= 256 * P && g.count * g.rows >= (wide ? 6 : 12) * (int64_t)sm_count())
+        return wide ? launch_forward_stream<T, MT, false, 2 * P, true, false, 256, 2>(op, g, st)
+                    : launch_forward_stream<T, MT, false, 2 * P, true, false, 160, 3>(op, g, st);
+    }
     if (nvec % (32 * P) == 0)
       return nvec <= 320 * P ? launch_forward_stream<T, MT, kRes, P, true, false, 320, 2>(op, g, st)
                              : launch_forward_stream<T, MT, kRes, P, true, false, 512, 1>(op, g, st);

@@ -12,10 +12,11 @@ BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("n", [300, 1000])
 @pytest.mark.parametrize("c", [2048, 4096, 4352, 5120, 5632, 6144, 7168, 8184, 8192, 8200])
-def test_norm_of_wide_rows(cuda, c, dtype):
+def test_norm_of_wide_rows(cuda, c, n, dtype):
     g = torch.Generator(device=cuda).manual_seed(c)
-    x = (torch.randn(2, 700, c, device=cuda, generator=g) * 2 + 0.5).to(dtype)
+    x = (torch.randn(2, n, c, device=cuda, generator=g) * 2 + 0.5).to(dtype)
     shift, scale = (torch.randn(s, device=cuda, generator=g) for s in ((c,), (c,)))
     x64 = x.double()
     mean = x64.mean(-1, keepdim=True)
